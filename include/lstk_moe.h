@@ -159,6 +159,35 @@ int lstk_pool_describe(const lstk_pool *pool, char *buf, size_t len);
 int lstk_moe_route(lstk_pool *pool, int layer, const float *d_hnorm, int n_tokens, const void *d_gate_inp,
                    int gate_type, int32_t *d_ids, float *d_weights, lstk_stream_t stream);
 
+/* Routing by a rule, for routers other than softmax + top-k (no counterpart in the reference, whose models have one rule).
+ * Per token, with x the router logits (NaN counts as -inf, +inf as the largest float):
+ *   s = softmax(x) or 1 / (1 + e^-x);  c = s + bias (choice values; a NaN counts as -inf);
+ *   the experts form n_group runs of n_expert / n_group; a group's value is the sum of its group_top largest c; the
+ *   n_group_used best groups stay (equal values: the lower group);
+ *   of their experts the n_expert_used largest c are chosen (equal values: the lower id), written in that order;
+ *   weight = s (without bias), divided by max(sum of the chosen s, 2^-14) if renorm, times scale.
+ * A token whose logits are all -inf has softmax scores 0. Scores and choice values are held in 64 bits. */
+#define LSTK_SCORE_SOFTMAX 0
+#define LSTK_SCORE_SIGMOID 1
+typedef struct lstk_router_rule {
+    int32_t score;        /* LSTK_SCORE_SOFTMAX or LSTK_SCORE_SIGMOID */
+    int32_t n_group;      /* 1: no groups; divides n_expert */
+    int32_t n_group_used; /* groups that stay, in [1, n_group] */
+    int32_t group_top;    /* 1 or 2 */
+    int32_t renorm;       /* 0 or 1 */
+    float scale;
+} lstk_router_rule;
+
+/* The rule on given logits: row t at d_logits + t * ld_logits, d_bias [n_expert] f32 or NULL, d_ids and d_weights
+ * [n_tokens][n_expert_used]. n_expert <= 256, n_expert_used <= 64, n_tokens <= 2^24; allocates nothing, keeps no state. */
+int lstk_moe_select(const lstk_router_rule *rule, const float *d_logits, int64_t ld_logits, const float *d_bias, int n_tokens,
+                    int n_expert, int n_expert_used, int32_t *d_ids, float *d_weights, lstk_stream_t stream);
+/* lstk_moe_route by a rule: logits = gate_inp . hnorm as there, then lstk_moe_select. Its ids and weights go to
+ * lstk_moe_ffn (through lstk_pool_acquire for a streaming pool). */
+int lstk_moe_route_by(lstk_pool *pool, int layer, const lstk_router_rule *rule, const float *d_hnorm, int n_tokens,
+                      const void *d_gate_inp, int gate_type, const float *d_bias, int32_t *d_ids, float *d_weights,
+                      lstk_stream_t stream);
+
 /* moe_apply() + the residual add (src/qwen3.cpp:197-214 and :250 / :287) on the device:
  * out[t] = resid[t] + sum_{j=0..k-1} weights[t][j] * down_s(swiglu(gate_s(x_t), up_s(x_t))),
  * s = d_slots[t][j], summed left to right in j. x_t is quantized to the activation type ggml pairs with

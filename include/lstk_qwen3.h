@@ -109,6 +109,74 @@ int lstk_model_prepare(lstk_model *model, int32_t seq, const int32_t *tokens, in
 int lstk_model_forward(lstk_model *model, int32_t seq, int n_tokens, int32_t n_cells, float *d_logits,
                        int32_t *d_trace, lstk_stream_t stream);
 
+/* One new token for each of n_seq distinct sequences in one step (no counterpart in the reference, whose steps take one
+ * sequence): appends tokens[i] to sequence seqs[i] and writes the logits of every row, [n_seq][n_vocab] f32, to d_logits.
+ * 1 <= n_seq <= n_batch. With window > 0 each token attends its sequence's last `window` cells and first n_sink cells, else
+ * all of them (lstk_attn_paged); prompts run through lstk_model_decode attend everything. d_trace, when not NULL, receives the
+ * router's ids [n_layer][n_seq][n_expert_used]; a trace file (lstk_model_set_trace) gets the step like any other.
+ * Nothing is appended when the arguments are rejected or the cache has no room for all of them. */
+int lstk_model_decode_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int window, int n_sink,
+                            float *d_logits, int32_t *d_trace, lstk_stream_t stream);
+/* The same in two halves, like lstk_model_prepare / lstk_model_forward. prepare_batch returns the longest sequence's cells in
+ * *max_len. forward_batch takes the step last prepared (n_seq as there) and any max_len that holds its sequences; captured,
+ * it replays correctly after each later prepare_batch of n_seq sequences, whichever they are, none longer than max_len. */
+int lstk_model_prepare_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int32_t *max_len,
+                             lstk_stream_t stream);
+int lstk_model_forward_batch(lstk_model *model, int n_seq, int32_t max_len, int window, int n_sink, float *d_logits,
+                             int32_t *d_trace, lstk_stream_t stream);
+
+/* Attention of one new token per sequence over one layer's paged cache, on caller-owned device memory (the model's batch
+ * step runs it on its own cache):
+ *   out[b][h] = sum_i softmax_i(scale q[b][h] . k[i][h / (n_head / n_head_kv)]) v[i][..]   over the visible cells i of row b
+ * K is [n_head_kv][head_dim / 4][kv_size][4] fp16 (4 dims of a cell together, cells side by side), V
+ * [n_head_kv][kv_size / 4][head_dim][4] (4 cells of a dim together); head_dim 64, 128 or 256, kv_size a multiple of 32.
+ * Pages are runs of 32 cells: logical cell i of row b is cell d_blocks[d_first[b] + i / 32] * 32 + i % 32, 0 <= i < d_len[b];
+ * rows may share pages. Visible are the cells i < min(d_len[b], max_len), of them with window > 0 only the last `window` and
+ * the first n_sink (counted in cells the row holds). A page whose table index (outside [0, n_table)) or block number (outside the cache) is out of range is
+ * not visible; with d_cell_seq [kv_size] and d_seq [n_seq] given (both or neither), nor is a cell whose d_cell_seq entry is
+ * not d_seq[b]. What the cache holds in cells that are not visible is never used, whatever it is; a row with no visible cell
+ * gets zeros. */
+typedef struct lstk_paged_cache {
+    const uint16_t *d_k, *d_v;
+    int64_t kv_size;
+    int32_t n_head_kv, head_dim;
+    const int32_t *d_cell_seq; /* or NULL */
+} lstk_paged_cache;
+typedef struct lstk_paged_seqs {
+    int32_t n_seq;
+    int32_t max_len;         /* bound of the lengths: sizes the launch and the workspace */
+    const int32_t *d_len;    /* [n_seq] */
+    const int32_t *d_first;  /* [n_seq] index of a row's first page in d_blocks */
+    const int32_t *d_blocks; /* [n_table] block numbers */
+    int32_t n_table;
+    const int32_t *d_seq;    /* [n_seq] or NULL */
+} lstk_paged_seqs;
+/* d_q and d_out are [n_seq][n_head][head_dim] fp16; d_work holds at least lstk_attn_paged_work_bytes (0 for shapes that need
+ * none or are rejected; what serves one max_len serves smaller ones) and belongs to one call at a time: calls that may overlap, captured ones among them, take one each.
+ * Results do not depend on what else runs and repeat bit for bit. */
+size_t lstk_attn_paged_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink);
+int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head, int window,
+                    int n_sink, float scale, uint16_t *d_out, void *d_work, size_t work_bytes, lstk_stream_t stream);
+
+/* The next token of each row of logits (the reference's Sampler works on host logits, src/sampler.cpp:20-82; its repeat
+ * penalty is not part of this). Per row, with the values in descending order (equal values: the lower index first; NaN counts
+ * as -inf, +inf as the largest float) and w = e^((x - x_max) / temperature):
+ *   the first top_k values stay (<= 0: all), of those the ones with w >= min_p (<= 0: all; the largest always);
+ *   of those the shortest run from the top that holds top_p of their sum (>= 1: all; the largest always);
+ *   the token is the first whose running sum exceeds u times the sum of what stays, u in [0, 1); its probability is w over
+ *   that sum. temperature <= 0 or NaN: the largest value, probability 1.
+ * A row with nothing above -inf gives token -1 and probability 0. The four setting arrays are on the device, [n_rows] each;
+ * a NULL one means temperature 1 / no cut; a NaN top_p or min_p means no cut. Row r of the logits is at
+ * d_logits + r * ld_logits; n_vocab < 2^20. d_probs may be NULL. The workspace is as lstk_attn_paged's. */
+typedef struct lstk_sampling {
+    const float *d_temperature;
+    const int32_t *d_top_k;
+    const float *d_top_p, *d_min_p;
+} lstk_sampling;
+size_t lstk_sample_work_bytes(int n_rows, int n_vocab);
+int lstk_sample(const float *d_logits, int64_t ld_logits, int n_rows, int n_vocab, const lstk_sampling *how, const float *d_u,
+                int32_t *d_tokens, float *d_probs, void *d_work, size_t work_bytes, lstk_stream_t stream);
+
 /* KvCache::remove_seq / truncate_seq / length (src/kv_cache.cpp:97-150, src/engine.h:75-80). */
 int lstk_model_remove_seq(lstk_model *model, int32_t seq);
 int lstk_model_truncate_seq(lstk_model *model, int32_t seq, int32_t keep);

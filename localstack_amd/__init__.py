@@ -10,7 +10,9 @@ ctypes view of that ABI that mirrors the reference's interface for the path:
   ExpertStore.block    the resident MoE block of qwen3_build_graph (src/qwen3.cpp:239-250)
   Qwen3Model           the forward pass around it (include/lstk_qwen3.h): Engine::decode
                        (src/engine.cpp:250-278) over qwen3_build_graph (src/qwen3.cpp:223-259)
-                       with the KvCache block table (src/kv_cache.cpp:59-150)
+                       with the KvCache block table (src/kv_cache.cpp:59-150); decode_batch and generate
+                       step many sequences at once
+  paged_attention, sample, moe_select   the operators of such a step on plain tensors
 
 Device buffers are torch tensors on a ROCm device (or raw integer device pointers); torch is used
 only to own device memory and streams. There is no CPU fallback: every compute call runs the HIP
@@ -27,6 +29,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # LSTK_LIBRARY names another build of the library (the sanitizer build of the CPU tests)
 LIB_PATH = os.environ.get("LSTK_LIBRARY") or os.path.join(HERE, "liblstk_moe.so")
 
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K = 0, 1, 8, 12
 POOL_STREAMING, POOL_DRY, POOL_DEVICE_LRU, POOL_AUTO_SIZE = 1, 2, 4, 8
 E_INVALID, E_NOMEM, E_EXHAUSTED, E_DEVICE, E_IO, E_BADID = -1, -2, -3, -4, -5, -6
@@ -73,6 +76,26 @@ class Qwen3Layer(ctypes.Structure):
 class Qwen3Weights(ctypes.Structure):
     _fields_ = [("tok_embd", ctypes.c_void_p), ("output_norm", ctypes.c_void_p), ("output", ctypes.c_void_p),
                 ("layers", ctypes.c_void_p)]
+
+
+class CRouterRule(ctypes.Structure):
+    _fields_ = [("score", ctypes.c_int32), ("n_group", ctypes.c_int32), ("n_group_used", ctypes.c_int32),
+                ("group_top", ctypes.c_int32), ("renorm", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [("d_k", ctypes.c_void_p), ("d_v", ctypes.c_void_p), ("kv_size", ctypes.c_int64),
+                ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("d_cell_seq", ctypes.c_void_p)]
+
+
+class PagedSeqs(ctypes.Structure):
+    _fields_ = [("n_seq", ctypes.c_int32), ("max_len", ctypes.c_int32), ("d_len", ctypes.c_void_p),
+                ("d_first", ctypes.c_void_p), ("d_blocks", ctypes.c_void_p), ("n_table", ctypes.c_int32),
+                ("d_seq", ctypes.c_void_p)]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_temperature", "d_top_k", "d_top_p", "d_min_p")]
 
 
 # name -> (restype, argtypes); every function declared in include/lstk_moe.h and include/lstk_qwen3.h
@@ -132,6 +155,16 @@ SIGNATURES = {
     "lstk_gguf_qwen3_experts": (_I, [_P, ctypes.POINTER(Qwen3HParams), _P]),
     "lstk_dequant_f16": (_I, [_I, _P, ctypes.c_size_t, _P]),
     "lstk_model_set_timing": (_I, [_P, _I]),
+    "lstk_moe_select": (_I, [ctypes.POINTER(CRouterRule), _P, ctypes.c_int64, _P, _I, _I, _I, _P, _P, _P]),
+    "lstk_moe_route_by": (_I, [_P, _I, ctypes.POINTER(CRouterRule), _P, _I, _P, _I, _P, _P, _P, _P]),
+    "lstk_attn_paged_work_bytes": (_SZ, [_I] * 7),
+    "lstk_attn_paged": (_I, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedSeqs), _P, _I, _I, _I, ctypes.c_float, _P, _P, _SZ,
+                             _P]),
+    "lstk_sample_work_bytes": (_SZ, [_I, _I]),
+    "lstk_sample": (_I, [_P, ctypes.c_int64, _I, _I, ctypes.POINTER(Sampling), _P, _P, _P, _P, _SZ, _P]),
+    "lstk_model_decode_batch": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "lstk_model_prepare_batch": (_I, [_P, _I, _P, _P, ctypes.POINTER(ctypes.c_int32), _P]),
+    "lstk_model_forward_batch": (_I, [_P, _I, ctypes.c_int32, _I, _I, _P, _P, _P]),
     "lstk_debug_attn_plan": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "lstk_debug_attn_split": (_I, [_I, _I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(ctypes.c_int32)]),
     "lstk_debug_moe_plan": (_I, [ctypes.POINTER(MoeDims), _I, _I, _I, _I, _P]),
@@ -250,6 +283,157 @@ def unpack_matrix(type_, rows, cols, packed):
     return out
 
 
+# ---- operators of a step over many sequences -------------------------------------------------------
+
+def _tensor(t, name, dtype, shape, like=None):
+    """Checks a device tensor's dtype, shape (None: any size), layout (rows one after the other) and device."""
+    if not hasattr(t, "data_ptr") or t.dtype != dtype or t.dim() != len(shape) or \
+            any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        want = "x".join("n" if w is None else str(w) for w in shape)
+        raise LstkError(E_INVALID, f"{name} must be a {dtype} tensor of shape {want}, got "
+                                   f"{getattr(t, 'dtype', type(t))} {tuple(getattr(t, 'shape', ()))}")
+    if not t.is_contiguous():
+        raise LstkError(E_INVALID, f"{name} must be contiguous")
+    if not t.is_cuda or (like is not None and t.device != like.device):
+        raise LstkError(E_INVALID, f"{name} is on {t.device}" + ("" if like is None else f", not on {like.device}"))
+    return t.data_ptr()
+
+
+def _rows(t, name, dtype):
+    """A 2-D device tensor whose rows are contiguous: (pointer, row stride)."""
+    if not hasattr(t, "data_ptr") or t.dtype != dtype or t.dim() != 2:
+        raise LstkError(E_INVALID, f"{name} must be a 2-D {dtype} tensor")
+    if not t.is_cuda:
+        raise LstkError(E_INVALID, f"{name} is on {t.device}")
+    n, m = t.shape
+    if (m > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < m):
+        raise LstkError(E_INVALID, f"{name} must have contiguous rows that do not overlap")
+    return t.data_ptr(), t.stride(0) if n > 1 else m
+
+
+class _Call:
+    """The device and stream of a call on tensors: the tensors' device is current inside, and a workspace made for the call
+    stays until the stream is done with it."""
+
+    def __init__(self, like, stream):
+        import torch
+        self._torch, self._device, self._given = torch, like.device, stream
+        self._guard = None
+
+    def __enter__(self):
+        if self._torch.cuda.current_device() != self._device.index:
+            self._guard = self._torch.cuda.device(self._device)
+            self._guard.__enter__()
+        self.stream = _stream(self._given)
+        return self
+
+    def __exit__(self, *a):
+        if self._guard is not None:
+            self._guard.__exit__(*a)
+
+    def work(self, given, nbytes):
+        """(pointer, bytes) of the caller's workspace, or of a new one."""
+        if given is None:
+            given = self._torch.empty(nbytes, dtype=self._torch.uint8, device=self._device)
+            if self._given is not None:
+                s = self._given
+                given.record_stream(self._torch.cuda.ExternalStream(s, device=self._device) if isinstance(s, int) else s)
+        elif given.device != self._device or not given.is_contiguous():
+            raise LstkError(E_INVALID, f"work must be a contiguous tensor on {self._device}")
+        self._work = given
+        return given.data_ptr(), given.numel() * given.element_size()
+
+
+class RouterRule:
+    """How a router chooses experts from its logits (lstk_router_rule, include/lstk_moe.h): score "softmax" or "sigmoid";
+    n_group groups of which the n_group_used with the largest sum of their group_top best choice values stay; weights divided
+    by their sum (renorm) and scaled."""
+
+    def __init__(self, score="softmax", n_group=1, n_group_used=None, group_top=1, renorm=True, scale=1.0):
+        if score not in ("softmax", "sigmoid"):
+            raise LstkError(E_INVALID, f"unknown score function {score!r}")
+        self.c = CRouterRule(SCORE_SIGMOID if score == "sigmoid" else SCORE_SOFTMAX, int(n_group),
+                             int(n_group if n_group_used is None else n_group_used), int(group_top), 1 if renorm else 0, float(scale))
+
+
+def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, stream=None):
+    """The experts a rule chooses from router logits [T][n_expert] (f32, rows may be strided): (ids int32, weights f32), each
+    [T][n_expert_used], in descending order of choice. bias: f32 [n_expert], added to the scores for the choice only."""
+    import torch
+    p, ld = _rows(logits, "logits", torch.float32)
+    T, E = logits.shape
+    b = None if bias is None else _tensor(bias, "bias", torch.float32, (E,), logits)
+    k = int(n_expert_used)
+    if ids is None:
+        ids = torch.empty(T, max(k, 0), dtype=torch.int32, device=logits.device)
+    if weights is None:
+        weights = torch.empty(T, max(k, 0), dtype=torch.float32, device=logits.device)
+    with _Call(logits, stream) as c:
+        _check(lib().lstk_moe_select(ctypes.byref(rule.c), p, ld, b, T, E, k, _tensor(ids, "ids", torch.int32, (T, k), logits),
+                                     _tensor(weights, "weights", torch.float32, (T, k), logits), c.stream))
+    return ids, weights
+
+
+def paged_attention_work_bytes(n_seq, n_head, n_head_kv, head_dim, max_len, window=0, n_sink=0):
+    return lib().lstk_attn_paged_work_bytes(int(n_seq), int(n_head), int(n_head_kv), int(head_dim), int(max_len), int(window),
+                                            int(n_sink))
+
+
+def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0, n_sink=0, scale=None, cell_seq=None, seqs=None,
+                    out=None, work=None, stream=None):
+    """Attention of one new token per sequence over a paged cache (lstk_attn_paged, include/lstk_qwen3.h).
+
+    q: fp16 [n_seq][n_head][head_dim]. k_cache: fp16 [n_head_kv][head_dim / 4][kv_size][4], v_cache: fp16
+    [n_head_kv][kv_size / 4][head_dim][4]. lens, first: int32 [n_seq]; blocks: int32, the 32-cell block numbers of row b from
+    first[b] on. max_len bounds the lengths (it sizes the launch). window > 0: only the last `window` cells and the first
+    n_sink. cell_seq (int32 [kv_size]) with seqs (int32 [n_seq]): cells of other owners are not visible. Returns out, like q."""
+    import torch
+    n, H, hd = q.shape if q.dim() == 3 else (0, 0, 0)
+    qp = _tensor(q, "q", torch.float16, (None, None, None))
+    kv, _, size, _ = k_cache.shape if k_cache.dim() == 4 else (0, 0, 0, 0)
+    cache = PagedCache(_tensor(k_cache, "k_cache", torch.float16, (None, hd // 4, None, 4), q),
+                       _tensor(v_cache, "v_cache", torch.float16, (kv, size // 4, hd, 4), q), size, kv, hd,
+                       None if cell_seq is None else _tensor(cell_seq, "cell_seq", torch.int32, (size,), q))
+    s = PagedSeqs(n, int(max_len), _tensor(lens, "lens", torch.int32, (n,), q), _tensor(first, "first", torch.int32, (n,), q),
+                  _tensor(blocks, "blocks", torch.int32, (None,), q), blocks.numel(),
+                  None if seqs is None else _tensor(seqs, "seqs", torch.int32, (n,), q))
+    if out is None:
+        out = torch.empty_like(q)
+    op = _tensor(out, "out", torch.float16, (n, H, hd), q)
+    with _Call(q, stream) as c:
+        need = lib().lstk_attn_paged_work_bytes(n, H, kv, hd, s.max_len, int(window), int(n_sink)) if work is None else 0
+        wp, wn = c.work(work, need)
+        _check(lib().lstk_attn_paged(ctypes.byref(cache), ctypes.byref(s), qp, H, int(window), int(n_sink),
+                                     float(hd ** -0.5 if scale is None else scale), op, wp, wn, c.stream))
+    return out
+
+
+def sample_work_bytes(n_rows, n_vocab):
+    return lib().lstk_sample_work_bytes(int(n_rows), int(n_vocab))
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None, work=None, stream=None):
+    """The next token of each row of logits (f32 [n][n_vocab], rows may be strided), drawn with the random numbers u (f32 [n],
+    in [0, 1)): lstk_sample, include/lstk_qwen3.h. temperature, top_p, min_p (f32) and top_k (int32) are [n] device tensors;
+    None means temperature 1 / no cut. Returns (tokens int32 [n], probabilities f32 [n])."""
+    import torch
+    p, ld = _rows(logits, "logits", torch.float32)
+    n, V = logits.shape
+    f32 = lambda t, name: None if t is None else _tensor(t, name, torch.float32, (n,), logits)
+    how = Sampling(f32(temperature, "temperature"), None if top_k is None else _tensor(top_k, "top_k", torch.int32, (n,), logits),
+                   f32(top_p, "top_p"), f32(min_p, "min_p"))
+    up = _tensor(u, "u", torch.float32, (n,), logits)
+    if tokens is None:
+        tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+    if probs is None:
+        probs = torch.empty(n, dtype=torch.float32, device=logits.device)
+    tp, pp = _tensor(tokens, "tokens", torch.int32, (n,), logits), _tensor(probs, "probs", torch.float32, (n,), logits)
+    with _Call(logits, stream) as c:
+        wp, wn = c.work(work, lib().lstk_sample_work_bytes(n, V) if work is None else 0)
+        _check(lib().lstk_sample(p, ld, n, V, ctypes.byref(how), up, tp, pp, wp, wn, c.stream))
+    return tokens, probs
+
+
 _stores = weakref.WeakSet()  # stores not yet freed
 
 
@@ -344,6 +528,12 @@ class ExpertStore:
         T = hnorm.shape[0] if n_tokens is None else n_tokens
         _check(lib().lstk_moe_route(self._h, layer, _ptr(hnorm), T, _ptr(gate_inp), gate_type, _ptr(ids), _ptr(weights),
                                     _stream(stream)))
+
+    def route_by(self, layer, rule, hnorm, gate_inp, gate_type, ids, weights, bias=None, n_tokens=None, stream=None):
+        """route() by a RouterRule; bias: f32 [n_expert] or None."""
+        T = hnorm.shape[0] if n_tokens is None else n_tokens
+        _check(lib().lstk_moe_route_by(self._h, layer, ctypes.byref(rule.c), _ptr(hnorm), T, _ptr(gate_inp), gate_type, _ptr(bias),
+                                       _ptr(ids), _ptr(weights), _stream(stream)))
 
     def ffn(self, layer, hnorm, slots, weights, resid, out, n_tokens=None, stream=None):
         T = hnorm.shape[0] if n_tokens is None else n_tokens
@@ -475,6 +665,67 @@ class Qwen3Model:
         _check(lib().lstk_model_forward(self._h, int(seq), int(n_tokens), int(n_cells), _ptr(out), _ptr(trace),
                                         _stream(stream)))
         return out
+
+    def _batch_logits(self, n, logits):
+        import torch
+        return torch.empty(n, self.hp["n_vocab"], dtype=torch.float32, device=self.device) if logits is None else logits
+
+    def decode_batch(self, seqs, tokens, window=0, n_sink=0, trace=None, logits=None, stream=None):
+        """Appends tokens[i] to sequence seqs[i] (distinct), all in one step; returns the device logits [n_seq][n_vocab].
+        window > 0: each token attends its sequence's last `window` cells and first n_sink. trace: as decode's, with a row for
+        every sequence."""
+        s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
+        if s.size != tok.size:
+            raise LstkError(E_INVALID, "one token per sequence")
+        out = self._batch_logits(s.size, logits)
+        _check(lib().lstk_model_decode_batch(self._h, s.size, s.ctypes.data, tok.ctypes.data, int(window), int(n_sink), _ptr(out),
+                                             _ptr(trace), _stream(stream)))
+        return out
+
+    def prepare_batch(self, seqs, tokens, stream=None):
+        """First half of a batch step; returns the longest sequence's cells."""
+        s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
+        if s.size != tok.size:
+            raise LstkError(E_INVALID, "one token per sequence")
+        n = ctypes.c_int32()
+        _check(lib().lstk_model_prepare_batch(self._h, s.size, s.ctypes.data, tok.ctypes.data, ctypes.byref(n), _stream(stream)))
+        return n.value
+
+    def forward_batch(self, n_seq, max_len, window=0, n_sink=0, trace=None, logits=None, stream=None):
+        """Second half of a batch step (capturable; replays after each prepare_batch of n_seq sequences up to max_len)."""
+        out = self._batch_logits(n_seq, logits)
+        _check(lib().lstk_model_forward_batch(self._h, int(n_seq), int(max_len), int(window), int(n_sink), _ptr(out), _ptr(trace),
+                                              _stream(stream)))
+        return out
+
+    def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0):
+        """Continues several sequences together: prompts is {seq: token ids}, each is decoded (appended to what seq holds), then
+        n_new tokens are sampled for all of them, a batch step each. Returns {seq: the n_new tokens}; the last is not appended.
+        The settings are numbers, or sequences with one per prompt; generator: a torch generator on the model's device."""
+        import torch
+        seqs = [int(s) for s in prompts]
+        n, V = len(seqs), self.hp["n_vocab"]
+        if n == 0 or n_new <= 0:
+            return {s: [] for s in seqs}
+
+        def setting(v, dtype):
+            v = torch.as_tensor(v, dtype=dtype).flatten()
+            if v.numel() not in (1, n):
+                raise LstkError(E_INVALID, "a setting is one number, or one per prompt")
+            return v.expand(n).contiguous().to(self.device)
+
+        how = dict(temperature=setting(temperature, torch.float32), top_k=setting(top_k, torch.int32),
+                   top_p=setting(top_p, torch.float32), min_p=setting(min_p, torch.float32))
+        logits = torch.empty(n, V, dtype=torch.float32, device=self.device)
+        for i, s in enumerate(seqs):
+            self.decode(s, prompts[s], logits=logits[i])
+        got = []
+        for i in range(n_new):
+            u = torch.rand(n, device=self.device, generator=generator)
+            got.append(sample(logits, u, **how)[0].cpu().numpy())
+            if i + 1 < n_new:
+                self.decode_batch(seqs, got[-1], window=window, n_sink=n_sink, logits=logits)
+        return {s: [int(t[i]) for t in got] for i, s in enumerate(seqs)}
 
     def fill_context(self, seq, n_cells, seed=0, stream=None):
         """Appends n_cells synthetic positions (seeded random K/V, no tokens run) to sequence seq."""

@@ -3,7 +3,8 @@
 The library is the product: the MoE kernels (csrc/kernels.hip, grouped.hip, fused.hip), the HBM
 expert pool and the MoE C ABI (csrc/pool.cpp, include/lstk_moe.h), the host repacker
 (csrc/repack.cpp), the forward pass around the MoE block (csrc/forward.hip, csrc/model.cpp,
-include/lstk_qwen3.h) and the GGUF reader (csrc/gguf.cpp, include/lstk_gguf.h).
+include/lstk_qwen3.h), the operators of a step over many sequences (csrc/paged_attn.hip, sample.hip,
+select.hip, batch.cpp) and the GGUF reader (csrc/gguf.cpp, include/lstk_gguf.h).
 """
 import os
 import shutil
@@ -14,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblstk_moe.so")
-SOURCES = ["kernels.hip", "grouped.hip", "grouped_rows.hip", "fused.hip", "forward.hip", "pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp", "tier.hip"]
+SOURCES = ["kernels.hip", "grouped.hip", "grouped_rows.hip", "fused.hip", "forward.hip", "paged_attn.hip", "sample.hip", "select.hip", "pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp", "tier.hip", "batch.cpp"]
 ARCH = os.environ.get("LSTK_OFFLOAD_ARCH", "gfx950")
 
 
@@ -28,7 +29,7 @@ def hipcc():
 # Per-source extra flags. The MFMA kernels keep their accumulators in VGPRs (the VALU epilogue and the
 # attention's rescale then read them without v_accvgpr_read moves). In forward.hip only the attention
 # kernels change by it: fewer instructions at the same registers, steps of 1 to 63 tokens 1% faster.
-EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for s in ("grouped.hip", "grouped_rows.hip", "forward.hip")}
+EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for s in ("grouped.hip", "grouped_rows.hip", "forward.hip", "paged_attn.hip")}
 COMMON = ["-O3", "-std=c++20", "-fPIC",
           # packed-FP32 instructions off for all device code
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -54,7 +55,7 @@ def _run(cmd, verbose):
 OBJ_DIR = os.path.join(HERE, "_build")  # objects of the last build (not shipped; the sanitizer build reuses the kernels')
 ASAN_LIB = os.path.join(OBJ_DIR, "liblstk_moe_asan.so")
 # host sources checked by the sanitizer build: the pool's bookkeeping, the GGUF reader, the repacker, the model's host side
-HOST_SOURCES = ["pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp"]
+HOST_SOURCES = ["pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp", "batch.cpp"]
 SANITIZE = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
             "-Xarch_host", "-fno-omit-frame-pointer"]
 

@@ -47,6 +47,7 @@ struct RopeParams {
     uint16_t *kc, *vc; // this layer's caches
     const float *cs;   // [T][hd / 2][2]: cos and sin of each pair's angle (launch_rope_table), or null
     int ld;            // row stride of q, k and v (floats)
+    const int32_t *seqs = nullptr; // [T] when the tokens are of different sequences (seq is then unused)
 };
 
 // One F16 weight matrix of a GEMV launch: y[t * ldy + r] = sum_i fp16(x[t][i]) * w[r][i] (+ add[t * ldy + r]).

@@ -153,7 +153,7 @@ __device__ __forceinline__ void rope_head(const RopeParams &P, int t, int j, flo
 #pragma unroll
         for (int k = 0; k < kRopeMaxPer; k++) v[k] = lane + kWave * k < hd ? src[lane + kWave * k] : 0.0f;
         if (cells && lane == 0) {
-            P.cell_seq[cell] = P.seq;
+            P.cell_seq[cell] = P.seqs ? P.seqs[t] : P.seq;
             P.cell_pos[cell] = pos;
         }
 #pragma unroll
@@ -200,7 +200,7 @@ __device__ __forceinline__ void rope_head(const RopeParams &P, int t, int j, flo
         scale = 1.0f / sqrtf(mean + P.eps);
     }
     if (cells && lane == 0) {
-        P.cell_seq[cell] = P.seq;
+        P.cell_seq[cell] = P.seqs ? P.seqs[t] : P.seq;
         P.cell_pos[cell] = pos;
     }
     const float p = (float) pos;

@@ -28,4 +28,11 @@ int moe_block_normed(lstk_pool *pool, int layer, const float *d_x, const float *
                      const void *d_gate_inp, int gate_type, const float *d_resid, float *d_out, int32_t *d_ids,
                      float *d_weights, int T, hipStream_t st);
 
+struct SelectParams;
+// Whether a rule fits a router of n_expert experts, n_expert_used used (LSTK_E_INVALID and a message if not), and the launch
+// it makes.
+int check_rule(const lstk_router_rule *rule, int n_expert, int n_expert_used);
+SelectParams select_params(const lstk_router_rule &rule, const float *logits, int64_t ld, const float *bias, int T, int E, int k,
+                           int32_t *ids, float *weights);
+
 }  // namespace lstk

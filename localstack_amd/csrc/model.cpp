@@ -18,6 +18,8 @@
 //     which forms the same sums before it normalises them
 //     the last layer runs its FFN on the output row only (src/qwen3.cpp:233-237)
 //   output_norm + head on the last row                  (rmsnorm_kernel, gemv_kernel)
+// A batch step (one token for each of several sequences) runs the same sequence with every row kept to the
+// end, its attention over the sequences' own blocks (paged_attn_kernel) and the head on every row.
 // With several tokens per step the projections are plain F16 matrix products: the normalised rows and
 // the attention output are also written as fp16 (ggml rounds the activations of an F16 mat-mul to
 // fp16) and they are multiplied with f32 accumulation: on the matrix cores by gemm16_kernel (forward.hip)
@@ -37,6 +39,7 @@
 #include <vector>
 
 #include "../../include/lstk_qwen3.h"
+#include "batch.h"
 #include "forward.h"
 #include "internal.h"
 
@@ -77,6 +80,12 @@ struct KvBook {
         spare.resize(nb);
         for (uint32_t i = 0; i < nb; i++) spare[i] = nb - 1 - i;
         seqs.clear();
+    }
+    // Whether one more cell for each of n distinct sequences fits.
+    bool room_for_one_each(const int32_t *ids, int n) const {
+        size_t need = 0;
+        for (int i = 0; i < n; i++) need += (uint32_t) length(ids[i]) % kCellBlock == 0;
+        return need <= spare.size();
     }
     int32_t length(int32_t seq) const {
         const auto it = seqs.find(seq);
@@ -183,7 +192,10 @@ struct lstk_model {
     uint16_t *qr = nullptr; // [n_batch][n_head][head_dim] rotated Q, fp16 (the attention's Q operand)
     float *x = nullptr, *hn = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *attn = nullptr,
           *part = nullptr, *weights = nullptr;
-    int32_t *ids = nullptr, *slots = nullptr, *in = nullptr; // in = tokens | cells | positions
+    // in = tokens | cells | positions, and for batch steps sequences | lengths | first table entries | block table
+    int32_t *ids = nullptr, *slots = nullptr, *in = nullptr;
+    int batch_n = 0, batch_max_len = 0; // the batch step last prepared; 0: none, or something has replaced its inputs since
+    size_t part_bytes = 0;
     uint16_t *hn16 = nullptr, *attn16 = nullptr;             // fp16 inputs of the multi-token products
     int ld_qkv = 0; // row stride of q | k | v (one buffer: token t's Q, K and V rows side by side)
     std::vector<char> qkv_joined; // per layer: wk follows wq and wv follows wk in memory
@@ -222,6 +234,19 @@ hipError_t timed(lstk_model *M, int stage, F &&launch) {
     const hipError_t le = launch(&tm);
     M->launched[stage].push_back(t);
     return le;
+}
+
+// The shapes of a batch step's attention.
+lstk::PagedAttnParams paged_params(const lstk_model *M, int n_seq, int max_len, int window, int n_sink) {
+    lstk::PagedAttnParams p{};
+    p.n_seq = n_seq;
+    p.n_head = M->hp.n_head;
+    p.n_kv = M->hp.n_head_kv;
+    p.hd = M->hp.head_dim;
+    p.max_len = max_len;
+    p.window = window > 0 ? window : 0;
+    p.n_sink = n_sink;
+    return p;
 }
 
 void destroy(lstk_model *M) {
@@ -287,7 +312,13 @@ int create(const lstk_qwen3_hparams *hpp, const lstk_qwen3_weights *w, lstk_pool
     const size_t nb = n_batch, h = (size_t) hp.n_embd, hq = (size_t) hp.n_head * hp.head_dim,
                  hk = (size_t) hp.n_head_kv * hp.head_dim, k = (size_t) hp.n_expert_used;
     M->layer_elems = (size_t) kv_size * hk;
-    const size_t part_rows = lstk::attn_part_rows((int) nb, hp.n_head);
+    // partial rows: the larger of what steps of one sequence and batch steps of any size take
+    M->part_bytes = lstk::attn_part_rows((int) nb, hp.n_head) * (hp.head_dim + 4) * 4;
+    for (int n = 1; n <= (int) nb; n++) {
+        lstk::PagedAttnParams pp = paged_params(M, n, (int) kv_size, 0, 0);
+        M->part_bytes = std::max(M->part_bytes, lstk::paged_attn_plan(pp));
+    }
+    const size_t n_in = 6 * nb + kv_size / kCellBlock;
     struct Piece {
         void **dst;
         size_t bytes;
@@ -299,11 +330,11 @@ int create(const lstk_qwen3_hparams *hpp, const lstk_qwen3_weights *w, lstk_pool
         {(void **) &M->q, nb * (hq + 2 * hk) * 4},
         {(void **) &M->qr, nb * hq * 2},
         {(void **) &M->attn, nb * hq * 4},
-        {(void **) &M->part, part_rows * (hp.head_dim + 4) * 4},
+        {(void **) &M->part, M->part_bytes},
         {(void **) &M->weights, nb * k * 4},
         {(void **) &M->ids, nb * k * 4},
         {(void **) &M->slots, nb * k * 4},
-        {(void **) &M->in, 3 * nb * 4},
+        {(void **) &M->in, n_in * 4},
         {(void **) &M->hn16, nb * h * 2},
         {(void **) &M->attn16, nb * hq * 2},
         {(void **) &M->cell_seq, (size_t) kv_size * 4},
@@ -336,11 +367,11 @@ int create(const lstk_qwen3_hparams *hpp, const lstk_qwen3_weights *w, lstk_pool
     if ((e = hipMemset(M->kcache, 0, 2 * M->layer_elems * hp.n_layer * sizeof(uint16_t))) != hipSuccess ||
         (e = hipMemset(M->cell_seq, 0xff, (size_t) kv_size * 4)) != hipSuccess ||
         (e = hipMemset(M->cell_pos, 0xff, (size_t) kv_size * 4)) != hipSuccess ||
-        (e = hipMemset(M->in, 0, (size_t) 3 * nb * 4)) != hipSuccess) {
+        (e = hipMemset(M->in, 0, n_in * 4)) != hipSuccess) {
         destroy(M);
         return hip_fail(e, "hipMemset");
     }
-    if ((e = hipHostMalloc((void **) &M->h_in, (3 * nb + 2 * nb * k) * 4, hipHostMallocDefault)) != hipSuccess) {
+    if ((e = hipHostMalloc((void **) &M->h_in, (n_in + 2 * nb * k) * 4, hipHostMallocDefault)) != hipSuccess) {
         destroy(M);
         return set_error(LSTK_E_NOMEM, "hipHostMalloc of the step staging failed");
     }
@@ -349,7 +380,7 @@ int create(const lstk_qwen3_hparams *hpp, const lstk_qwen3_weights *w, lstk_pool
         destroy(M);
         return set_error(LSTK_E_DEVICE, "rocblas_create_handle failed");
     }
-    M->h_ids = M->h_in + 3 * nb;
+    M->h_ids = M->h_in + n_in;
     M->h_slots = M->h_ids + nb * k;
     if ((e = hipEventCreateWithFlags(&M->in_free, hipEventDisableTiming)) != hipSuccess ||
         (e = hipEventRecord(M->in_free, nullptr)) != hipSuccess) {
@@ -447,6 +478,7 @@ int moe(lstk_model *M, int l, int rows, float *xr, int32_t *ids, hipStream_t st,
 // Engine::make_step_inputs (src/engine.cpp:200-243): reserves the KV cells of T tokens of seq and queues
 // the upload of the tokens, cells and positions to the model's input buffer; *n_cells = the attended cells.
 int prepare(lstk_model *M, int32_t seq, const int32_t *tokens, int T, int *n_cells, hipStream_t st) {
+    M->batch_n = 0;
     std::vector<int32_t> cells, pos;
     if (!M->kv.alloc(seq, T, cells, pos)) return set_error(LSTK_E_EXHAUSTED, "KV cache is full");
     *n_cells = M->kv.n_kv();
@@ -463,16 +495,53 @@ int prepare(lstk_model *M, int32_t seq, const int32_t *tokens, int T, int *n_cel
     return LSTK_OK;
 }
 
+// The same for one token of each of n distinct sequences, with their lengths and block lists. Room for all of them is checked
+// before the first cell is taken.
+int prepare_batch(lstk_model *M, int n, const int32_t *seqs, const int32_t *tokens, hipStream_t st) {
+    if (!M->kv.room_for_one_each(seqs, n)) return set_error(LSTK_E_EXHAUSTED, "KV cache is full");
+    const int nb = M->n_batch;
+    const hipError_t e = hipEventSynchronize(M->in_free);
+    if (e != hipSuccess) return hip_fail(e, "hipEventSynchronize");
+    int32_t *const h = M->h_in;
+    std::vector<int32_t> cells, pos;
+    int n_table = 0, longest = 0;
+    for (int i = 0; i < n; i++) {
+        (void) M->kv.alloc(seqs[i], 1, cells, pos);
+        const KvBook::Seq &q = M->kv.seqs[seqs[i]];
+        h[i] = tokens[i];
+        h[nb + i] = cells[0];
+        h[2 * nb + i] = pos[0];
+        h[3 * nb + i] = seqs[i];
+        h[4 * nb + i] = q.len;
+        h[5 * nb + i] = n_table;
+        for (uint32_t b : q.blocks) h[6 * nb + n_table++] = (int32_t) b;
+        longest = std::max(longest, q.len);
+    }
+    M->batch_n = n;
+    M->batch_max_len = longest;
+    hipError_t c = hipMemcpyAsync(M->in, h, ((size_t) 6 * nb + n_table) * 4, hipMemcpyHostToDevice, st);
+    if (c == hipSuccess) c = hipEventRecord(M->in_free, st);
+    return c == hipSuccess ? LSTK_OK : hip_fail(c, "step input upload");
+}
+
+// What a batch step's kernels take beyond its rows.
+struct BatchStep {
+    int max_len, window, n_sink;
+};
+
 // The kernels of one step (qwen3_build_graph, src/qwen3.cpp:223-259) over the inputs prepare() uploaded.
 // With a resident pool (or a streaming pool that acquires on the device) this makes no host
-// synchronisation, so a caller may capture it in a HIP graph.
-int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int32_t *d_trace, hipStream_t st) {
+// synchronisation, so a caller may capture it in a HIP graph. With `batch` the T rows are tokens of T sequences (seq and
+// n_cells are then unused) and every row is kept to the end.
+int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int32_t *d_trace, hipStream_t st,
+            const BatchStep *batch = nullptr) {
     const lstk_qwen3_hparams &hp = M->hp;
     const int nb = M->n_batch, h = hp.n_embd, hd = hp.head_dim, k = hp.n_expert_used;
     const int hq = hp.n_head * hd, hk = hp.n_head_kv * hd;
     hipError_t e;
     const int32_t *d_tok = M->in, *d_cells = M->in + nb, *d_pos = M->in + 2 * nb;
-    const bool blas = T >= kBlasMinTokens;
+    const bool one = T == 1 && !batch; // a step of one token has launches of its own
+    const bool blas = T >= kBlasMinTokens || batch;
     // The attended range starts at the sequence's lowest block when the step runs now. A captured forward
     // is replayed after later prepares whose new blocks may lie below that block (freed blocks come back
     // in the order they were released), so a capture attends from cell 0: cells of other sequences and
@@ -507,7 +576,7 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
         gp.rows_total = hq + 2 * hk;
         gp.cols = h;
         gp.T = T;
-        if (T == 1) {
+        if (one) {
             // one token: attn_norm (and layer 0's embedding gather) run inside the Q/K/V launch
             gp.x = M->x;
             gp.norm_w = L.attn_norm;
@@ -535,7 +604,8 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
                             M->ld_qkv};
         // one token (its query rows in one 16-row tile): QK-norm, RoPE and the K / V store run inside
         // the attention launch
-        const bool rope_in_attn = T == 1 && hp.n_head / hp.n_head_kv <= 16 && !M->rope_apart;
+        if (batch) rp.seqs = M->in + 3 * nb;
+        const bool rope_in_attn = one && hp.n_head / hp.n_head_kv <= 16 && !M->rope_apart;
         if (blas) {
             const int rc = timed_span(M, 1, st, [&] {
                 // Q, K and V rows side by side in the output; one product when the weights are too
@@ -571,10 +641,34 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
         ap.out16 = blas ? M->attn16 : nullptr;
         ap.rope_in = rope_in_attn ? 1 : 0;
         ap.rope = rp;
-        lstk::attn_plan(ap); // clears rope_in when the context is too long for one pass per chunk
+        lstk::PagedAttnParams pp{};
+        if (batch) {
+            pp = paged_params(M, T, batch->max_len, batch->window, batch->n_sink);
+            if (lstk::paged_attn_plan(pp) > M->part_bytes) return set_error(LSTK_E_INVALID, "the step's attention does not fit the scratch");
+            pp.q = M->qr;
+            pp.kc = kc;
+            pp.vc = vc;
+            pp.len = M->in + 4 * nb;
+            pp.first = M->in + 5 * nb;
+            pp.blocks = M->in + 6 * nb;
+            pp.n_table = (int) (M->kv.size / kCellBlock);
+            pp.cell_seq = M->cell_seq;
+            pp.seq = M->in + 3 * nb;
+            pp.kv_size = M->kv.size;
+            pp.scale = ap.scale * 1.44269504088896341f;
+            pp.part = M->part;
+            pp.out = M->attn16;
+        } else {
+            lstk::attn_plan(ap); // clears rope_in when the context is too long for one pass per chunk
+        }
         if (!ap.rope_in && (e = timed(M, 1, [&](const lstk::LaunchTiming *tm) { return lstk::launch_rope(rp, st, tm); })) != hipSuccess)
             return hip_fail(e, "rope launch");
-        if ((e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_attn(ap, st, tm); })) != hipSuccess ||
+        if (batch) {
+            if ((e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_paged_attn(pp, st, tm); })) != hipSuccess ||
+                (pp.n_chunk > 1 &&
+                 (e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_paged_attn_join(pp, st, tm); })) != hipSuccess))
+                return hip_fail(e, "attention launch");
+        } else if ((e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_attn(ap, st, tm); })) != hipSuccess ||
             (ap.n_chunk > 1 &&
              (e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_attn_combine(ap, st, tm); })) != hipSuccess))
             return hip_fail(e, "attention launch");
@@ -587,7 +681,7 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
         op.T = T;
         // after the last attention only the output row goes on (src/qwen3.cpp:233-237)
         const bool last = l == hp.n_layer - 1;
-        const int rows = last ? 1 : T;
+        const int rows = last && !batch ? 1 : T;
         float *xr = M->x + (size_t) (T - rows) * h;
         lstk::NormParams fp{xr, nullptr, nullptr, nullptr, L.ffn_norm, M->hn, rows, h, hp.rms_eps};
         if (blas) {
@@ -606,7 +700,7 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
             (e = timed(M, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_rmsnorm(fp, st, tm); })) != hipSuccess)
             return hip_fail(e, "ffn_norm launch");
         int32_t *ids = d_trace ? d_trace + ((size_t) l * T + (T - rows)) * k : M->ids;
-        if (last && d_trace && T > 1) {
+        if (last && d_trace && rows < T) {
             lstk::FillParams fl{d_trace + (size_t) l * T * k, (T - 1) * k, -1};
             if ((e = lstk::launch_fill(fl, st, nullptr)) != hipSuccess) return hip_fail(e, "trace fill launch");
         }
@@ -619,6 +713,12 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
         if (M->capture && (e = hipMemcpyAsync(M->capture + (size_t) l * T * h, M->x, (size_t) T * h * sizeof(float),
                                               hipMemcpyDeviceToDevice, st)) != hipSuccess)
             return hip_fail(e, "capture copy");
+    }
+    if (batch) {
+        lstk::NormParams np{M->x, nullptr, nullptr, nullptr, M->output_norm, M->hn, T, h, hp.rms_eps, M->hn16};
+        if ((e = timed(M, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_rmsnorm(np, st, tm); })) != hipSuccess)
+            return hip_fail(e, "output_norm launch");
+        return timed_span(M, 4, st, [&] { return project(M, M->output, hp.n_vocab, h, M->hn16, T, d_logits, hp.n_vocab, false, st); });
     }
     lstk::NormParams onp{M->x + (size_t) (T - 1) * h, nullptr, nullptr, nullptr, M->output_norm, M->hn, 1, h, hp.rms_eps};
     if ((e = timed(M, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_rmsnorm(onp, st, tm); })) != hipSuccess)
@@ -641,12 +741,39 @@ int step(lstk_model *M, int32_t seq, const int32_t *tokens, int T, float *d_logi
     return rc != LSTK_OK ? rc : forward(M, seq, T, n_cells, d_logits, d_trace, st);
 }
 
+// Engine::step_resident's trace write (src/engine.cpp:299-316): token count, then each layer's ids
+int write_trace(lstk_model *M, const int32_t *d_ids, int n, hipStream_t st) {
+    const size_t cnt = (size_t) M->hp.n_layer * n * M->hp.n_expert_used;
+    M->trace_host.resize(cnt);
+    hipError_t e;
+    if ((e = hipMemcpyAsync(M->trace_host.data(), d_ids, cnt * 4, hipMemcpyDeviceToHost, st)) != hipSuccess ||
+        (e = hipStreamSynchronize(st)) != hipSuccess)
+        return hip_fail(e, "trace download");
+    const int32_t n32 = n;
+    if (fwrite(&n32, 4, 1, M->trace) != 1 || fwrite(M->trace_host.data(), 4, cnt, M->trace) != cnt || fflush(M->trace) != 0)
+        return set_error(LSTK_E_IO, "routing trace write failed");
+    return LSTK_OK;
+}
+
 int check_tokens(const lstk_model *M, const int32_t *tokens, int n) {
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= M->hp.n_vocab)
             return set_error(LSTK_E_INVALID, "token id " + std::to_string(tokens[i]) + " out of range");
     return LSTK_OK;
 }
+
+int check_batch(const lstk_model *M, int n_seq, const int32_t *seqs, const int32_t *tokens) {
+    if (!M || !seqs || !tokens) return set_error(LSTK_E_INVALID, "null argument");
+    if (n_seq < 1 || n_seq > M->n_batch) return set_error(LSTK_E_INVALID, "n_seq must be in [1, n_batch]");
+    std::vector<int32_t> sorted(seqs, seqs + n_seq);
+    std::sort(sorted.begin(), sorted.end());
+    if (sorted[0] < 0) return set_error(LSTK_E_INVALID, "seq must be >= 0");
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+        return set_error(LSTK_E_INVALID, "a sequence is in the batch twice");
+    return check_tokens(M, tokens, n_seq);
+}
+
+int check_window(int n_sink) { return n_sink < 0 ? set_error(LSTK_E_INVALID, "n_sink must be >= 0") : LSTK_OK; }
 
 }  // namespace
 
@@ -677,17 +804,8 @@ int lstk_model_decode(lstk_model *model, int32_t seq, const int32_t *tokens, int
             const int rc = step(model, seq, tokens + done, n, d_logits, tr, st);
             if (rc != LSTK_OK) return rc;
             if (model->trace) {
-                // Engine::step_resident's trace write (src/engine.cpp:299-316): token count, then each layer's ids
-                const size_t cnt = (size_t) model->hp.n_layer * n * model->hp.n_expert_used;
-                model->trace_host.resize(cnt);
-                hipError_t e;
-                if ((e = hipMemcpyAsync(model->trace_host.data(), tr, cnt * 4, hipMemcpyDeviceToHost, st)) != hipSuccess ||
-                    (e = hipStreamSynchronize(st)) != hipSuccess)
-                    return hip_fail(e, "trace download");
-                const int32_t n32 = n;
-                if (fwrite(&n32, 4, 1, model->trace) != 1 || fwrite(model->trace_host.data(), 4, cnt, model->trace) != cnt ||
-                    fflush(model->trace) != 0)
-                    return set_error(LSTK_E_IO, "routing trace write failed");
+                const int wrc = write_trace(model, tr, n, st);
+                if (wrc != LSTK_OK) return wrc;
             }
             done += n;
         }
@@ -721,12 +839,56 @@ int lstk_model_forward(lstk_model *model, int32_t seq, int n_tokens, int32_t n_c
     return forward(model, seq, n_tokens, n_cells, d_logits, d_trace, static_cast<hipStream_t>(stream));
 }
 
+int lstk_model_decode_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int window, int n_sink,
+                            float *d_logits, int32_t *d_trace, lstk_stream_t stream) {
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    try {
+        int rc;
+        if ((rc = check_batch(model, n_seq, seqs, tokens)) != LSTK_OK || (rc = check_window(n_sink)) != LSTK_OK) return rc;
+        if (!d_logits) return set_error(LSTK_E_INVALID, "null argument");
+        if ((rc = prepare_batch(model, n_seq, seqs, tokens, st)) != LSTK_OK) return rc;
+        int32_t *tr = d_trace ? d_trace : model->trace ? model->trace_dev : nullptr;
+        const BatchStep step{model->batch_max_len, window, n_sink};
+        rc = forward(model, 0, n_seq, 0, d_logits, tr, st, &step);
+        return rc == LSTK_OK && model->trace ? write_trace(model, tr, n_seq, st) : rc;
+    } catch (const std::exception &ex) {
+        return set_error(LSTK_E_NOMEM, std::string("lstk_model_decode_batch: ") + ex.what());
+    }
+}
+
+int lstk_model_prepare_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int32_t *max_len,
+                             lstk_stream_t stream) {
+    if (!max_len) return set_error(LSTK_E_INVALID, "null argument");
+    try {
+        int rc;
+        if ((rc = check_batch(model, n_seq, seqs, tokens)) != LSTK_OK) return rc;
+        rc = prepare_batch(model, n_seq, seqs, tokens, static_cast<hipStream_t>(stream));
+        if (rc == LSTK_OK) *max_len = model->batch_max_len;
+        return rc;
+    } catch (const std::exception &ex) {
+        return set_error(LSTK_E_NOMEM, std::string("lstk_model_prepare_batch: ") + ex.what());
+    }
+}
+
+int lstk_model_forward_batch(lstk_model *model, int n_seq, int32_t max_len, int window, int n_sink, float *d_logits,
+                             int32_t *d_trace, lstk_stream_t stream) {
+    if (!model || !d_logits) return set_error(LSTK_E_INVALID, "null argument");
+    if (n_seq < 1 || n_seq != model->batch_n) return set_error(LSTK_E_INVALID, "n_seq is not that of the batch step last prepared");
+    if (max_len < model->batch_max_len || max_len > (int32_t) model->kv.size)
+        return set_error(LSTK_E_INVALID, "max_len must hold the step last prepared, and be at most kv_size");
+    const int rc = check_window(n_sink);
+    if (rc != LSTK_OK) return rc;
+    const BatchStep step{max_len, window, n_sink};
+    return forward(model, 0, n_seq, 0, d_logits, d_trace, static_cast<hipStream_t>(stream), &step);
+}
+
 int lstk_model_fill_context(lstk_model *model, int32_t seq, int n_cells, uint64_t seed, lstk_stream_t stream) {
     if (!model) return set_error(LSTK_E_INVALID, "null model");
     if (seq < 0 || n_cells < 0) return set_error(LSTK_E_INVALID, "seq and n_cells must be >= 0");
     lstk_model *M = model;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int nb = M->n_batch;
+    M->batch_n = 0;
     try {
         for (int done = 0; done < n_cells;) {
             const int T = std::min(nb, n_cells - done);
@@ -790,12 +952,14 @@ int lstk_model_set_trace(lstk_model *model, const char *path) {
 int lstk_model_remove_seq(lstk_model *model, int32_t seq) {
     if (!model) return set_error(LSTK_E_INVALID, "null model");
     model->kv.remove_seq(seq);
+    model->batch_n = 0;
     return sync_cells(model);
 }
 
 int lstk_model_truncate_seq(lstk_model *model, int32_t seq, int32_t keep) {
     if (!model) return set_error(LSTK_E_INVALID, "null model");
     model->kv.truncate_seq(seq, keep);
+    model->batch_n = 0;
     return sync_cells(model);
 }
 

@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "../../include/lstk_moe.h"
+#include "batch.h"
 #include "formats.h"
 #include "internal.h"
 #include "kernels.h"
@@ -1361,6 +1362,35 @@ int lstk_moe_route(lstk_pool *pool, int layer, const float *d_hnorm, int n_token
     e = timed(pool, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_topk(tp, st, tm); });
     if (e != hipSuccess) return hip_fail(e, "topk launch");
     return LSTK_OK;
+}
+
+int lstk_moe_route_by(lstk_pool *pool, int layer, const lstk_router_rule *rule, const float *d_hnorm, int n_tokens,
+                      const void *d_gate_inp, int gate_type, const float *d_bias, int32_t *d_ids, float *d_weights,
+                      lstk_stream_t stream) {
+    int rc;
+    if ((rc = check_call(pool, layer, n_tokens)) != LSTK_OK) return rc;
+    const int E = pool->dims.n_expert, k = pool->dims.n_expert_used;
+    if ((rc = lstk::check_rule(rule, E, k)) != LSTK_OK) return rc;
+    if (n_tokens == 0) return LSTK_OK;
+    if ((rc = check_router_args(d_gate_inp, gate_type)) != LSTK_OK || (rc = check_act(d_hnorm, "hnorm")) != LSTK_OK) return rc;
+    if (!d_ids || !d_weights) return fail(LSTK_E_INVALID, "ids and weights must be non-null");
+    if (!aligned(d_bias, 4)) return fail(LSTK_E_INVALID, "bias must be 4-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    lstk::RouteParams rp{};
+    rp.hnorm = d_hnorm;
+    rp.T = n_tokens;
+    rp.h = pool->dims.n_embd;
+    rp.do_route = 1;
+    rp.gate_inp = d_gate_inp;
+    rp.gate_type = gate_type;
+    rp.E = E;
+    rp.logits = pool->logits;
+    rp.qtype = 0;
+    hipError_t e = timed(pool, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_route(rp, st, tm); });
+    if (e != hipSuccess) return hip_fail(e, "route launch");
+    const lstk::SelectParams sp = lstk::select_params(*rule, pool->logits, E, d_bias, n_tokens, E, k, d_ids, d_weights);
+    e = timed(pool, 0, [&](const lstk::LaunchTiming *tm) { return lstk::launch_select(sp, st, tm); });
+    return e == hipSuccess ? LSTK_OK : hip_fail(e, "select launch");
 }
 
 int lstk_moe_ffn(lstk_pool *pool, int layer, const float *d_hnorm, const int32_t *d_slots, const float *d_weights,

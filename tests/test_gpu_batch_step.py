@@ -1,0 +1,318 @@
+"""A step of one token for each of several sequences (lstk_model_decode_batch) against the oracle and the one-sequence path.
+
+Bars are those of the forward pass's own tests: logits within 1e-2 max-abs and 2.5e-3 RMS of the oracle (activations are
+quantized on both sides, so an fp32 rounding can move a value across a quantization step)."""
+import numpy as np
+import pytest
+
+import oracle
+from localstack_amd import synth
+
+pytestmark = pytest.mark.gpu
+
+LOGITS_TOL, RMS_TOL = 1e-2, 2.5e-3
+TINY = dict(n_layer=2, n_embd=256, n_head=4, n_head_kv=2, head_dim=64, n_vocab=1024, n_expert=8, n_expert_used=2,
+            n_ff_exp=512, n_ctx_train=1024, rms_eps=1e-6, rope_freq_base=10000.0)
+MID = dict(n_layer=2, n_embd=2048, n_head=32, n_head_kv=4, head_dim=128, n_vocab=4096, n_expert=128, n_expert_used=8,
+           n_ff_exp=768, n_ctx_train=4096, rms_eps=1e-6, rope_freq_base=1000000.0)
+_w = {}
+
+
+def weights(name):
+    if name not in _w:
+        hp, wtype, seed = {"tiny": (TINY, 8, 1234), "mid": (MID, 12, 99), "one": (dict(TINY, n_layer=1), 8, 77)}[name]
+        _w[name] = (hp, synth.qwen3_weights(np.random.default_rng(seed), hp, wtype=wtype))
+    return _w[name]
+
+
+def build(lstk, dev, hp, w, n_batch=64, kv_size=1024, **kw):
+    layers = [(L["types"], L["up"], L["gate"], L["down"]) for L in w["layers"]]
+    store = lstk.ExpertStore(hp["n_layer"], hp["n_embd"], hp["n_ff_exp"], hp["n_expert"], hp["n_expert_used"], n_batch, layers, **kw)
+    return store, lstk.Qwen3Model(hp, w, store, kv_size, n_batch, device=dev)
+
+
+def prompt(seed, n, vocab):
+    return np.random.default_rng(seed).integers(0, vocab, n).astype(np.int32)
+
+
+def near(got, ref, what):
+    err, rms, a, b = oracle.diff_logits(ref, got)
+    assert err <= LOGITS_TOL and rms <= RMS_TOL, (what, err, rms)
+    assert a == b, what
+
+
+@pytest.mark.parametrize("name,lens", [("tiny", [5, 1, 40, 33, 64, 17]), ("tiny", [12])])
+def test_matches_the_oracle(lstk, dev, name, lens):
+    """Prompts one by one, then steps for all sequences in changing order and number: logits and router ids of every row."""
+    import torch
+    hp, w = weights(name)
+    _, model = build(lstk, dev, hp, w, n_batch=16 if name == "mid" else 64)
+    refs, feed = {}, {}
+    for s, n in enumerate(lens):
+        toks = prompt(100 + s, n, hp["n_vocab"])
+        refs[s] = oracle.Qwen3(hp, w, 256)
+        for i in range(0, n, 16):
+            model.decode(10 * s, toks[i:i + 16])
+            r = refs[s].decode(toks[i:i + 16])
+        feed[s] = int(np.argmax(r))
+    rng = np.random.default_rng(5)
+    for step in range(5):
+        order = rng.permutation(len(lens))[:max(1, len(lens) - step % 2)]
+        tr = torch.full((hp["n_layer"], len(order), hp["n_expert_used"]), -7, dtype=torch.int32, device=dev)
+        got = model.decode_batch([10 * s for s in order], [feed[s] for s in order], trace=tr).cpu().numpy()
+        for i, s in enumerate(order):
+            rl, rt = refs[s].decode(np.array([feed[s]], np.int32), want_trace=True)
+            near(got[i], rl, (name, step, s))
+            np.testing.assert_array_equal(tr.cpu().numpy()[:, i], rt[:, 0])
+            feed[s] = int(np.argmax(rl))
+        print(f"[batch {name}] step {step}: {len(order)} sequences", flush=True)
+    for s, n in enumerate(lens):
+        assert model.seq_len(10 * s) >= n + 2
+
+
+def test_attention_at_the_30b_layout(lstk, dev):
+    """32 query heads on 4 KV heads of 128, prompts of 20, 3 and 70 tokens: the residual after layer 0's attention, row by row,
+    against one-sequence steps. (Logits are no measure here: on these prompts the one-sequence path itself is 2.2e-2 from the
+    oracle, since a router near-tie in the prompt turns out the other way.)
+
+    Both paths round weights and outputs of the attention to fp16, and scores' errors are smaller, so an output value differs
+    by at most d = 6 * 2^-11 max|v|; the o-projection adds n_head * head_dim such errors of either sign, so the RMS of the
+    difference stays below the largest row norm of wo times d. A wrong cell or head moves the residual by the size of the
+    attention's share, an order of magnitude more."""
+    import torch
+    hp, w = weights("mid")
+    models = [build(lstk, dev, hp, w, n_batch=16)[1] for _ in range(2)]
+    prompts = [prompt(100 + s, n, hp["n_vocab"]) for s, n in enumerate((20, 3, 70))]
+    L = w["layers"][0]
+    h, hd = hp["n_embd"], hp["head_dim"]
+    emb = np.asarray(w["tok_embd"]).view(np.float16).reshape(-1, h).astype(np.float64)
+    f16 = lambda a, n: np.asarray(a).view(np.float16).reshape(n, -1).astype(np.float64)
+    used = emb[np.concatenate(prompts + [np.array([9, 10, 11])])]
+    v = (used / np.sqrt((used ** 2).mean(1, keepdims=True) + hp["rms_eps"]) * np.asarray(L["attn_norm"])) @ f16(L["wv"], hp["n_head_kv"] * hd).T
+    d = 6 * 2.0 ** -11 * np.abs(v).max()
+    bound = d * np.linalg.norm(f16(L["wo"], h), axis=1).max()
+    for m in models:
+        for s, p in enumerate(prompts):
+            for i in range(0, len(p), 16):
+                m.decode(s, p[i:i + 16])
+    many = torch.zeros((hp["n_layer"], 3, h), device=dev)
+    models[0].debug_capture_moe_in(many)
+    models[0].decode_batch([2, 0, 1], [9, 10, 11])
+    for i, s in enumerate([2, 0, 1]):
+        one = torch.zeros((hp["n_layer"], 1, h), device=dev)
+        models[1].debug_capture_moe_in(one)
+        models[1].decode(s, [9 + i])
+        torch.cuda.synchronize()
+        diff = (many[0, i] - one[0, 0]).double()
+        share = (one[0, 0].cpu().double().numpy() - emb[9 + i])
+        rms = float(diff.square().mean().sqrt())
+        print(f"[batch 30b layout] row {i}: rms of the difference {rms:.2e}, bound {bound:.2e}, attention's share {np.sqrt((share ** 2).mean()):.2e}", flush=True)
+        assert rms <= bound
+    for m in models:
+        m.debug_capture_moe_in(None)
+
+
+def test_window_of_one_layer(lstk, dev):
+    """With one layer a cell's K and V depend on its own token alone, and attention on distances alone: a token that sees the
+    last 20 cells answers like one whose sequence holds only those."""
+    hp, w = weights("one")
+    _, model = build(lstk, dev, hp, w)
+    toks = prompt(3, 90, hp["n_vocab"])
+    model.decode(0, toks[:60])
+    model.decode(1, toks[60:61])
+    for i in range(61, 90):
+        got = model.decode_batch([0, 1], [toks[i - 1], toks[i]], window=20).cpu().numpy()
+        if i in (61, 75, 89):
+            ref = oracle.Qwen3(hp, w, 256)
+            near(got[0], ref.decode(toks[i - 20:i]), ("window", i))
+    wide = model.decode_batch([0, 1], [5, 6], window=1000, n_sink=3).cpu().numpy()
+    model.truncate_seq(0, model.seq_len(0) - 1)
+    model.truncate_seq(1, model.seq_len(1) - 1)
+    assert np.abs(wide - model.decode_batch([0, 1], [5, 6]).cpu().numpy()).max() <= LOGITS_TOL
+
+
+def test_streaming_pool(lstk, dev):
+    hp, w = weights("tiny")
+    out = []
+    slab = 3 * 512 * 256 // 32 * 34
+    for kw in (dict(), dict(streaming=True, pool_bytes=8 * slab, min_slots=8),
+               dict(streaming=True, pool_bytes=8 * slab, min_slots=8, device_lru=True)):
+        _, model = build(lstk, dev, hp, w, n_batch=4, **kw)
+        for s in range(3):
+            model.decode(s, prompt(s, 4, hp["n_vocab"]))
+        out.append([model.decode_batch([2, 0, 1], [7, 8, 9 + i]).cpu().numpy() for i in range(3)])
+    for o in out[1:]:
+        np.testing.assert_array_equal(out[0], o)
+
+
+def test_graph_replay(lstk, dev):
+    """A captured step replayed for other sequences of the same number and other lengths, eager work between: the eager
+    results bit for bit."""
+    import torch
+    hp, w = weights("tiny")
+    models = [build(lstk, dev, hp, w)[1] for _ in range(2)]
+    for m in models:
+        for s in range(5):
+            m.decode(s, prompt(s, 3 + 29 * s, hp["n_vocab"]))
+    eager, m = models
+    logits = torch.empty(3, hp["n_vocab"], device=dev)
+    groups = [([0, 1, 2], [5, 6, 7]), ([4, 3, 0], [1, 2, 3]), ([2, 4, 1], [9, 9, 9]), ([0, 1, 2], [5, 6, 7])] * 3
+
+    def ref(gr):
+        eager.prepare_batch(*gr)
+        return eager.forward_batch(3, 200)
+
+    m.prepare_batch(*groups[0])
+    m.forward_batch(3, 200, logits=logits)  # warm up outside the capture
+    assert torch.equal(ref(groups[0]), logits)
+    m.prepare_batch(*groups[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        m.forward_batch(3, 200, logits=logits)
+    g.replay()
+    assert torch.equal(ref(groups[1]), logits)
+    for step, gr in enumerate(groups[2:]):
+        m.prepare_batch(*gr)
+        g.replay()
+        assert torch.equal(ref(gr), logits), step
+        torch.zeros(1000, device=dev).sum().item()
+
+
+def test_prepared_cells_that_never_ran_are_not_seen(lstk, dev):
+    """A prepare whose forward never runs reserves cells that hold nothing: a later batch step does not attend them."""
+    hp, w = weights("one")
+    _, m = build(lstk, dev, hp, w)
+    m.decode(0, prompt(1, 10, 1024))
+    m.decode(1, prompt(2, 10, 1024))
+    m.prepare_batch([0, 1], [3, 4])  # cells 10 of both, never run
+    m.prepare(0, [5])                # cell 11 of sequence 0
+    got = m.decode_batch([0, 1], [8, 9]).cpu().numpy()
+    assert m.seq_len(0) == 13 and m.seq_len(1) == 12
+    # the same with the holes closed: only RoPE distances to the first ten cells differ, so compare against a
+    # one-sequence step of the same positions, which masks by the cells' owners
+    _, r = build(lstk, dev, hp, w)
+    for s, (seed, holes, tok) in enumerate(((1, 2, 8), (2, 1, 9))):
+        r.decode(s, prompt(seed, 10, 1024))
+        for _ in range(holes):
+            r.prepare(s, [3])
+        ref = r.decode(s, [tok]).cpu().numpy()
+        assert np.abs(got[s] - ref).max() <= LOGITS_TOL
+
+
+def test_isolation_and_reuse(lstk, dev):
+    """Sequences do not see each other; removed ones' blocks are taken over; a batch of one agrees with decode."""
+    hp, w = weights("tiny")
+    _, m = build(lstk, dev, hp, w)
+    _, solo = build(lstk, dev, hp, w)
+    A, B, C = prompt(1, 50, 1024), prompt(2, 70, 1024), prompt(3, 45, 1024)
+    m.decode(1, B)
+    m.decode(0, A)
+    m.remove_seq(1)
+    m.decode(2, C)
+    solo.decode(0, A)
+    for t in (4, 5, 6):
+        got = m.decode_batch([2, 0], [9, t]).cpu().numpy()
+        ref = solo.decode(0, [t]).cpu().numpy()
+        assert np.abs(got[1] - ref).max() <= LOGITS_TOL and np.argmax(got[1]) == np.argmax(ref)
+
+
+def among_best(hp, w, p, tokens, k):
+    """Whether every token is one of the oracle's k best after what came before, within the logits' tolerance."""
+    ref, feed = oracle.Qwen3(hp, w, 128), p
+    for t in tokens:
+        lg = ref.decode(feed)
+        assert (lg > lg[t] + 2 * LOGITS_TOL).sum() < k, t
+        feed = np.array([t], np.int32)
+
+
+def test_generate(lstk, dev):
+    """Greedy generation for several prompts follows the oracle token by token; sampled generation repeats for the same seed,
+    keeps to each prompt's top-k, and its windowed form runs."""
+    import torch
+    hp, w = weights("tiny")
+    prompts = {3: prompt(1, 9, 1024), 0: prompt(2, 30, 1024), 7: prompt(3, 1, 1024)}
+    _, m = build(lstk, dev, hp, w)
+    got = m.generate(prompts, 8)
+    for s, p in prompts.items():
+        assert len(got[s]) == 8 and m.seq_len(s) == len(p) + 7
+        among_best(hp, w, p, got[s], 1)
+    runs = []
+    for _ in range(2):
+        _, m = build(lstk, dev, hp, w)
+        gen = torch.Generator(device=dev)
+        gen.manual_seed(5)
+        runs.append(m.generate(prompts, 6, temperature=[0.9, 0.0, 1.5], top_k=[30, 0, 10], top_p=0.95, generator=gen))
+    assert runs[0] == runs[1]
+    for (s, p), k in zip(prompts.items(), (30, 1, 10)):
+        among_best(hp, w, p, runs[0][s], k)
+    more = m.generate({3: [5], 0: [6]}, 5, temperature=1.0, window=16, n_sink=2)
+    assert [len(t) for t in more.values()] == [5, 5] and m.seq_len(3) == 9 + 5 + 1 + 4
+    assert m.generate({}, 3) == {} and m.generate({3: [1]}, 0) == {3: []}
+    with pytest.raises(lstk.LstkError):
+        m.generate(prompts, 2, temperature=[1.0, 2.0])
+
+
+def test_errors(lstk, dev):
+    hp, w = weights("tiny")
+    _, m = build(lstk, dev, hp, w, n_batch=4, kv_size=256)
+    m.decode(0, [1, 2, 3])
+
+    def refused(f, code=lstk.E_INVALID):
+        n = [m.seq_len(s) for s in range(10)]
+        with pytest.raises(lstk.LstkError) as e:
+            f()
+        assert e.value.code == code
+        assert n == [m.seq_len(s) for s in range(10)]
+
+    refused(lambda: m.decode_batch([0, 0], [1, 2]))
+    refused(lambda: m.decode_batch([0, -1], [1, 2]))
+    refused(lambda: m.decode_batch([0, 1], [1, 1024]))
+    refused(lambda: m.decode_batch([0, 1], [1]))
+    refused(lambda: m.decode_batch([], []))
+    refused(lambda: m.decode_batch(range(5), range(5)))
+    refused(lambda: m.decode_batch([0], [1], window=5, n_sink=-1))
+    refused(lambda: m.forward_batch(1, 10))
+    n = m.prepare_batch([0, 1], [1, 2])
+    assert n == 4
+    refused(lambda: m.forward_batch(1, 10))
+    refused(lambda: m.forward_batch(2, 3))
+    refused(lambda: m.forward_batch(2, 257))
+    m.forward_batch(2, n)
+    m.prepare_batch([0, 1], [1, 2])
+    m.remove_seq(1)
+    refused(lambda: m.forward_batch(2, 10))
+    # room: 8 blocks of 32 cells; sequences 0 and 2 .. 7 take one each, sequence 7 a second one
+    for s in range(2, 8):
+        m.decode(s, [1])
+    m.truncate_seq(0, 3)
+    for i in range(8):
+        m.decode(7, [1] * 4)
+    assert m.seq_len(7) == 33
+    refused(lambda: m.decode_batch([0, 8], [1, 1]), lstk.E_EXHAUSTED)
+    m.decode_batch([0, 2, 7], [1, 1, 1])
+    assert m.seq_len(0) == 4 and m.seq_len(8) == 0
+
+
+def test_trace_file(lstk, dev, tmp_path):
+    from localstack_amd import trace
+    hp, w = weights("tiny")
+    _, m = build(lstk, dev, hp, w)
+    path = str(tmp_path / "t.bin")
+    m.set_trace(path)
+    m.decode(0, [1, 2, 3])
+    import torch
+    tr = torch.zeros((2, 2, 2), dtype=torch.int32, device=dev)
+    m.decode_batch([0, 1], [4, 5], trace=tr)
+    m.decode_batch([1], [5])
+    m.set_trace(None)
+    raw = np.fromfile(path, np.uint8)
+    assert raw[:8].tobytes() == b"LSTKRTE1"
+    v = raw[8:].view(np.int32)
+    assert v[0:3].tolist() == [2, 8, 2]
+    v = v[3:]
+    assert v[0] == 3
+    v = v[1 + 2 * 3 * 2:]
+    assert v[0] == 2
+    np.testing.assert_array_equal(v[1:9].reshape(2, 2, 2), tr.cpu().numpy())
+    v = v[9:]
+    assert v[0] == 1 and len(v) == 5 and (v[1:] >= 0).all()
