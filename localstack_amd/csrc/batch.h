@@ -46,12 +46,13 @@ struct SampleParams {
     const float *top_p, *min_p, *u;
     int32_t *tokens;
     float *probs;
-    int slices, slice; // work-groups per row and values per slice (sample_plan)
+    int slices, slice; // work-groups per row and 16-byte quads per slice (sample_plan)
     unsigned long long *best; // [n_rows][slices] largest (logit, lowest index) of a slice
     unsigned long long *mass; // [n_rows][kSampleBins]
     uint32_t *count;          // [n_rows][kSampleBins]
-    uint32_t *n_list;         // [n_rows]
-    uint32_t *list;           // [n_rows][n_vocab] indices of the values in the bins where a cut may fall
+    uint32_t *n_list;         // [n_rows] entries of list
+    uint32_t *n_done;         // [n_rows] work-groups of the last launch that are through
+    int *list;                // [n_rows][n_vocab] indices of the values in the bins where a cut may fall
 };
 // Fills slices and slice, and the workspace pointers from `work`; returns the workspace's bytes.
 size_t sample_plan(SampleParams &P, void *work);

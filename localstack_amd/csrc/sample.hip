@@ -35,18 +35,40 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 __device__ __forceinline__ u64 place_of(float x, uint32_t i) { return (u64) key_of(x) << 32 | (uint32_t) ~i; }
 
 struct Row {
-    float temperature, top;
+    float top;
     float step; // bins per unit of x
-    float min_p;
+    double inv_t, min_p;
 };
+// e^z for z <= 0, to 7e-15 of its value; 0 below -40, where it is no whole multiple of 2^-44 any more. e^z = 2^n e^r with
+// |r| <= ln 2 / 2, and e^r by its series to r^11 (the next term is below 6.4e-15).
+__device__ __forceinline__ double exp_scaled(double z, int scale) {
+    const double n = rint(z * 1.4426950408889634);
+    double r = fma(n, -0.6931471803691238, z); // ln 2 in two parts, the first of 33 bits
+    r = fma(n, -1.9082149292705877e-10, r);
+    double p = 1.0 / 39916800;
+    p = fma(p, r, 1.0 / 3628800);
+    p = fma(p, r, 1.0 / 362880);
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return z < -40.0 ? 0.0 : ldexp(p, (int) n + scale);
+}
+// The weight times 2^44 (the largest value's: 2^44 exactly).
 __device__ __forceinline__ double weight_of(const Row &r, float x) {
-    return x == r.top ? 1.0 : exp(((double) x - (double) r.top) / (double) r.temperature);
+    return exp_scaled(((double) x - (double) r.top) * r.inv_t, 44);
 }
 // A value's weight as a whole number; 0 for one that min-p drops. The values that min-p keeps are a run from the top, so
-// the first top_k of them are those of the first top_k values that it keeps.
+// the first top_k of them are those of the first top_k values that it keeps. The sum with 2^52 rounds to a whole number,
+// which is then its mantissa.
 __device__ __forceinline__ u64 mass_of(const Row &r, float x) {
     const double w = weight_of(r, x);
-    return w >= (double) r.min_p ? (u64) __double2ll_rn(w * kUnit) : 0;
+    return w >= r.min_p ? __builtin_bit_cast(u64, w + 0x1p52) & 0xfffffffffffffull : 0;
 }
 __device__ __forceinline__ int bin_of(const Row &r, float x) {
     const float d = r.top - x;
@@ -72,34 +94,85 @@ __device__ __forceinline__ u64 best_of(const SampleParams &P, int b) {
 }
 __device__ __forceinline__ Row row_of(const SampleParams &P, int b, u64 best) {
     Row r;
-    r.temperature = P.temperature ? P.temperature[b] : 1.0f;
+    const float t = P.temperature ? P.temperature[b] : 1.0f;
     r.top = of_key((uint32_t) (best >> 32));
-    r.step = (float) kSampleBins / (kSmRange * r.temperature);
+    r.step = (float) kSampleBins / (kSmRange * t);
+    r.inv_t = 1.0 / (double) t;
     const float p = P.min_p ? P.min_p[b] : 0.0f;
-    r.min_p = p > 0.0f ? fminf(p, 1.0f) : 0.0f;
+    r.min_p = p > 0.0f ? (double) fminf(p, 1.0f) * kUnit : 0.0;
     return r;
 }
 __device__ __forceinline__ bool greedy(const SampleParams &P, int b) { return P.temperature && !(P.temperature[b] > 0.0f); }
 
-// Largest value of each slice, and cleared histograms for the next launch.
+__device__ __forceinline__ uint32_t top_k_of(const SampleParams &P, int b) {
+    const int k = P.top_k ? P.top_k[b] : 0;
+    return k > 0 ? (uint32_t) k : UINT_MAX;
+}
+
+// A row is read as 16-byte quads on 16-byte addresses: quad j holds the values 4 j - off .. + 3, off = the row's offset from
+// such an address. What lies outside the row reads as -inf.
+struct Quads {
+    const float *x;
+    int off, n, first, end; // values of the row; the slice's quads
+};
+__device__ __forceinline__ Quads quads_of(const SampleParams &P, int b, int s) {
+    Quads q;
+    q.x = P.logits + (int64_t) b * P.ld;
+    q.off = (int) (reinterpret_cast<uintptr_t>(q.x) / 4 % 4);
+    q.n = P.n_vocab;
+    q.first = s * P.slice;
+    q.end = min((q.n + q.off + 3) / 4, q.first + P.slice);
+    return q;
+}
+__device__ __forceinline__ float4 quad_at(const Quads &q, int j) {
+    const int i = 4 * j - q.off;
+    if (i >= 0 && i + 4 <= q.n) return *reinterpret_cast<const float4 *>(q.x + i);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = i + e >= 0 && i + e < q.n ? q.x[i + e] : -INFINITY;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+// Calls f(value, index) for the slice's values that are above -inf. kSmAhead quads of a thread are in flight at once.
+constexpr int kSmAhead = 4;
+template <typename F>
+__device__ __forceinline__ void each_value(const Quads &q, F f) {
+    for (int j0 = q.first + (int) threadIdx.x; j0 < q.end; j0 += kSmAhead * kSmThreads) {
+        float4 v[kSmAhead];
+#pragma unroll
+        for (int a = 0; a < kSmAhead; a++)
+            if (j0 + a * kSmThreads < q.end) v[a] = quad_at(q, j0 + a * kSmThreads);
+#pragma unroll
+        for (int a = 0; a < kSmAhead; a++) {
+            const int j = j0 + a * kSmThreads;
+            if (j >= q.end) break;
+            const float w[4] = {v[a].x, v[a].y, v[a].z, v[a].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = value_of(w[e]);
+                if (x > -INFINITY) f(x, 4 * j - q.off + e);
+            }
+        }
+    }
+}
+
+// Largest value of each slice, and cleared histograms and counters for the next launches.
 __global__ __launch_bounds__(kSmThreads) void sample_max_kernel(SampleParams P) {
     __shared__ u64 s_best[kSmThreads / kWave];
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
-    const float *x = P.logits + (int64_t) b * P.ld;
-    const int end = min(P.n_vocab, (s + 1) * P.slice);
-    u64 best = 0;
-    for (int i = s * P.slice + tid; i < end; i += kSmThreads) {
-        const float v = value_of(x[i]);
-        if (v > -INFINITY) {
-            const u64 p = place_of(v, i);
-            best = p > best ? p : best;
+    float top = -INFINITY;
+    int at = 0;
+    each_value(quads_of(P, b, s), [&](float x, int i) {
+        if (x > top) { // a thread's values come in rising order of index
+            top = x;
+            at = i;
         }
-    }
+    });
+    u64 best = top > -INFINITY ? place_of(top, at) : 0;
     for (int i = s * kSmThreads + tid; i < kSampleBins; i += P.slices * kSmThreads) {
         P.mass[(int64_t) b * kSampleBins + i] = 0;
         P.count[(int64_t) b * kSampleBins + i] = 0;
     }
-    if (s == 0 && tid == 0) P.n_list[b] = 0;
+    if (s == 0 && tid == 0) P.n_list[b] = P.n_done[b] = 0u;
     best = wave_max_u64(best);
     if ((tid & (kWave - 1)) == 0) s_best[tid / kWave] = best;
     __syncthreads();
@@ -122,47 +195,53 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SampleParams P)
         s_count[i] = 0;
     }
     __syncthreads();
-    const float *x = P.logits + (int64_t) b * P.ld;
-    const int end = min(P.n_vocab, (s + 1) * P.slice);
-    for (int i = s * P.slice + tid; i < end; i += kSmThreads) {
-        const float v = value_of(x[i]);
-        if (!(v > -INFINITY)) continue;
-        const u64 m = mass_of(r, v);
-        if (m == 0) continue;
-        const int bin = bin_of(r, v);
+    const bool ranked = top_k_of(P, b) != UINT_MAX; // the counts are asked for only where ranks cut
+    each_value(quads_of(P, b, s), [&](float x, int) {
+        const u64 m = mass_of(r, x);
+        if (m == 0) return;
+        const int bin = bin_of(r, x);
         atomicAdd(&s_mass[bin], m);
-        atomicAdd(&s_count[bin], 1u);
-    }
+        if (ranked) atomicAdd(&s_count[bin], 1u);
+    });
     __syncthreads();
     for (int i = tid; i < kSampleBins; i += kSmThreads) {
-        if (s_count[i] == 0) continue;
+        if (s_mass[i] == 0) continue;
         atomicAdd(&P.mass[(int64_t) b * kSampleBins + i], s_mass[i]);
-        atomicAdd(&P.count[(int64_t) b * kSampleBins + i], s_count[i]);
+        if (ranked) atomicAdd(&P.count[(int64_t) b * kSampleBins + i], s_count[i]);
     }
 }
 
-// Inclusive running sums of a row's histogram in LDS.
+// Inclusive running sums of a row's histogram, kept by the threads: bins per * tid .. + per - 1.
+constexpr int kSmPer = kSampleBins / kSmThreads;
 struct Sums {
-    u64 mass[kSampleBins];
-    uint32_t count[kSampleBins];
+    u64 mass[kSmPer], mass0; // through each bin, and before the first
+    uint32_t count[kSmPer], count0;
+};
+struct Found { // a bin in which a running sum reaches its target
+    int bin;
+    u64 mass0, mass;
+    uint32_t count0, count;
+};
+struct SumsLds {
     u64 wave_mass[kSmThreads / kWave];
     uint32_t wave_count[kSmThreads / kWave];
+    Found found[2];
 };
-__device__ __forceinline__ void sums_of(const SampleParams &P, int b, Sums &S) {
-    constexpr int per = kSampleBins / kSmThreads;
+__device__ __forceinline__ Sums sums_of(const SampleParams &P, int b, SumsLds &L) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
-    u64 m[per];
-    uint32_t c[per];
+    Sums S;
     u64 ms = 0;
     uint32_t cs = 0;
-    for (int i = 0; i < per; i++) {
-        ms += P.mass[(int64_t) b * kSampleBins + tid * per + i];
-        cs += P.count[(int64_t) b * kSampleBins + tid * per + i];
-        m[i] = ms;
-        c[i] = cs;
+#pragma unroll
+    for (int i = 0; i < kSmPer; i++) {
+        ms += P.mass[(int64_t) b * kSampleBins + tid * kSmPer + i];
+        cs += P.count[(int64_t) b * kSampleBins + tid * kSmPer + i];
+        S.mass[i] = ms;
+        S.count[i] = cs;
     }
     u64 im = ms;
     uint32_t ic = cs;
+#pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
         const u64 om = __shfl_up(im, d, kWave);
         const uint32_t oc = __shfl_up(ic, d, kWave);
@@ -172,32 +251,39 @@ __device__ __forceinline__ void sums_of(const SampleParams &P, int b, Sums &S) {
         }
     }
     if (lane == kWave - 1) {
-        S.wave_mass[wv] = im;
-        S.wave_count[wv] = ic;
+        L.wave_mass[wv] = im;
+        L.wave_count[wv] = ic;
     }
     __syncthreads();
-    u64 bm = im - ms;
-    uint32_t bc = ic - cs;
+    S.mass0 = im - ms;
+    S.count0 = ic - cs;
     for (int w = 0; w < wv; w++) {
-        bm += S.wave_mass[w];
-        bc += S.wave_count[w];
+        S.mass0 += L.wave_mass[w];
+        S.count0 += L.wave_count[w];
     }
-    for (int i = 0; i < per; i++) {
-        S.mass[tid * per + i] = bm + m[i];
-        S.count[tid * per + i] = bc + c[i];
+#pragma unroll
+    for (int i = 0; i < kSmPer; i++) {
+        S.mass[i] += S.mass0;
+        S.count[i] += S.count0;
+    }
+    return S;
+}
+// The first bins whose running sums reach two targets (found[0], found[1]); a target lies in [1, the whole sum].
+template <bool BY_MASS>
+__device__ __forceinline__ void reaching(const Sums &S, SumsLds &L, u64 t0, u64 t1) {
+    __syncthreads(); // the last call's results have been read
+    u64 m0 = S.mass0;
+    uint32_t c0 = S.count0;
+#pragma unroll
+    for (int i = 0; i < kSmPer; i++) {
+        const u64 before = BY_MASS ? m0 : c0, sum = BY_MASS ? S.mass[i] : S.count[i];
+        const Found f{(int) threadIdx.x * kSmPer + i, m0, S.mass[i], c0, S.count[i]};
+        if (before < t0 && t0 <= sum) L.found[0] = f;
+        if (before < t1 && t1 <= sum) L.found[1] = f;
+        m0 = S.mass[i];
+        c0 = S.count[i];
     }
     __syncthreads();
-}
-// The first bin whose running sum reaches `target` (the last bin if none does).
-template <typename T>
-__device__ __forceinline__ int bin_reaching(const T *sums, T target) {
-    int lo = 0, hi = kSampleBins - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (sums[mid] >= target) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
 }
 
 // The run of the top: how much of M it has to reach, as a whole number in [1, M].
@@ -216,177 +302,244 @@ __device__ __forceinline__ u64 draw_target(const SampleParams &P, int b, u64 S) 
     const u64 t = (u64) floor(u * (double) S) + 1;
     return t > S ? S : t;
 }
-__device__ __forceinline__ uint32_t top_k_of(const SampleParams &P, int b) {
-    const int k = P.top_k ? P.top_k[b] : 0;
-    return k > 0 ? (uint32_t) k : UINT_MAX;
-}
 
-// The bins where a cut may fall. The cut by rank: bin `cut`, inside it where `part` is set (else at its end). What stays, M,
-// lies between the sums before and after that bin, so the run that top-p keeps ends in bins [p_lo, p_hi] (where top-p cuts at
-// all), and the draw in [d_lo, d_hi].
+// The bins where a cut may fall. What stays by rank ends in bin `cut`, inside it where `part` is set (else at its end, or
+// nowhere). The sum of what stays, M, lies between those before and after that bin, so the run that top-p keeps ends in bins
+// [p_lo, p_hi] (where top-p cuts at all), and the draw in [d_lo, d_hi].
 struct Cuts {
     uint32_t k; // values that stay by rank
     bool part, by_p;
-    int cut, p_lo, p_hi, d_lo, d_hi;
+    Found cut;
+    u64 sum; // of what stays by rank, where not `part`
+    int p_lo, p_hi, d_lo, d_hi;
     __device__ __forceinline__ bool holds(int bin) const {
-        return (bin >= d_lo && bin <= d_hi) || (part && bin == cut) || (by_p && bin >= p_lo && bin <= p_hi);
+        return (bin >= d_lo && bin <= d_hi) || (part && bin == cut.bin) || (by_p && bin >= p_lo && bin <= p_hi);
     }
 };
-__device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums &S) {
+__device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums &S, SumsLds &L) {
     Cuts c;
-    c.k = min(top_k_of(P, b), S.count[kSampleBins - 1]);
-    c.cut = bin_reaching(S.count, c.k);
-    c.part = S.count[c.cut] != c.k;
-    // the largest value is in bin 0 and stays, so no sum here is 0
-    const u64 m_hi = S.mass[c.cut], m_lo = !c.part ? m_hi : c.cut > 0 ? S.mass[c.cut - 1] : 1;
-    u64 s_lo = m_lo, s_hi = m_hi;
-    const float p = P.top_p ? P.top_p[b] : 1.0f;
-    c.by_p = p < 1.0f;
-    c.p_lo = c.p_hi = 0;
-    if (c.by_p) {
-        c.p_lo = bin_reaching(S.mass, top_p_target(P, b, m_lo));
-        c.p_hi = bin_reaching(S.mass, top_p_target(P, b, m_hi));
-        s_lo = c.p_lo > 0 ? S.mass[c.p_lo - 1] : 1;
-        s_hi = S.mass[c.p_hi] < m_hi ? S.mass[c.p_hi] : m_hi;
+    u64 m_hi = 0;
+    uint32_t n = 0;
+    for (int w = 0; w < kSmThreads / kWave; w++) {
+        m_hi += L.wave_mass[w];
+        n += L.wave_count[w];
     }
-    c.d_lo = bin_reaching(S.mass, draw_target(P, b, s_lo));
-    c.d_hi = bin_reaching(S.mass, draw_target(P, b, s_hi));
+    u64 m_lo = m_hi;
+    c.k = top_k_of(P, b);
+    c.part = false;
+    if (c.k < n) {
+        reaching<false>(S, L, c.k, c.k);
+        c.cut = L.found[0];
+        c.part = c.cut.count != c.k;
+        m_hi = c.cut.mass;
+        m_lo = !c.part ? m_hi : c.cut.mass0 > 0 ? c.cut.mass0 : 1;
+    }
+    c.sum = m_hi;
+    u64 s_lo = m_lo, s_hi = m_hi;
+    c.by_p = (P.top_p ? P.top_p[b] : 1.0f) < 1.0f;
+    if (c.by_p) {
+        reaching<true>(S, L, top_p_target(P, b, m_lo), top_p_target(P, b, m_hi));
+        c.p_lo = L.found[0].bin;
+        c.p_hi = L.found[1].bin;
+        s_lo = L.found[0].mass0 > 0 ? L.found[0].mass0 : 1;
+        s_hi = L.found[1].mass < m_hi ? L.found[1].mass : m_hi;
+    }
+    reaching<true>(S, L, draw_target(P, b, s_lo), draw_target(P, b, s_hi));
+    c.d_lo = L.found[0].bin;
+    c.d_hi = L.found[1].bin;
     return c;
 }
 
-// Gathers the indices of the values in the bins where a cut may fall.
-__global__ __launch_bounds__(kSmThreads) void sample_collect_kernel(SampleParams P) {
-    __shared__ Sums S;
-    const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
-    if (greedy(P, b)) return;
-    const u64 best = best_of(P, b);
-    if (best == 0) return;
-    const Row r = row_of(P, b, best);
-    sums_of(P, b, S);
-    const Cuts c = cuts_of(P, b, S);
-    const float *x = P.logits + (int64_t) b * P.ld;
-    const int end = min(P.n_vocab, (s + 1) * P.slice);
-    for (int i = s * P.slice + tid; i < end; i += kSmThreads) {
-        const float v = value_of(x[i]);
-        if (v > -INFINITY && c.holds(bin_of(r, v)) && mass_of(r, v) > 0) P.list[(int64_t) b * P.n_vocab + atomicAdd(&P.n_list[b], 1u)] = i;
-    }
-}
-
-// One work-group per row finds the cuts among the gathered values and draws.
-struct Digits {
-    u64 mass[256];
-    uint32_t count[256];
-    u64 place, mass_before;
-    uint32_t count_before;
+// The gathered values, and the search among those of one bin.
+constexpr int kSmKeep = 1024; // gathered values that are kept in LDS; more are read from the list again
+struct Search {
+    u64 place[kSmKeep], mass[kSmKeep];
+    u64 digit_mass[256];
+    uint32_t digit_count[256];
+    u64 hi, lo, at, mass0;
+    uint32_t count0, left;
 };
 struct Reached {
-    u64 place;       // of the value at which the running sum reaches the target
-    u64 mass_before; // running sum before it
+    u64 place; // of the value at which the running sum reaches the target
+    u64 mass0; // running sum before it
 };
-// The value of bin `bin` at which the running sum of weights (by_mass) or of values reaches `target`; `mass0` and `count0`
-// are the sums of the bins before. Found a byte of the place at a time, from the highest: histogram of the byte over the
-// values that share the bytes so far, then the byte in which the sum gets there.
-__device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row &r, Digits &D, int bin, bool by_mass, u64 target, u64 mass0,
-                         uint32_t count0) {
-    const int tid = threadIdx.x;
-    const uint32_t n = P.n_list[b];
+// The value of bin `f` at which the running sum of weights (BY_MASS) or of values reaches `target`, which lies in that bin.
+// The places of the bin's values, as whole numbers, are told apart 8 bits at a time from the first bit in which they differ:
+// a histogram of those bits over the values still in question, and the running sum over it from the top.
+template <bool BY_MASS>
+__device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row &r, Search &D, const Found &f, uint32_t n, u64 target) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const float *x = P.logits + (int64_t) b * P.ld;
-    u64 prefix = 0, mask = 0;
-    if (tid == 0) {
-        D.place = 0;
-        D.mass_before = mass0;
-        D.count_before = count0;
-    }
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        __syncthreads();
-        prefix = D.place;
-        for (int i = tid; i < 256; i += kSmThreads) {
-            D.mass[i] = 0;
-            D.count[i] = 0;
-        }
-        __syncthreads();
+    auto each = [&](auto &&take) {
         for (uint32_t i = tid; i < n; i += kSmThreads) {
-            const uint32_t at = P.list[(int64_t) b * P.n_vocab + i];
-            const float v = value_of(x[at]);
-            const u64 p = place_of(v, at);
-            if (bin_of(r, v) != bin || (p & mask) != prefix) continue;
-            const int digit = (int) (p >> shift & 255);
-            atomicAdd(&D.mass[digit], mass_of(r, v));
-            atomicAdd(&D.count[digit], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            u64 m = D.mass_before;
-            uint32_t c = D.count_before;
-            int digit = 255, last = 255;
-            for (; digit >= 0; digit--) {
-                if (D.count[digit] == 0) continue;
-                last = digit;
-                if (by_mass ? m + D.mass[digit] >= target : c + D.count[digit] >= target) break;
-                m += D.mass[digit];
-                c += D.count[digit];
+            if (n <= (uint32_t) kSmKeep) {
+                const u64 p = D.place[i];
+                if (bin_of(r, of_key((uint32_t) (p >> 32))) == f.bin) take(p, D.mass[i]);
+            } else {
+                const int at = ld_dev(P.list + (int64_t) b * P.n_vocab + i);
+                const float v = value_of(x[at]);
+                if (bin_of(r, v) == f.bin) take(place_of(v, (uint32_t) at), mass_of(r, v));
             }
-            if (digit < 0) { // the sums hold the target, so this is not reached
-                digit = last;
-                m -= D.mass[digit];
-                c -= D.count[digit];
-            }
-            D.mass_before = m;
-            D.count_before = c;
-            D.place = prefix | (u64) digit << shift;
         }
-        mask |= (u64) 255 << shift;
+    };
+    __syncthreads();
+    if (tid == 0) {
+        D.hi = 0;
+        D.lo = ~0ull;
+        D.mass0 = f.mass0;
+        D.count0 = f.count0;
     }
     __syncthreads();
-    const Reached out{D.place, D.mass_before};
+    u64 hi = 0, lo = ~0ull;
+    each([&](u64 p, u64) {
+        hi = p > hi ? p : hi;
+        lo = p < lo ? p : lo;
+    });
+    if (hi >= lo) {
+        atomicMax(&D.hi, hi);
+        atomicMin(&D.lo, lo);
+    }
     __syncthreads();
-    return out;
+    hi = D.hi;
+    // places in question: those that share their bits from `bit` up with `at`
+    u64 at = hi;
+    int bit = hi == D.lo ? 0 : 64 - __clzll((long long) (hi ^ D.lo));
+    while (bit > 0) {
+        const int shift = bit > 8 ? bit - 8 : 0;
+        const u64 above = bit < 64 ? ~0ull << bit : 0;
+        for (int i = tid; i < 256; i += kSmThreads) {
+            D.digit_mass[i] = 0;
+            D.digit_count[i] = 0;
+        }
+        __syncthreads();
+        each([&](u64 p, u64 m) {
+            if ((p ^ at) & above) return;
+            const int d = (int) (p >> shift & 255);
+            atomicAdd(&D.digit_mass[d], m);
+            atomicAdd(&D.digit_count[d], 1u);
+        });
+        __syncthreads();
+        if (tid < kWave) {
+            // lane l takes digits 255 - 4 l .. 252 - 4 l
+            u64 m = 0;
+            uint32_t c = 0;
+            u64 dm[4];
+            uint32_t dc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                dm[i] = D.digit_mass[255 - 4 * lane - i];
+                dc[i] = D.digit_count[255 - 4 * lane - i];
+                m += dm[i];
+                c += dc[i];
+            }
+            u64 im = m;
+            uint32_t ic = c;
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const u64 om = __shfl_up(im, d, kWave);
+                const uint32_t oc = __shfl_up(ic, d, kWave);
+                if (lane >= d) {
+                    im += om;
+                    ic += oc;
+                }
+            }
+            u64 m0 = D.mass0 + im - m;
+            uint32_t c0 = D.count0 + ic - c;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const u64 before = BY_MASS ? m0 : c0, sum = BY_MASS ? m0 + dm[i] : c0 + dc[i];
+                if (before < target && target <= sum) {
+                    D.at = (at & above & ~(255ull << shift)) | (u64) (255 - 4 * lane - i) << shift;
+                    D.left = dc[i];
+                    D.mass0 = m0; // every lane has read the old sums: the wavefront runs in step
+                    D.count0 = c0;
+                }
+                m0 += dm[i];
+                c0 += dc[i];
+            }
+        }
+        __syncthreads();
+        at = D.at;
+        bit = shift;
+        if (D.left == 1) { // one value: its place
+            each([&](u64 p, u64) {
+                if (!((p ^ at) & ~0ull << shift)) D.hi = p;
+            });
+            __syncthreads();
+            at = D.hi;
+            break;
+        }
+    }
+    return {at, D.mass0};
 }
 
+// Gathers the values in the bins where a cut may fall; the row's last work-group to be done finds the cuts among them and
+// draws.
 __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P) {
-    __shared__ Sums S;
-    __shared__ Digits D;
-    const int b = blockIdx.x, tid = threadIdx.x;
+    __shared__ SumsLds L;
+    __shared__ Search D;
+    __shared__ uint32_t s_n;
+    const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
     const u64 best = best_of(P, b);
     if (best == 0 || greedy(P, b)) {
-        if (tid == 0) {
+        if (s == 0 && tid == 0) {
             P.tokens[b] = best == 0 ? -1 : (int32_t) ~(uint32_t) best;
             if (P.probs) P.probs[b] = best == 0 ? 0.0f : 1.0f;
         }
         return;
     }
     const Row r = row_of(P, b, best);
-    sums_of(P, b, S);
-    const Cuts c = cuts_of(P, b, S);
-    auto mass_at = [&](u64 place) { return mass_of(r, of_key((uint32_t) (place >> 32))); };
-    auto before = [&](int bin) { return bin > 0 ? S.mass[bin - 1] : 0; };
-    u64 M = S.mass[c.cut];
-    if (c.part) {
-        const Reached at = reach(P, b, r, D, c.cut, false, c.k, before(c.cut), c.cut > 0 ? S.count[c.cut - 1] : 0);
-        M = at.mass_before + mass_at(at.place);
+    const Sums S = sums_of(P, b, L);
+    const Cuts c = cuts_of(P, b, S, L);
+    int *list = P.list + (int64_t) b * P.n_vocab;
+    each_value(quads_of(P, b, s), [&](float x, int i) {
+        if (c.holds(bin_of(r, x)) && mass_of(r, x) > 0) st_dev(list + atomicAdd(&P.n_list[b], 1u), i);
+    });
+    // Hand-over without an L2 write-back: the entries are device-coherent stores, complete before the work-group counts itself
+    // done, and read with device-coherent loads by the one that counts last.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) s_n = atomicAdd(&P.n_done[b], 1u) + 1 == (uint32_t) P.slices ? atomicAdd(&P.n_list[b], 0u) : UINT_MAX;
+    __syncthreads();
+    const uint32_t n = s_n;
+    if (n == UINT_MAX) return;
+    if (n <= (uint32_t) kSmKeep) {
+        const float *x = P.logits + (int64_t) b * P.ld;
+        for (uint32_t i = tid; i < n; i += kSmThreads) {
+            const int at = ld_dev(list + i);
+            const float v = value_of(x[at]);
+            D.place[i] = place_of(v, (uint32_t) at);
+            D.mass[i] = mass_of(r, v);
+        }
     }
-    u64 total = M;
+    auto mass_at = [&](u64 place) { return mass_of(r, of_key((uint32_t) (place >> 32))); };
+    u64 total = c.sum;
+    if (c.part) {
+        const Reached at = reach<false>(P, b, r, D, c.cut, n, c.k);
+        total = at.mass0 + mass_at(at.place);
+    }
     if (c.by_p) {
-        const u64 target = top_p_target(P, b, M);
-        const int bin = bin_reaching(S.mass, target);
-        const Reached at = reach(P, b, r, D, bin, true, target, before(bin), 0);
-        total = at.mass_before + mass_at(at.place);
+        const u64 target = top_p_target(P, b, total);
+        reaching<true>(S, L, target, target);
+        const Reached at = reach<true>(P, b, r, D, L.found[0], n, target);
+        total = at.mass0 + mass_at(at.place);
     }
     const u64 target = draw_target(P, b, total);
-    const int bin = bin_reaching(S.mass, target);
-    const Reached at = reach(P, b, r, D, bin, true, target, before(bin), 0);
+    reaching<true>(S, L, target, target);
+    const Reached at = reach<true>(P, b, r, D, L.found[0], n, target);
     if (tid == 0) {
         P.tokens[b] = (int32_t) ~(uint32_t) at.place;
-        if (P.probs) P.probs[b] = (float) (weight_of(r, of_key((uint32_t) (at.place >> 32))) * kUnit / (double) total);
+        if (P.probs) P.probs[b] = (float) (weight_of(r, of_key((uint32_t) (at.place >> 32))) / (double) total);
     }
 }
 
 }  // namespace
 
 size_t sample_plan(SampleParams &P, void *work) {
-    // slices of at least 4096 values, as many as bring the launches to 512 work-groups
-    P.slices = std::max(1, std::min((P.n_vocab + 4095) / 4096, 512 / std::max(1, P.n_rows)));
-    P.slice = (P.n_vocab + P.slices - 1) / P.slices;
+    // slices of at least 1024 quads, as many as bring the launches to 512 work-groups; a row out of line has a quad more
+    const int quads = (P.n_vocab + 6) / 4;
+    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, 512 / std::max(1, P.n_rows)));
+    P.slice = (quads + P.slices - 1) / P.slices;
     size_t off = 0;
     auto take = [&](auto *&p, size_t n) {
         p = work ? reinterpret_cast<std::remove_reference_t<decltype(p)>>(static_cast<uint8_t *>(work) + off) : nullptr;
@@ -397,6 +550,7 @@ size_t sample_plan(SampleParams &P, void *work) {
     take(P.mass, rows * kSampleBins);
     take(P.count, rows * kSampleBins);
     take(P.n_list, rows);
+    take(P.n_done, rows);
     take(P.list, rows * P.n_vocab);
     return off;
 }
@@ -407,8 +561,7 @@ hipError_t launch_sample(const SampleParams &P, hipStream_t st) {
     hipError_t e;
     if ((e = launch(sample_max_kernel, all, block, 0, st, nullptr, P)) != hipSuccess) return e;
     if ((e = launch(sample_bins_kernel, all, block, 0, st, nullptr, P)) != hipSuccess) return e;
-    if ((e = launch(sample_collect_kernel, all, block, 0, st, nullptr, P)) != hipSuccess) return e;
-    return launch(sample_pick_kernel, dim3(P.n_rows), block, 0, st, nullptr, P);
+    return launch(sample_pick_kernel, all, block, 0, st, nullptr, P);
 }
 
 }  // namespace lstk
