@@ -21,8 +21,10 @@ typedef unsigned long long u64;
 
 constexpr int kSmThreads = 1024;
 constexpr double kUnit = 0x1p44;
-// (x_max - x) / T of the last bin's lower edge: e^-31 * 2^44 = 0.6, so everything beyond rounds to zero or one step
-constexpr float kSmRange = 31.0f;
+// (x_max - x) / T that the bins cover; the last one starts at 31.2347, where the weight is 0.479 * 2^-44, so all that it
+// holds rounds to zero
+constexpr float kSmRange = 31.25f;
+constexpr double kSmStep = 31.25 / kSampleBins; // of (x_max - x) / T per bin
 
 __device__ __forceinline__ float value_of(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 // order-preserving key of a float
@@ -39,13 +41,19 @@ struct Row {
     float step; // bins per unit of x
     double inv_t, min_p;
 };
-// e^z for z <= 0, to 7e-15 of its value; 0 below -40, where it is no whole multiple of 2^-44 any more. e^z = 2^n e^r with
-// |r| <= ln 2 / 2, and e^r by its series to r^11 (the next term is below 6.4e-15).
-__device__ __forceinline__ double exp_scaled(double z, int scale) {
+__device__ __forceinline__ int bin_of(const Row &r, float x) {
+    const float d = r.top - x;
+    return d == 0.0f ? 0 : (int) fminf(d * r.step, (float) (kSampleBins - 1));
+}
+// e^(-i kSmStep) 2^44, the weight at the edge of bin i: e^z = 2^n e^r with |r| <= ln 2 / 2, and e^r by its series to r^12
+// (what is left out is below 2e-16 of it).
+__device__ __forceinline__ double edge_weight(int i) {
+    const double z = -kSmStep * (double) i;
     const double n = rint(z * 1.4426950408889634);
     double r = fma(n, -0.6931471803691238, z); // ln 2 in two parts, the first of 33 bits
     r = fma(n, -1.9082149292705877e-10, r);
-    double p = 1.0 / 39916800;
+    double p = 1.0 / 479001600;
+    p = fma(p, r, 1.0 / 39916800);
     p = fma(p, r, 1.0 / 3628800);
     p = fma(p, r, 1.0 / 362880);
     p = fma(p, r, 1.0 / 40320);
@@ -57,22 +65,32 @@ __device__ __forceinline__ double exp_scaled(double z, int scale) {
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     p = fma(p, r, 1.0);
-    return z < -40.0 ? 0.0 : ldexp(p, (int) n + scale);
+    return ldexp(p, (int) n + 44);
 }
-// The weight times 2^44 (the largest value's: 2^44 exactly).
-__device__ __forceinline__ double weight_of(const Row &r, float x) {
-    return exp_scaled(((double) x - (double) r.top) * r.inv_t, 44);
+// The weight of a value of bin `bin`, times 2^44 (the largest value's: 2^44 exactly): the edge's, times e^r for the rest, which
+// is at most a bin wide (0.0153), by its series to r^6 (what is left out is below 4e-17; the bin's own fp32 rounding can put a
+// value 2e-6 of a bin beyond its edges, which changes nothing).
+__device__ __forceinline__ double weight_of(const Row &r, float x, int bin, double edge) {
+    const double d = fma((double) bin, kSmStep, ((double) x - (double) r.top) * r.inv_t);
+    double p = 1.0 / 720;
+    p = fma(p, d, 1.0 / 120);
+    p = fma(p, d, 1.0 / 24);
+    p = fma(p, d, 1.0 / 6);
+    p = fma(p, d, 0.5);
+    p = fma(p, d, 1.0);
+    p = fma(p, d, 1.0);
+    return p * edge;
 }
-// A value's weight as a whole number; 0 for one that min-p drops. The values that min-p keeps are a run from the top, so
-// the first top_k of them are those of the first top_k values that it keeps. The sum with 2^52 rounds to a whole number,
-// which is then its mantissa.
+// A value's weight as a whole number; 0 for those of the last bin and for one that min-p drops. The values that min-p keeps
+// are a run from the top, so the first top_k of them are those of the first top_k values that it keeps. The sum with 2^52
+// rounds to a whole number, which is then its mantissa.
+__device__ __forceinline__ u64 mass_of(const Row &r, float x, int bin, double edge) {
+    const double w = weight_of(r, x, bin, edge);
+    return bin < kSampleBins - 1 && w >= r.min_p ? __builtin_bit_cast(u64, w + 0x1p52) & 0xfffffffffffffull : 0;
+}
 __device__ __forceinline__ u64 mass_of(const Row &r, float x) {
-    const double w = weight_of(r, x);
-    return w >= r.min_p ? __builtin_bit_cast(u64, w + 0x1p52) & 0xfffffffffffffull : 0;
-}
-__device__ __forceinline__ int bin_of(const Row &r, float x) {
-    const float d = r.top - x;
-    return d == 0.0f ? 0 : (int) fminf(d * r.step, (float) (kSampleBins - 1));
+    const int bin = bin_of(r, x);
+    return mass_of(r, x, bin, edge_weight(bin));
 }
 
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
@@ -185,6 +203,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_max_kernel(SampleParams P) 
 __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SampleParams P) {
     __shared__ u64 s_mass[kSampleBins];
     __shared__ uint32_t s_count[kSampleBins];
+    __shared__ double s_edge[kSampleBins];
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
     if (greedy(P, b)) return;
     const u64 best = best_of(P, b);
@@ -193,13 +212,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SampleParams P)
     for (int i = tid; i < kSampleBins; i += kSmThreads) {
         s_mass[i] = 0;
         s_count[i] = 0;
+        s_edge[i] = edge_weight(i);
     }
     __syncthreads();
     const bool ranked = top_k_of(P, b) != UINT_MAX; // the counts are asked for only where ranks cut
     each_value(quads_of(P, b, s), [&](float x, int) {
-        const u64 m = mass_of(r, x);
-        if (m == 0) return;
         const int bin = bin_of(r, x);
+        const u64 m = mass_of(r, x, bin, s_edge[bin]);
+        if (m == 0) return;
         atomicAdd(&s_mass[bin], m);
         if (ranked) atomicAdd(&s_count[bin], 1u);
     });
@@ -351,9 +371,14 @@ __device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums
 }
 
 // The gathered values, and the search among those of one bin.
-constexpr int kSmKeep = 1024; // gathered values that are kept in LDS; more are read from the list again
+constexpr int kSmKeep = 1024;           // gathered values that are kept in LDS; more are read from the list again
+constexpr int kSmGather = 2 * kSmKeep; // of a work-group's own, before they go to the list together
 struct Search {
-    u64 place[kSmKeep], mass[kSmKeep];
+    union {
+        u64 place[kSmKeep];
+        int gathered[kSmGather]; // (before the search) this work-group's indices
+    };
+    u64 mass[kSmKeep];
     u64 digit_mass[256];
     uint32_t digit_count[256];
     u64 hi, lo, at, mass0;
@@ -478,7 +503,7 @@ __device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row
 __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P) {
     __shared__ SumsLds L;
     __shared__ Search D;
-    __shared__ uint32_t s_n;
+    __shared__ uint32_t s_n, s_base;
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
     const u64 best = best_of(P, b);
     if (best == 0 || greedy(P, b)) {
@@ -489,12 +514,24 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
         return;
     }
     const Row r = row_of(P, b, best);
+    if (tid == 0) s_n = 0;
     const Sums S = sums_of(P, b, L);
     const Cuts c = cuts_of(P, b, S, L);
     int *list = P.list + (int64_t) b * P.n_vocab;
     each_value(quads_of(P, b, s), [&](float x, int i) {
-        if (c.holds(bin_of(r, x)) && mass_of(r, x) > 0) st_dev(list + atomicAdd(&P.n_list[b], 1u), i);
+        const int bin = bin_of(r, x);
+        if (!c.holds(bin) || mass_of(r, x, bin, edge_weight(bin)) == 0) return;
+        const uint32_t at = atomicAdd(&s_n, 1u);
+        if (at < (uint32_t) kSmGather) D.gathered[at] = i;
+        else st_dev(list + atomicAdd(&P.n_list[b], 1u), i);
     });
+    // one place in the list for all that fitted (a global counter's answer takes a microsecond: one each, and a wavefront that
+    // meets 20 such values takes 20)
+    __syncthreads();
+    const uint32_t mine = min(s_n, (uint32_t) kSmGather);
+    if (tid == 0 && mine > 0) s_base = atomicAdd(&P.n_list[b], mine);
+    __syncthreads();
+    for (uint32_t i = tid; i < mine; i += kSmThreads) st_dev(list + s_base + i, D.gathered[i]);
     // Hand-over without an L2 write-back: the entries are device-coherent stores, complete before the work-group counts itself
     // done, and read with device-coherent loads by the one that counts last.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -529,7 +566,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     const Reached at = reach<true>(P, b, r, D, L.found[0], n, target);
     if (tid == 0) {
         P.tokens[b] = (int32_t) ~(uint32_t) at.place;
-        if (P.probs) P.probs[b] = (float) (weight_of(r, of_key((uint32_t) (at.place >> 32))) / (double) total);
+        const float x = of_key((uint32_t) (at.place >> 32));
+        const int bin = bin_of(r, x);
+        if (P.probs) P.probs[b] = (float) (weight_of(r, x, bin, edge_weight(bin)) / (double) total);
     }
 }
 
@@ -538,7 +577,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
 size_t sample_plan(SampleParams &P, void *work) {
     // slices of at least 1024 quads, as many as bring the launches to 512 work-groups; a row out of line has a quad more
     const int quads = (P.n_vocab + 6) / 4;
-    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, 512 / std::max(1, P.n_rows)));
+    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, 256 / std::max(1, P.n_rows)));
     P.slice = (quads + P.slices - 1) / P.slices;
     size_t off = 0;
     auto take = [&](auto *&p, size_t n) {
