@@ -10,6 +10,7 @@
 // counts and weights over kSampleBins equal steps of (x_max - x) / T says in which bins the three cuts fall; only those
 // bins' values are looked at one by one. Weights that round to zero cannot be drawn and take no part.
 #include <cfloat>
+#include <type_traits>
 
 #include "batch.h"
 #include "device.h"
@@ -23,8 +24,8 @@ constexpr int kSmThreads = 1024;
 constexpr double kUnit = 0x1p44;
 // (x_max - x) / T that the bins cover; the last one starts at 31.2347, where the weight is 0.479 * 2^-44, so all that it
 // holds rounds to zero
-constexpr float kSmRange = 31.25f;
-constexpr double kSmStep = 31.25 / kSampleBins; // of (x_max - x) / T per bin
+constexpr double kSmRange = 31.25;
+constexpr double kSmStep = kSmRange / kSampleBins; // of (x_max - x) / T per bin
 
 __device__ __forceinline__ float value_of(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
 // order-preserving key of a float
@@ -37,14 +38,19 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 __device__ __forceinline__ u64 place_of(float x, uint32_t i) { return (u64) key_of(x) << 32 | (uint32_t) ~i; }
 
 struct Row {
-    float top;
-    float step; // bins per unit of x
-    double inv_t, min_p;
+    double top;   // the largest value
+    double scale; // bins per unit of x
+    double min_p; // in units of 2^-44
+    float least;  // nothing below has a weight, -inf and NaN among it (a little lower than need be)
 };
-__device__ __forceinline__ int bin_of(const Row &r, float x) {
-    const float d = r.top - x;
-    return d == 0.0f ? 0 : (int) fminf(d * r.step, (float) (kSampleBins - 1));
+// The largest float that is at most x, or one a few steps lower; at least the lowest finite one.
+__device__ __forceinline__ float float_below(double x) {
+    const float f = (float) fmin(fmax(x, (double) -FLT_MAX), (double) FLT_MAX);
+    return fmaxf(f - fabsf(f) * 0x1p-22f - FLT_MIN, -FLT_MAX);
 }
+// How many bins below the largest value x lies, up to the last bin's edge.
+__device__ __forceinline__ double bins_below(const Row &r, float x) { return fmin((r.top - (double) x) * r.scale, (double) (kSampleBins - 1)); }
+__device__ __forceinline__ int bin_of(const Row &r, float x) { return (int) bins_below(r, x); }
 // e^(-i kSmStep) 2^44, the weight at the edge of bin i: e^z = 2^n e^r with |r| <= ln 2 / 2, and e^r by its series to r^12
 // (what is left out is below 2e-16 of it).
 __device__ __forceinline__ double edge_weight(int i) {
@@ -67,30 +73,29 @@ __device__ __forceinline__ double edge_weight(int i) {
     p = fma(p, r, 1.0);
     return ldexp(p, (int) n + 44);
 }
-// The weight of a value of bin `bin`, times 2^44 (the largest value's: 2^44 exactly): the edge's, times e^r for the rest, which
-// is at most a bin wide (0.0153), by its series to r^6 (what is left out is below 4e-17; the bin's own fp32 rounding can put a
-// value 2e-6 of a bin beyond its edges, which changes nothing).
-__device__ __forceinline__ double weight_of(const Row &r, float x, int bin, double edge) {
-    const double d = fma((double) bin, kSmStep, ((double) x - (double) r.top) * r.inv_t);
-    double p = 1.0 / 720;
-    p = fma(p, d, 1.0 / 120);
-    p = fma(p, d, 1.0 / 24);
-    p = fma(p, d, 1.0 / 6);
-    p = fma(p, d, 0.5);
-    p = fma(p, d, 1.0);
-    p = fma(p, d, 1.0);
+// The weight of a value `below` bins from the largest, times 2^44 (the largest value's: 2^44 exactly): that of its bin's edge,
+// times e^-r for the rest of a bin r < kSmStep = 0.0153, by its series to r^5 (what is left out is below 1.8e-14).
+__device__ __forceinline__ double weight_of(double below, int bin, double edge) {
+    constexpr double h = kSmStep;
+    const double f = below - (double) bin;
+    double p = -h * h * h * h * h / 120;
+    p = fma(p, f, h * h * h * h / 24);
+    p = fma(p, f, -h * h * h / 6);
+    p = fma(p, f, h * h / 2);
+    p = fma(p, f, -h);
+    p = fma(p, f, 1.0);
     return p * edge;
 }
 // A value's weight as a whole number; 0 for those of the last bin and for one that min-p drops. The values that min-p keeps
 // are a run from the top, so the first top_k of them are those of the first top_k values that it keeps. The sum with 2^52
 // rounds to a whole number, which is then its mantissa.
-__device__ __forceinline__ u64 mass_of(const Row &r, float x, int bin, double edge) {
-    const double w = weight_of(r, x, bin, edge);
+__device__ __forceinline__ u64 mass_of(const Row &r, double below, int bin, double edge) {
+    const double w = weight_of(below, bin, edge);
     return bin < kSampleBins - 1 && w >= r.min_p ? __builtin_bit_cast(u64, w + 0x1p52) & 0xfffffffffffffull : 0;
 }
 __device__ __forceinline__ u64 mass_of(const Row &r, float x) {
-    const int bin = bin_of(r, x);
-    return mass_of(r, x, bin, edge_weight(bin));
+    const double below = bins_below(r, x);
+    return mass_of(r, below, (int) below, edge_weight((int) below));
 }
 
 __device__ __forceinline__ u64 wave_max_u64(u64 v) {
@@ -110,21 +115,27 @@ __device__ __forceinline__ u64 best_of(const SampleParams &P, int b) {
     }
     return wave_max_u64(v);
 }
-__device__ __forceinline__ Row row_of(const SampleParams &P, int b, u64 best) {
-    Row r;
-    const float t = P.temperature ? P.temperature[b] : 1.0f;
-    r.top = of_key((uint32_t) (best >> 32));
-    r.step = (float) kSampleBins / (kSmRange * t);
-    r.inv_t = 1.0 / (double) t;
-    const float p = P.min_p ? P.min_p[b] : 0.0f;
-    r.min_p = p > 0.0f ? (double) fminf(p, 1.0f) * kUnit : 0.0;
-    return r;
-}
-__device__ __forceinline__ bool greedy(const SampleParams &P, int b) { return P.temperature && !(P.temperature[b] > 0.0f); }
-
-__device__ __forceinline__ uint32_t top_k_of(const SampleParams &P, int b) {
+// A row's settings, asked for together at a kernel's start (each would be a wait of its own where it is used).
+struct Settings {
+    float t, p, min_p, u;
+    uint32_t k;
+    bool greedy;
+};
+__device__ __forceinline__ Settings settings_of(const SampleParams &P, int b) {
+    const float t = P.temperature ? P.temperature[b] : 1.0f, p = P.top_p ? P.top_p[b] : 1.0f, min_p = P.min_p ? P.min_p[b] : 0.0f;
     const int k = P.top_k ? P.top_k[b] : 0;
-    return k > 0 ? (uint32_t) k : UINT_MAX;
+    const float u = P.u[b];
+    return {t, p, min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f, u, k > 0 ? (uint32_t) k : UINT_MAX, !(t > 0.0f)};
+}
+__device__ __forceinline__ Row row_of(const Settings &how, u64 best) {
+    Row r;
+    r.top = (double) of_key((uint32_t) (best >> 32));
+    r.scale = (double) kSampleBins / (kSmRange * (double) how.t);
+    r.min_p = (double) how.min_p * kUnit;
+    double range = kSmRange;
+    if (how.min_p > 0.0f) range = fmin(range, 1e-6 - log((double) how.min_p));
+    r.least = float_below(r.top - range * (double) how.t);
+    return r;
 }
 
 // A row is read as 16-byte quads on 16-byte addresses: quad j holds the values 4 j - off .. + 3, off = the row's offset from
@@ -150,26 +161,37 @@ __device__ __forceinline__ float4 quad_at(const Quads &q, int j) {
     for (int e = 0; e < 4; e++) v[e] = i + e >= 0 && i + e < q.n ? q.x[i + e] : -INFINITY;
     return make_float4(v[0], v[1], v[2], v[3]);
 }
-// Calls f(value, index) for the slice's values that are above -inf. kSmAhead quads of a thread are in flight at once.
+// kSmAhead quads of a thread are in flight at once; the first ones may be asked for long before they are needed.
 constexpr int kSmAhead = 4;
+struct Ahead {
+    float4 v[kSmAhead];
+};
+__device__ __forceinline__ Ahead ahead_of(const Quads &q, int j0) {
+    Ahead a;
+#pragma unroll
+    for (int i = 0; i < kSmAhead; i++) {
+        const int j = j0 + i * kSmThreads;
+        a.v[i] = j < q.end ? quad_at(q, j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    return a;
+}
+// Calls f(value as stored, index) for the slice's values and some -inf beyond, a thread's in rising order of index; `a` =
+// ahead_of(q, q.first + threadIdx.x).
 template <typename F>
-__device__ __forceinline__ void each_value(const Quads &q, F f) {
-    for (int j0 = q.first + (int) threadIdx.x; j0 < q.end; j0 += kSmAhead * kSmThreads) {
-        float4 v[kSmAhead];
+__device__ __forceinline__ void each_value(const Quads &q, Ahead a, F f) {
+    for (int j0 = q.first + (int) threadIdx.x; j0 < q.end;) {
+        const Ahead now = a;
+        const int j1 = j0 + kSmAhead * kSmThreads;
+        if (j1 < q.end) a = ahead_of(q, j1);
 #pragma unroll
-        for (int a = 0; a < kSmAhead; a++)
-            if (j0 + a * kSmThreads < q.end) v[a] = quad_at(q, j0 + a * kSmThreads);
-#pragma unroll
-        for (int a = 0; a < kSmAhead; a++) {
-            const int j = j0 + a * kSmThreads;
-            if (j >= q.end) break;
-            const float w[4] = {v[a].x, v[a].y, v[a].z, v[a].w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float x = value_of(w[e]);
-                if (x > -INFINITY) f(x, 4 * j - q.off + e);
-            }
+        for (int i = 0; i < kSmAhead; i++) {
+            const int at = 4 * (j0 + i * kSmThreads) - q.off;
+            f(now.v[i].x, at);
+            f(now.v[i].y, at + 1);
+            f(now.v[i].z, at + 2);
+            f(now.v[i].w, at + 3);
         }
+        j0 = j1;
     }
 }
 
@@ -179,8 +201,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_max_kernel(SampleParams P) 
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
     float top = -INFINITY;
     int at = 0;
-    each_value(quads_of(P, b, s), [&](float x, int i) {
-        if (x > top) { // a thread's values come in rising order of index
+    const Quads q = quads_of(P, b, s);
+    each_value(q, ahead_of(q, q.first + tid), [&](float x, int i) {
+        x = x > FLT_MAX ? FLT_MAX : x;
+        if (x > top) { // (a NaN is not)
             top = x;
             at = i;
         }
@@ -205,20 +229,25 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SampleParams P)
     __shared__ uint32_t s_count[kSampleBins];
     __shared__ double s_edge[kSampleBins];
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
-    if (greedy(P, b)) return;
+    const Settings how = settings_of(P, b);
+    if (how.greedy) return;
+    const Quads q = quads_of(P, b, s);
+    const Ahead ahead = ahead_of(q, q.first + tid);
+    const bool ranked = how.k != UINT_MAX; // the counts are asked for only where ranks cut
     const u64 best = best_of(P, b);
     if (best == 0) return;
-    const Row r = row_of(P, b, best);
     for (int i = tid; i < kSampleBins; i += kSmThreads) {
         s_mass[i] = 0;
         s_count[i] = 0;
         s_edge[i] = edge_weight(i);
     }
+    const Row r = row_of(how, best);
     __syncthreads();
-    const bool ranked = top_k_of(P, b) != UINT_MAX; // the counts are asked for only where ranks cut
-    each_value(quads_of(P, b, s), [&](float x, int) {
-        const int bin = bin_of(r, x);
-        const u64 m = mass_of(r, x, bin, s_edge[bin]);
+    each_value(q, ahead, [&](float x, int) {
+        if (!(x >= r.least)) return;
+        const double below = bins_below(r, fminf(x, FLT_MAX));
+        const int bin = (int) below;
+        const u64 m = mass_of(r, below, bin, s_edge[bin]);
         if (m == 0) return;
         atomicAdd(&s_mass[bin], m);
         if (ranked) atomicAdd(&s_count[bin], 1u);
@@ -247,15 +276,15 @@ struct SumsLds {
     uint32_t wave_count[kSmThreads / kWave];
     Found found[2];
 };
-__device__ __forceinline__ Sums sums_of(const SampleParams &P, int b, SumsLds &L) {
+__device__ __forceinline__ Sums sums_of(const u64 *mass, const uint32_t *count, SumsLds &L) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
     Sums S;
     u64 ms = 0;
     uint32_t cs = 0;
 #pragma unroll
     for (int i = 0; i < kSmPer; i++) {
-        ms += P.mass[(int64_t) b * kSampleBins + tid * kSmPer + i];
-        cs += P.count[(int64_t) b * kSampleBins + tid * kSmPer + i];
+        ms += mass[tid * kSmPer + i];
+        cs += count[tid * kSmPer + i];
         S.mass[i] = ms;
         S.count[i] = cs;
     }
@@ -307,19 +336,17 @@ __device__ __forceinline__ void reaching(const Sums &S, SumsLds &L, u64 t0, u64 
 }
 
 // The run of the top: how much of M it has to reach, as a whole number in [1, M].
-__device__ __forceinline__ u64 top_p_target(const SampleParams &P, int b, u64 M) {
-    const float p = P.top_p ? P.top_p[b] : 1.0f;
-    if (!(p < 1.0f)) return M;
-    if (!(p > 0.0f)) return 1;
-    const u64 t = (u64) ceil((double) p * (double) M);
+__device__ __forceinline__ u64 top_p_target(const Settings &how, u64 M) {
+    if (!(how.p < 1.0f)) return M;
+    if (!(how.p > 0.0f)) return 1;
+    const u64 t = (u64) ceil((double) how.p * (double) M);
     return t < 1 ? 1 : t > M ? M : t;
 }
 // The least whole running sum above u S, in [1, S].
-__device__ __forceinline__ u64 draw_target(const SampleParams &P, int b, u64 S) {
-    const double u = (double) P.u[b];
-    if (!(u > 0.0)) return 1;
-    if (u >= 1.0) return S;
-    const u64 t = (u64) floor(u * (double) S) + 1;
+__device__ __forceinline__ u64 draw_target(const Settings &how, u64 S) {
+    if (!(how.u > 0.0f)) return 1;
+    if (how.u >= 1.0f) return S;
+    const u64 t = (u64) floor((double) how.u * (double) S) + 1;
     return t > S ? S : t;
 }
 
@@ -336,7 +363,7 @@ struct Cuts {
         return (bin >= d_lo && bin <= d_hi) || (part && bin == cut.bin) || (by_p && bin >= p_lo && bin <= p_hi);
     }
 };
-__device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums &S, SumsLds &L) {
+__device__ __forceinline__ Cuts cuts_of(const Settings &how, const Sums &S, SumsLds &L) {
     Cuts c;
     u64 m_hi = 0;
     uint32_t n = 0;
@@ -345,7 +372,7 @@ __device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums
         n += L.wave_count[w];
     }
     u64 m_lo = m_hi;
-    c.k = top_k_of(P, b);
+    c.k = how.k;
     c.part = false;
     if (c.k < n) {
         reaching<false>(S, L, c.k, c.k);
@@ -356,55 +383,130 @@ __device__ __forceinline__ Cuts cuts_of(const SampleParams &P, int b, const Sums
     }
     c.sum = m_hi;
     u64 s_lo = m_lo, s_hi = m_hi;
-    c.by_p = (P.top_p ? P.top_p[b] : 1.0f) < 1.0f;
+    c.by_p = how.p < 1.0f;
     if (c.by_p) {
-        reaching<true>(S, L, top_p_target(P, b, m_lo), top_p_target(P, b, m_hi));
+        reaching<true>(S, L, top_p_target(how, m_lo), top_p_target(how, m_hi));
         c.p_lo = L.found[0].bin;
         c.p_hi = L.found[1].bin;
         s_lo = L.found[0].mass0 > 0 ? L.found[0].mass0 : 1;
         s_hi = L.found[1].mass < m_hi ? L.found[1].mass : m_hi;
     }
-    reaching<true>(S, L, draw_target(P, b, s_lo), draw_target(P, b, s_hi));
+    reaching<true>(S, L, draw_target(how, s_lo), draw_target(how, s_hi));
     c.d_lo = L.found[0].bin;
     c.d_hi = L.found[1].bin;
     return c;
 }
 
-// The gathered values, and the search among those of one bin.
-constexpr int kSmKeep = 1024;           // gathered values that are kept in LDS; more are read from the list again
-constexpr int kSmGather = 2 * kSmKeep; // of a work-group's own, before they go to the list together
+// The search among the gathered values. Up to kSmKeep of them are sorted by place (larger first) once, with the running sum of
+// their weights; more are left in the list, and told apart there by digits.
+constexpr int kSmKeep = 1024;
+constexpr int kSmGather = 2 * kSmKeep; // indices that a work-group gathers before they go to the list together
 struct Search {
     union {
-        u64 place[kSmKeep];
-        int gathered[kSmGather]; // (before the search) this work-group's indices
+        struct {
+            u64 place[kSmKeep], before[kSmKeep]; // sorted, and the sum of the weights before each
+        };
+        int gathered[kSmGather];
+        struct {
+            u64 digit_mass[256];
+            uint32_t digit_count[256];
+            u64 hi, lo, at;
+            uint32_t count0, left;
+        };
     };
-    u64 mass[kSmKeep];
-    u64 digit_mass[256];
-    uint32_t digit_count[256];
-    u64 hi, lo, at, mass0;
-    uint32_t count0, left;
+    u64 wave_mass[kSmThreads / kWave];
+    u64 found, mass0; // answer
+    u64 base;         // sum of the weights before the bin's first value
+    int first;        // and its index
 };
 struct Reached {
     u64 place; // of the value at which the running sum reaches the target
     u64 mass0; // running sum before it
 };
+
+// Sorts the places of `n` values (index_at(i), i < n <= kSmKeep) and sums their weights.
+template <typename F>
+__device__ __forceinline__ void sort_gathered(const Row &r, const float *x, Search &D, int n, F index_at) {
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
+    u64 mine = 0;
+    if (tid < n) {
+        const int at = index_at(tid);
+        mine = place_of(value_of(x[at]), (uint32_t) at);
+    }
+    __syncthreads(); // index_at may read what is written now
+    D.place[tid] = mine;
+    __syncthreads();
+    int size = 1;
+    while (size < n) size *= 2;
+    for (int run = 2; run <= size; run *= 2) {
+        for (int step = run / 2; step > 0; step /= 2) {
+            const int other = tid ^ step;
+            u64 a = 0;
+            if (tid < size) {
+                a = D.place[tid];
+                const u64 o = D.place[other];
+                const bool larger = ((tid & run) == 0) == (tid < other); // the larger of the two comes here
+                a = (o > a) == larger ? o : a;
+            }
+            __syncthreads();
+            if (tid < size) D.place[tid] = a;
+            __syncthreads();
+        }
+    }
+    mine = D.place[tid];
+    const u64 m = tid < n ? mass_of(r, of_key((uint32_t) (mine >> 32))) : 0;
+    u64 sum = m;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const u64 o = __shfl_up(sum, d, kWave);
+        if (lane >= d) sum += o;
+    }
+    if (lane == kWave - 1) D.wave_mass[wv] = sum;
+    __syncthreads();
+    sum -= m;
+    for (int w = 0; w < wv; w++) sum += D.wave_mass[w];
+    D.before[tid] = sum;
+    __syncthreads();
+}
+
 // The value of bin `f` at which the running sum of weights (BY_MASS) or of values reaches `target`, which lies in that bin.
-// The places of the bin's values, as whole numbers, are told apart 8 bits at a time from the first bit in which they differ:
-// a histogram of those bits over the values still in question, and the running sum over it from the top.
 template <bool BY_MASS>
-__device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row &r, Search &D, const Found &f, uint32_t n, u64 target) {
+__device__ __forceinline__ Reached reach_sorted(const Row &r, Search &D, const Found &f, int n, u64 target) {
+    const int tid = threadIdx.x;
+    const u64 place = tid < n ? D.place[tid] : 0;
+    const float x = of_key((uint32_t) (place >> 32));
+    const bool here = tid < n && bin_of(r, x) == f.bin;
+    if (here && (tid == 0 || bin_of(r, of_key((uint32_t) (D.place[tid - 1] >> 32))) != f.bin)) {
+        D.first = tid;
+        D.base = D.before[tid];
+    }
+    __syncthreads();
+    if (here) {
+        const u64 mass0 = f.mass0 + D.before[tid] - D.base;
+        const u64 before = BY_MASS ? mass0 : f.count0 + (uint32_t) (tid - D.first);
+        if (before < target && target <= before + (BY_MASS ? mass_of(r, x) : 1)) {
+            D.found = place;
+            D.mass0 = mass0;
+        }
+    }
+    __syncthreads();
+    const Reached out{D.found, D.mass0};
+    __syncthreads();
+    return out;
+}
+
+// The same among the n entries of the list: the places of the bin's values, as whole numbers, are told apart 8 bits at a time
+// from the first bit in which they differ, by a histogram of those bits over the values still in question and the running sum
+// over it from the top.
+template <bool BY_MASS>
+__device__ __forceinline__ Reached reach_in_list(const Row &r, const float *x, const int *list, Search &D, const Found &f, uint32_t n,
+                                                 u64 target) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
-    const float *x = P.logits + (int64_t) b * P.ld;
     auto each = [&](auto &&take) {
         for (uint32_t i = tid; i < n; i += kSmThreads) {
-            if (n <= (uint32_t) kSmKeep) {
-                const u64 p = D.place[i];
-                if (bin_of(r, of_key((uint32_t) (p >> 32))) == f.bin) take(p, D.mass[i]);
-            } else {
-                const int at = ld_dev(P.list + (int64_t) b * P.n_vocab + i);
-                const float v = value_of(x[at]);
-                if (bin_of(r, v) == f.bin) take(place_of(v, (uint32_t) at), mass_of(r, v));
-            }
+            const int at = ld_dev(list + i);
+            const float v = value_of(x[at]);
+            if (bin_of(r, v) == f.bin) take(place_of(v, (uint32_t) at), v);
         }
     };
     __syncthreads();
@@ -416,7 +518,7 @@ __device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row
     }
     __syncthreads();
     u64 hi = 0, lo = ~0ull;
-    each([&](u64 p, u64) {
+    each([&](u64 p, float) {
         hi = p > hi ? p : hi;
         lo = p < lo ? p : lo;
     });
@@ -437,10 +539,10 @@ __device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row
             D.digit_count[i] = 0;
         }
         __syncthreads();
-        each([&](u64 p, u64 m) {
+        each([&](u64 p, float v) {
             if ((p ^ at) & above) return;
             const int d = (int) (p >> shift & 255);
-            atomicAdd(&D.digit_mass[d], m);
+            atomicAdd(&D.digit_mass[d], mass_of(r, v));
             atomicAdd(&D.digit_count[d], 1u);
         });
         __syncthreads();
@@ -487,7 +589,7 @@ __device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row
         at = D.at;
         bit = shift;
         if (D.left == 1) { // one value: its place
-            each([&](u64 p, u64) {
+            each([&](u64 p, float) {
                 if (!((p ^ at) & ~0ull << shift)) D.hi = p;
             });
             __syncthreads();
@@ -498,6 +600,43 @@ __device__ __forceinline__ Reached reach(const SampleParams &P, int b, const Row
     return {at, D.mass0};
 }
 
+// The cuts and the draw. reach(by_mass, bin, target) is one of the two above.
+template <typename F>
+__device__ __forceinline__ void draw(const SampleParams &P, const Settings &how, int b, const Row &r, const Cuts &c, const Sums &S, SumsLds &L, F reach) {
+    auto mass_at = [&](u64 place) { return mass_of(r, of_key((uint32_t) (place >> 32))); };
+    u64 total = c.sum;
+    if (c.part) {
+        const Reached at = reach(std::false_type(), c.cut, c.k);
+        total = at.mass0 + mass_at(at.place);
+    }
+    if (c.by_p) {
+        const u64 target = top_p_target(how, total);
+        reaching<true>(S, L, target, target);
+        const Reached at = reach(std::true_type(), L.found[0], target);
+        total = at.mass0 + mass_at(at.place);
+    }
+    const u64 target = draw_target(how, total);
+    reaching<true>(S, L, target, target);
+    const Reached at = reach(std::true_type(), L.found[0], target);
+    if (threadIdx.x == 0) {
+        P.tokens[b] = (int32_t) ~(uint32_t) at.place;
+        const double below = bins_below(r, of_key((uint32_t) (at.place >> 32)));
+        if (P.probs) P.probs[b] = (float) (weight_of(below, (int) below, edge_weight((int) below)) / (double) total);
+    }
+}
+
+// The values from bin `lo` to bin `hi`, and a few steps more on either side.
+struct Span {
+    float least, most;
+    __device__ __forceinline__ bool holds(float x) const { return x >= least && x <= most; } // (no NaN)
+};
+__device__ __forceinline__ Span span_of(const Row &r, int lo, int hi) {
+    Span s;
+    s.least = float_below(r.top - (double) (hi + 1) / r.scale);
+    s.most = lo == 0 ? INFINITY : -float_below((double) lo / r.scale - r.top);
+    return s;
+}
+
 // Gathers the values in the bins where a cut may fall; the row's last work-group to be done finds the cuts among them and
 // draws.
 __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P) {
@@ -505,22 +644,29 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     __shared__ Search D;
     __shared__ uint32_t s_n, s_base;
     const int b = blockIdx.x / P.slices, s = blockIdx.x % P.slices, tid = threadIdx.x;
+    const Settings how = settings_of(P, b);
+    const Quads q = quads_of(P, b, s);
+    const Ahead ahead = ahead_of(q, q.first + tid);
     const u64 best = best_of(P, b);
-    if (best == 0 || greedy(P, b)) {
+    if (best == 0 || how.greedy) {
         if (s == 0 && tid == 0) {
             P.tokens[b] = best == 0 ? -1 : (int32_t) ~(uint32_t) best;
             if (P.probs) P.probs[b] = best == 0 ? 0.0f : 1.0f;
         }
         return;
     }
-    const Row r = row_of(P, b, best);
     if (tid == 0) s_n = 0;
-    const Sums S = sums_of(P, b, L);
-    const Cuts c = cuts_of(P, b, S, L);
+    const Sums S = sums_of(P.mass + (int64_t) b * kSampleBins, P.count + (int64_t) b * kSampleBins, L);
+    const Row r = row_of(how, best);
+    const Cuts c = cuts_of(how, S, L);
     int *list = P.list + (int64_t) b * P.n_vocab;
-    each_value(quads_of(P, b, s), [&](float x, int i) {
-        const int bin = bin_of(r, x);
-        if (!c.holds(bin) || mass_of(r, x, bin, edge_weight(bin)) == 0) return;
+    const Span drawn = span_of(r, c.d_lo, c.d_hi);
+    const Span ranked = c.part ? span_of(r, c.cut.bin, c.cut.bin) : drawn, run = c.by_p ? span_of(r, c.p_lo, c.p_hi) : drawn;
+    each_value(q, ahead, [&](float x, int i) {
+        if (!(drawn.holds(x) || ranked.holds(x) || run.holds(x))) return;
+        const double below = bins_below(r, fminf(x, FLT_MAX));
+        const int bin = (int) below;
+        if (!c.holds(bin) || mass_of(r, below, bin, edge_weight(bin)) == 0) return;
         const uint32_t at = atomicAdd(&s_n, 1u);
         if (at < (uint32_t) kSmGather) D.gathered[at] = i;
         else st_dev(list + atomicAdd(&P.n_list[b], 1u), i);
@@ -541,34 +687,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     const uint32_t n = s_n;
     if (n == UINT_MAX) return;
     if (n <= (uint32_t) kSmKeep) {
-        const float *x = P.logits + (int64_t) b * P.ld;
-        for (uint32_t i = tid; i < n; i += kSmThreads) {
-            const int at = ld_dev(list + i);
-            const float v = value_of(x[at]);
-            D.place[i] = place_of(v, (uint32_t) at);
-            D.mass[i] = mass_of(r, v);
-        }
-    }
-    auto mass_at = [&](u64 place) { return mass_of(r, of_key((uint32_t) (place >> 32))); };
-    u64 total = c.sum;
-    if (c.part) {
-        const Reached at = reach<false>(P, b, r, D, c.cut, n, c.k);
-        total = at.mass0 + mass_at(at.place);
-    }
-    if (c.by_p) {
-        const u64 target = top_p_target(P, b, total);
-        reaching<true>(S, L, target, target);
-        const Reached at = reach<true>(P, b, r, D, L.found[0], n, target);
-        total = at.mass0 + mass_at(at.place);
-    }
-    const u64 target = draw_target(P, b, total);
-    reaching<true>(S, L, target, target);
-    const Reached at = reach<true>(P, b, r, D, L.found[0], n, target);
-    if (tid == 0) {
-        P.tokens[b] = (int32_t) ~(uint32_t) at.place;
-        const float x = of_key((uint32_t) (at.place >> 32));
-        const int bin = bin_of(r, x);
-        if (P.probs) P.probs[b] = (float) (weight_of(r, x, bin, edge_weight(bin)) / (double) total);
+        sort_gathered(r, q.x, D, (int) n, [&](int i) { return ld_dev(list + i); });
+        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_sorted<by_mass>(r, D, f, (int) n, target); });
+    } else {
+        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_in_list<by_mass>(r, q.x, list, D, f, n, target); });
     }
 }
 
