@@ -284,64 +284,66 @@ def unpack_matrix(type_, rows, cols, packed):
 
 
 # ---- operators of a step over many sequences -------------------------------------------------------
+# A call that takes the device a few microseconds is bound by what Python does around it, so the checks below look at each
+# tensor once, in the cheapest order, and build a message only when one fails.
 
-def _tensor(t, name, dtype, shape, like=None):
-    """Checks a device tensor's dtype, shape (None: any size), layout (rows one after the other) and device."""
-    if not hasattr(t, "data_ptr") or t.dtype != dtype or t.dim() != len(shape) or \
-            any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        want = "x".join("n" if w is None else str(w) for w in shape)
-        raise LstkError(E_INVALID, f"{name} must be a {dtype} tensor of shape {want}, got "
-                                   f"{getattr(t, 'dtype', type(t))} {tuple(getattr(t, 'shape', ()))}")
-    if not t.is_contiguous():
-        raise LstkError(E_INVALID, f"{name} must be contiguous")
-    if not t.is_cuda or (like is not None and t.device != like.device):
-        raise LstkError(E_INVALID, f"{name} is on {t.device}" + ("" if like is None else f", not on {like.device}"))
-    return t.data_ptr()
+def _tensor(t, name, dtype, shape, dev=None):
+    """Pointer of a contiguous tensor of this dtype and shape (None: any size) on device `dev` (None: any GPU)."""
+    try:
+        s = t.shape
+        if t.dtype is dtype and (s == shape or (len(s) == len(shape) and all(w is None or n == w for n, w in zip(s, shape)))) and \
+                t.is_contiguous():
+            d = t.get_device()
+            if d == dev or (dev is None and d >= 0):
+                return t.data_ptr()
+    except AttributeError:
+        raise LstkError(E_INVALID, f"{name} must be a tensor, got {type(t)}") from None
+    if t.is_contiguous() and t.dtype is dtype and len(s) == len(shape) and all(w is None or n == w for n, w in zip(s, shape)):
+        raise LstkError(E_INVALID, f"{name} is on {t.device}" + ("" if dev is None else f", not on GPU {dev}"))
+    want = "x".join("n" if w is None else str(w) for w in shape)
+    raise LstkError(E_INVALID, f"{name} must be a contiguous {dtype} tensor of shape {want}, got {t.dtype} {tuple(s)}")
 
 
 def _rows(t, name, dtype):
-    """A 2-D device tensor whose rows are contiguous: (pointer, row stride)."""
-    if not hasattr(t, "data_ptr") or t.dtype != dtype or t.dim() != 2:
-        raise LstkError(E_INVALID, f"{name} must be a 2-D {dtype} tensor")
-    if not t.is_cuda:
+    """A 2-D tensor on a GPU whose rows are contiguous: (pointer, row stride, rows, row length, device)."""
+    try:
+        n, m = t.shape
+        ld, one = t.stride()
+        dev = t.get_device()
+    except (AttributeError, ValueError):
+        raise LstkError(E_INVALID, f"{name} must be a 2-D tensor") from None
+    if t.dtype is not dtype:
+        raise LstkError(E_INVALID, f"{name} must be a 2-D {dtype} tensor, got {t.dtype}")
+    if dev < 0:
         raise LstkError(E_INVALID, f"{name} is on {t.device}")
-    n, m = t.shape
-    if (m > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < m):
+    if (m > 1 and one != 1) or (n > 1 and ld < m):
         raise LstkError(E_INVALID, f"{name} must have contiguous rows that do not overlap")
-    return t.data_ptr(), t.stride(0) if n > 1 else m
+    return t.data_ptr(), ld if n > 1 else m, n, m, dev
 
 
-class _Call:
-    """The device and stream of a call on tensors: the tensors' device is current inside, and a workspace made for the call
-    stays until the stream is done with it."""
+def _on_device(dev, stream, call):
+    """call(stream handle) with device `dev` current; the handle is `stream`'s, or that of the device's current stream."""
+    import torch
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(dev)
+    else:
+        handle = stream if isinstance(stream, int) else stream.cuda_stream
+    if torch.cuda.current_device() == dev:
+        return call(handle)
+    with torch.cuda.device(dev):
+        return call(handle)
 
-    def __init__(self, like, stream):
-        import torch
-        self._torch, self._device, self._given = torch, like.device, stream
-        self._guard = None
 
-    def __enter__(self):
-        if self._torch.cuda.current_device() != self._device.index:
-            self._guard = self._torch.cuda.device(self._device)
-            self._guard.__enter__()
-        self.stream = _stream(self._given)
-        return self
-
-    def __exit__(self, *a):
-        if self._guard is not None:
-            self._guard.__exit__(*a)
-
-    def work(self, given, nbytes):
-        """(pointer, bytes) of the caller's workspace, or of a new one."""
-        if given is None:
-            given = self._torch.empty(nbytes, dtype=self._torch.uint8, device=self._device)
-            if self._given is not None:
-                s = self._given
-                given.record_stream(self._torch.cuda.ExternalStream(s, device=self._device) if isinstance(s, int) else s)
-        elif given.device != self._device or not given.is_contiguous():
-            raise LstkError(E_INVALID, f"work must be a contiguous tensor on {self._device}")
-        self._work = given
-        return given.data_ptr(), given.numel() * given.element_size()
+def _work(given, nbytes, dev, stream):
+    """(tensor, pointer, bytes) of the caller's workspace, or of a new one that lives until `stream` is done with it."""
+    import torch
+    if given is None:
+        given = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        if stream is not None:
+            given.record_stream(torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream)
+    elif not hasattr(given, "data_ptr") or given.get_device() != dev or not given.is_contiguous():
+        raise LstkError(E_INVALID, f"work must be a contiguous tensor on GPU {dev}")
+    return given, given.data_ptr(), given.numel() * given.element_size()
 
 
 class RouterRule:
@@ -360,17 +362,16 @@ def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, s
     """The experts a rule chooses from router logits [T][n_expert] (f32, rows may be strided): (ids int32, weights f32), each
     [T][n_expert_used], in descending order of choice. bias: f32 [n_expert], added to the scores for the choice only."""
     import torch
-    p, ld = _rows(logits, "logits", torch.float32)
-    T, E = logits.shape
-    b = None if bias is None else _tensor(bias, "bias", torch.float32, (E,), logits)
+    p, ld, T, E, dev = _rows(logits, "logits", torch.float32)
+    b = None if bias is None else _tensor(bias, "bias", torch.float32, (E,), dev)
     k = int(n_expert_used)
+    shape = (T, k)
     if ids is None:
-        ids = torch.empty(T, max(k, 0), dtype=torch.int32, device=logits.device)
+        ids = torch.empty(T, max(k, 0), dtype=torch.int32, device=dev)
     if weights is None:
-        weights = torch.empty(T, max(k, 0), dtype=torch.float32, device=logits.device)
-    with _Call(logits, stream) as c:
-        _check(lib().lstk_moe_select(ctypes.byref(rule.c), p, ld, b, T, E, k, _tensor(ids, "ids", torch.int32, (T, k), logits),
-                                     _tensor(weights, "weights", torch.float32, (T, k), logits), c.stream))
+        weights = torch.empty(T, max(k, 0), dtype=torch.float32, device=dev)
+    ip, wp = _tensor(ids, "ids", torch.int32, shape, dev), _tensor(weights, "weights", torch.float32, shape, dev)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_moe_select(ctypes.byref(rule.c), p, ld, b, T, E, k, ip, wp, st)))
     return ids, weights
 
 
@@ -388,23 +389,25 @@ def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0,
     first[b] on. max_len bounds the lengths (it sizes the launch). window > 0: only the last `window` cells and the first
     n_sink. cell_seq (int32 [kv_size]) with seqs (int32 [n_seq]): cells of other owners are not visible. Returns out, like q."""
     import torch
-    n, H, hd = q.shape if q.dim() == 3 else (0, 0, 0)
-    qp = _tensor(q, "q", torch.float16, (None, None, None))
-    kv, _, size, _ = k_cache.shape if k_cache.dim() == 4 else (0, 0, 0, 0)
-    cache = PagedCache(_tensor(k_cache, "k_cache", torch.float16, (None, hd // 4, None, 4), q),
-                       _tensor(v_cache, "v_cache", torch.float16, (kv, size // 4, hd, 4), q), size, kv, hd,
-                       None if cell_seq is None else _tensor(cell_seq, "cell_seq", torch.int32, (size,), q))
-    s = PagedSeqs(n, int(max_len), _tensor(lens, "lens", torch.int32, (n,), q), _tensor(first, "first", torch.int32, (n,), q),
-                  _tensor(blocks, "blocks", torch.int32, (None,), q), blocks.numel(),
-                  None if seqs is None else _tensor(seqs, "seqs", torch.int32, (n,), q))
+    i32, f16 = torch.int32, torch.float16
+    qp = _tensor(q, "q", f16, (None, None, None))
+    dev = q.get_device()
+    n, H, hd = shape = q.shape
+    kp = _tensor(k_cache, "k_cache", f16, (None, hd // 4, None, 4), dev)
+    kv, _, size, _ = k_cache.shape
+    cache = PagedCache(kp, _tensor(v_cache, "v_cache", f16, (kv, size // 4, hd, 4), dev), size, kv, hd,
+                       None if cell_seq is None else _tensor(cell_seq, "cell_seq", i32, (size,), dev))
+    table = _tensor(blocks, "blocks", i32, (None,), dev)
+    s = PagedSeqs(n, int(max_len), _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table,
+                  blocks.numel(), None if seqs is None else _tensor(seqs, "seqs", i32, (n,), dev))
     if out is None:
         out = torch.empty_like(q)
-    op = _tensor(out, "out", torch.float16, (n, H, hd), q)
-    with _Call(q, stream) as c:
-        need = lib().lstk_attn_paged_work_bytes(n, H, kv, hd, s.max_len, int(window), int(n_sink)) if work is None else 0
-        wp, wn = c.work(work, need)
-        _check(lib().lstk_attn_paged(ctypes.byref(cache), ctypes.byref(s), qp, H, int(window), int(n_sink),
-                                     float(hd ** -0.5 if scale is None else scale), op, wp, wn, c.stream))
+    op = _tensor(out, "out", f16, shape, dev)
+    need = 0 if work is not None else lib().lstk_attn_paged_work_bytes(n, H, kv, hd, s.max_len, int(window), int(n_sink))
+    wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
+    f = float(hd ** -0.5 if scale is None else scale)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_attn_paged(ctypes.byref(cache), ctypes.byref(s), qp, H, int(window),
+                                                                    int(n_sink), f, op, wp, wn, st)))
     return out
 
 
@@ -417,20 +420,21 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     in [0, 1)): lstk_sample, include/lstk_qwen3.h. temperature, top_p, min_p (f32) and top_k (int32) are [n] device tensors;
     None means temperature 1 / no cut. Returns (tokens int32 [n], probabilities f32 [n])."""
     import torch
-    p, ld = _rows(logits, "logits", torch.float32)
-    n, V = logits.shape
-    f32 = lambda t, name: None if t is None else _tensor(t, name, torch.float32, (n,), logits)
-    how = Sampling(f32(temperature, "temperature"), None if top_k is None else _tensor(top_k, "top_k", torch.int32, (n,), logits),
-                   f32(top_p, "top_p"), f32(min_p, "min_p"))
-    up = _tensor(u, "u", torch.float32, (n,), logits)
+    f32, i32 = torch.float32, torch.int32
+    p, ld, n, V, dev = _rows(logits, "logits", f32)
+    shape = (n,)
+    how = Sampling(None if temperature is None else _tensor(temperature, "temperature", f32, shape, dev),
+                   None if top_k is None else _tensor(top_k, "top_k", i32, shape, dev),
+                   None if top_p is None else _tensor(top_p, "top_p", f32, shape, dev),
+                   None if min_p is None else _tensor(min_p, "min_p", f32, shape, dev))
+    up = _tensor(u, "u", f32, shape, dev)
     if tokens is None:
-        tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+        tokens = torch.empty(n, dtype=i32, device=dev)
     if probs is None:
-        probs = torch.empty(n, dtype=torch.float32, device=logits.device)
-    tp, pp = _tensor(tokens, "tokens", torch.int32, (n,), logits), _tensor(probs, "probs", torch.float32, (n,), logits)
-    with _Call(logits, stream) as c:
-        wp, wn = c.work(work, lib().lstk_sample_work_bytes(n, V) if work is None else 0)
-        _check(lib().lstk_sample(p, ld, n, V, ctypes.byref(how), up, tp, pp, wp, wn, c.stream))
+        probs = torch.empty(n, dtype=f32, device=dev)
+    tp, pp = _tensor(tokens, "tokens", i32, shape, dev), _tensor(probs, "probs", f32, shape, dev)
+    wt, wp, wn = _work(work, lib().lstk_sample_work_bytes(n, V) if work is None else 0, dev, stream)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_sample(p, ld, n, V, ctypes.byref(how), up, tp, pp, wp, wn, st)))
     return tokens, probs
 
 
