@@ -89,33 +89,55 @@ __global__ __launch_bounds__(kPaWaves *kWave) void paged_attn_kernel(PagedAttnPa
 #pragma unroll
     for (int t = 0; t < 2 * NM; t++) o[t] = float4v{0, 0, 0, 0};
 
-    const int64_t n_blocks = P.kv_size / kPageCells;
-    const int end = min((c + 1) * P.chunk, sp.count);
-    for (int j = c * P.chunk + wv; j < end; j += kPaWaves) {
-        const int page = j < sp.ps ? j : sp.pw + (j - sp.ps);
-        const int64_t at = (int64_t) P.first[b] + page;
-        const int id = at >= 0 && at < P.n_table ? P.blocks[at] : -1;
-        if (id < 0 || id >= n_blocks) continue;
-        const int64_t cell0 = (int64_t) id * kPageCells;
-        unsigned see = visible_cells(sp, page * kPageCells);
-        if (P.cell_seq) see &= (unsigned) __ballot(P.cell_seq[cell0 + (lane & (kPageCells - 1))] == P.seq[b]);
-        if (see == 0) continue;
-        uint4 k[NK], v[NK];
-        const uint16_t *ksrc = P.kc + ((int64_t) (g * (HD / 4) + g4) * P.kv_size + cell0 + 2 * col) * 4;
+    // The wavefront's pages are the chunk's pages wv, wv + 4, ..; lane l looks up the l-th of the next 64. A page that is out of
+    // range reads page 0 and shows nothing.
+    const int begin = c * P.chunk + wv, end = min((c + 1) * P.chunk, sp.count);
+    const int n_page = end > begin ? (end - begin + kPaWaves - 1) / kPaWaves : 0;
+    const int64_t first = P.first[b];
+    auto page_of = [&](int i) {
+        const int j = begin + i * kPaWaves;
+        return j < sp.ps ? j : sp.pw + (j - sp.ps);
+    };
+    auto look_up = [&](int i) {
+        const int64_t at = first + page_of(i);
+        const int id = i < n_page && at >= 0 && at < P.n_table ? P.blocks[at] : -1;
+        return id >= 0 && id < P.kv_size / kPageCells ? id : -1;
+    };
+    const int seq = P.cell_seq ? P.seq[b] : 0;
+    const uint16_t *const k_lane = P.kc + ((int64_t) (g * (HD / 4) + g4) * P.kv_size + 2 * col) * 4;
+    const uint16_t *const v_lane = P.vc + ((int64_t) g * P.kv_size / 4 + 2 * g4) * HD * 4 + 8 * col;
+    uint4 k[NK];
+    int owner = 0;
+    auto load_k = [&](int id) {
+        const int64_t cell0 = (int64_t) max(id, 0) * kPageCells;
 #pragma unroll
-        for (int i = 0; i < NK; i++) k[i] = *reinterpret_cast<const uint4 *>(ksrc + (int64_t) i * 16 * P.kv_size);
-        const uint16_t *vsrc = P.vc + (((int64_t) g * P.kv_size + cell0) / 4 + 2 * g4) * HD * 4 + 8 * col;
+        for (int i = 0; i < NK; i++) k[i] = *reinterpret_cast<const uint4 *>(k_lane + cell0 * 4 + (int64_t) i * 16 * P.kv_size);
+        if (P.cell_seq) owner = P.cell_seq[cell0 + (lane & (kPageCells - 1))];
+    };
+    int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
+    if (n_page > 0) load_k(id);
+    for (int it = 0; it < n_page; it++) {
+        const int64_t cell0 = (int64_t) max(id, 0) * kPageCells;
+        uint4 v[NK];
 #pragma unroll
         for (int t = 0; t < NM; t++) {
-            v[2 * t] = *reinterpret_cast<const uint4 *>(vsrc + 128 * t);
-            v[2 * t + 1] = *reinterpret_cast<const uint4 *>(vsrc + HD * 4 + 128 * t);
+            v[2 * t] = *reinterpret_cast<const uint4 *>(v_lane + cell0 * HD + 128 * t);
+            v[2 * t + 1] = *reinterpret_cast<const uint4 *>(v_lane + cell0 * HD + HD * 4 + 128 * t);
         }
+        unsigned see = id >= 0 ? visible_cells(sp, page_of(it) * kPageCells) : 0u;
+        if (P.cell_seq) see &= (unsigned) __ballot(owner == seq);
         float4v se{0, 0, 0, 0}, so{0, 0, 0, 0}; // cells 8 g4 + 2 i and + 1
 #pragma unroll
         for (int m = 0; m < NM; m++) {
             se = mfma(halves(k[2 * m].x, k[2 * m].y, k[2 * m + 1].x, k[2 * m + 1].y), q[m], se);
             so = mfma(halves(k[2 * m].z, k[2 * m].w, k[2 * m + 1].z, k[2 * m + 1].w), q[m], so);
         }
+        // the next page's K is on its way while this one's scores and V are worked on
+        __builtin_amdgcn_sched_barrier(0);
+        if ((it + 1) % kWave == 0) ids = look_up(it + 1 + lane);
+        id = __builtin_amdgcn_readlane(ids, (it + 1) % kWave);
+        if (it + 1 < n_page) load_k(id);
+        __builtin_amdgcn_sched_barrier(0);
         float s[8];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -216,24 +238,58 @@ __global__ __launch_bounds__(kPaWaves *kWave) void paged_attn_kernel(PagedAttnPa
     }
 }
 
-// The chunks of one (sequence, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c. HD threads, a dim each.
+// The chunks of one (sequence, head): out = sum_c 2^(m_c - m) o_c / sum_c 2^(m_c - m) l_c. A thread takes four dims of every
+// (kBlock / (HD / 4))-th chunk; those of the same dims meet in LDS.
 template <int HD>
-__global__ __launch_bounds__(HD) void paged_attn_join_kernel(PagedAttnParams P) {
-    const int b = blockIdx.x, h = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams P) {
+    constexpr int NQ = HD / 4, NC = kBlock / NQ, kAhead = 4;
+    __shared__ __align__(16) float4 s_o[NC][NQ];
+    __shared__ float s_m[kBlock / kWave], s_l[NC];
+    const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, dq = tid % NQ, cl = tid / NQ;
     const Span sp = span_of(P, b);
     const int n = (sp.count + P.chunk - 1) / P.chunk;
     if (n <= 1) return; // written by the first launch
     const float *src = P.part + ((int64_t) b * P.n_head + h) * P.n_chunk * (HD + 4);
     float m = kLowest;
-    for (int c = 0; c < n; c++) m = fmaxf(m, src[(int64_t) c * (HD + 4)]);
-    float l = 0.0f, a = 0.0f;
-    for (int c = 0; c < n; c++) {
-        const float *p = src + (int64_t) c * (HD + 4);
-        const float f = __builtin_amdgcn_exp2f(p[0] - m);
-        l = fmaf(p[1], f, l);
-        a = fmaf(p[4 + d], f, a);
+    for (int c = tid; c < n; c += kBlock) m = fmaxf(m, src[(int64_t) c * (HD + 4)]);
+    m = wave_max(m);
+    if (tid % kWave == 0) s_m[tid / kWave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float l = 0.0f;
+    float4 a = make_float4(0, 0, 0, 0);
+    for (int c0 = cl; c0 < n; c0 += kAhead * NC) {
+        float2 ml[kAhead];
+        float4 o[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const float *p = src + (int64_t) min(c0 + i * NC, n - 1) * (HD + 4);
+            ml[i] = *reinterpret_cast<const float2 *>(p);
+            o[i] = *reinterpret_cast<const float4 *>(p + 4 + 4 * dq);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (c0 + i * NC >= n) break;
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - m);
+            l = fmaf(ml[i].y, f, l);
+            a.x = fmaf(o[i].x, f, a.x);
+            a.y = fmaf(o[i].y, f, a.y);
+            a.z = fmaf(o[i].z, f, a.z);
+            a.w = fmaf(o[i].w, f, a.w);
+        }
     }
-    P.out[((int64_t) b * P.n_head + h) * HD + d] = __half_as_ushort(__float2half_rn(l == 0.0f ? 0.0f : a / l));
+    s_o[cl][dq] = a;
+    if (dq == 0) s_l[cl] = l;
+    __syncthreads();
+    if (tid >= HD) return;
+    float sum = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+        sum += reinterpret_cast<const float *>(s_o[i])[tid];
+        l += s_l[i];
+    }
+    P.out[((int64_t) b * P.n_head + h) * HD + tid] = __half_as_ushort(__float2half_rn(l == 0.0f ? 0.0f : sum / l));
 }
 
 template <int HD>
@@ -273,9 +329,9 @@ hipError_t launch_paged_attn_join(const PagedAttnParams &P, hipStream_t st, cons
     if (P.n_chunk == 1) return hipSuccess;
     const dim3 grid(P.n_seq, P.n_head);
     switch (P.hd) {
-    case 64: return launch(paged_attn_join_kernel<64>, grid, dim3(64), 0, st, tm, P);
-    case 128: return launch(paged_attn_join_kernel<128>, grid, dim3(128), 0, st, tm, P);
-    case 256: return launch(paged_attn_join_kernel<256>, grid, dim3(256), 0, st, tm, P);
+    case 64: return launch(paged_attn_join_kernel<64>, grid, dim3(kBlock), 0, st, tm, P);
+    case 128: return launch(paged_attn_join_kernel<128>, grid, dim3(kBlock), 0, st, tm, P);
+    case 256: return launch(paged_attn_join_kernel<256>, grid, dim3(kBlock), 0, st, tm, P);
     default: return hipErrorInvalidValue;
     }
 }
