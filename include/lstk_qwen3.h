@@ -129,7 +129,7 @@ int lstk_model_forward_batch(lstk_model *model, int n_seq, int32_t max_len, int 
  * step runs it on its own cache):
  *   out[b][h] = sum_i softmax_i(scale q[b][h] . k[i][h / (n_head / n_head_kv)]) v[i][..]   over the visible cells i of row b
  * K is [n_head_kv][head_dim / 4][kv_size][4] fp16 (4 dims of a cell together, cells side by side), V
- * [n_head_kv][kv_size / 4][head_dim][4] (4 cells of a dim together); head_dim 64, 128 or 256, kv_size a multiple of 32.
+ * [n_head_kv][kv_size / 4][head_dim][4] (4 cells of a dim together); head_dim 64, 128 or 256, kv_size a multiple of 32, at most 2^27.
  * Pages are runs of 32 cells: logical cell i of row b is cell d_blocks[d_first[b] + i / 32] * 32 + i % 32, 0 <= i < d_len[b];
  * rows may share pages. Visible are the cells i < min(d_len[b], max_len), of them with window > 0 only the last `window` and
  * the first n_sink (counted in cells the row holds). A page whose table index (outside [0, n_table)) or block number (outside the cache) is out of range is

@@ -20,9 +20,10 @@ int hip_fail(hipError_t e, const char *what) { return set_error(LSTK_E_DEVICE, s
 int bad(const std::string &msg) { return set_error(LSTK_E_INVALID, msg); }
 bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// A launch has fewer than 2^32 threads along x, in work-groups of up to 1024, and up to 65535 work-groups along y.
+// A launch has fewer than 2^32 threads along x, in work-groups of up to 1024.
 constexpr int64_t kMostGrid = (int64_t(1) << 22) - 1;
-constexpr int kMostGridY = 65535;
+constexpr int kMostHeads = 65535;
+constexpr int64_t kMostCells = int64_t(1) << 27; // of a cache: the kernel's 32-bit offsets
 constexpr int kMostTokens = 1 << 24;
 
 // Shapes of a paged attention call, checked, and its plan.
@@ -40,7 +41,7 @@ int paged_plan(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, 
     P.window = window > 0 ? window : 0;
     P.n_sink = n_sink;
     bytes = lstk::paged_attn_plan(P);
-    if ((int64_t) n_seq * P.n_chunk > kMostGrid || (int64_t) n_head_kv * P.n_rowblk > kMostGridY || n_head > kMostGridY)
+    if (n_head > kMostHeads || (int64_t) n_seq * n_head_kv * P.n_rowblk > kMostGrid)
         return bad("too many sequences or heads for one launch");
     return LSTK_OK;
 }
@@ -62,8 +63,8 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
     size_t bytes = 0;
     const int rc = paged_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
     if (rc != LSTK_OK) return rc;
-    if (cache->kv_size < lstk::kPageCells || cache->kv_size % lstk::kPageCells || cache->kv_size > INT32_MAX)
-        return bad("kv_size must be a positive multiple of 32 below 2^31");
+    if (cache->kv_size < lstk::kPageCells || cache->kv_size % lstk::kPageCells || cache->kv_size > kMostCells)
+        return bad("kv_size must be a positive multiple of 32, at most 2^27");
     if (seqs->n_table < 0) return bad("n_table must be >= 0");
     if (!std::isfinite(scale)) return bad("scale must be finite");
     if (P.n_seq == 0) return LSTK_OK;
@@ -88,7 +89,7 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
     P.cell_seq = cache->d_cell_seq;
     P.seq = seqs->d_seq;
     P.scale = scale * 1.44269504088896341f;
-    P.part = static_cast<float *>(d_work);
+    lstk::paged_attn_work(P, d_work);
     P.out = d_out;
     hipStream_t st = static_cast<hipStream_t>(stream);
     hipError_t e = lstk::launch_paged_attn(P, st, nullptr);

@@ -16,6 +16,9 @@ constexpr int kPageCells = 32; // cells of a page: the cache's block (KvCache::b
 // Attention of one query token per sequence over one layer's cache in the cell layouts of forward.h. Logical cell i of
 // sequence b is cell blocks[first[b] + i / 32] * 32 + i % 32; cells [0, len[b]) exist, and of those the last `window` and
 // the first `n_sink` are visible (window <= 0: all). A page whose table entry or block number is out of range is not.
+struct PagedAttnSplit { // the work-group that began a task, and how many others went on with it
+    int wg, more;
+};
 struct PagedAttnParams {
     const uint16_t *q; // [n_seq][n_head][hd] fp16
     const uint16_t *kc, *vc;
@@ -24,13 +27,15 @@ struct PagedAttnParams {
     int64_t kv_size;
     int n_seq, n_head, n_kv, hd, n_table, max_len, window, n_sink;
     float scale; // of the scores, times log2(e)
-    int chunk, n_chunk, n_rowblk; // pages per work-group, chunks of the longest sequence, 16-row blocks (paged_attn_plan)
-    float *part;                  // [n_seq][n_head][n_chunk][hd + 4]: max, sum, 2 unused, unnormalised output
-    uint16_t *out;                // [n_seq][n_head][hd] fp16
+    int n_rowblk, n_wg;    // blocks of 16 query heads per KV head; work-groups of equal shares, 0: one per task (paged_attn_plan)
+    PagedAttnSplit *split; // [n_seq][n_kv * n_rowblk], a task each
+    float *part;           // [n_wg][2][min(16, heads per KV head)][hd + 4]: max, sum, 2 unused, unnormalised output of a part of a task
+    uint16_t *out;         // [n_seq][n_head][hd] fp16
 };
-// Fills chunk, n_chunk and n_rowblk; returns the bytes of `part` that calls of these shapes with this max_len or a smaller
-// one take (0 where every sequence takes one chunk).
+// Fills n_rowblk and n_wg; returns the bytes of workspace (16-byte aligned) that calls of these shapes with this max_len or a
+// smaller one take (0 where every task has a work-group), which paged_attn_work points at.
 size_t paged_attn_plan(PagedAttnParams &P);
+void paged_attn_work(PagedAttnParams &P, void *work);
 hipError_t launch_paged_attn(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm);
 hipError_t launch_paged_attn_join(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm);
 

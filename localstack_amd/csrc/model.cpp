@@ -656,7 +656,7 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
             pp.seq = M->in + 3 * nb;
             pp.kv_size = M->kv.size;
             pp.scale = ap.scale * 1.44269504088896341f;
-            pp.part = M->part;
+            lstk::paged_attn_work(pp, M->part);
             pp.out = M->attn16;
         } else {
             lstk::attn_plan(ap); // clears rope_in when the context is too long for one pass per chunk
@@ -665,7 +665,7 @@ int forward(lstk_model *M, int32_t seq, int T, int n_cells, float *d_logits, int
             return hip_fail(e, "rope launch");
         if (batch) {
             if ((e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_paged_attn(pp, st, tm); })) != hipSuccess ||
-                (pp.n_chunk > 1 &&
+                (pp.n_wg > 1 &&
                  (e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_paged_attn_join(pp, st, tm); })) != hipSuccess))
                 return hip_fail(e, "attention launch");
         } else if ((e = timed(M, 2, [&](const lstk::LaunchTiming *tm) { return lstk::launch_attn(ap, st, tm); })) != hipSuccess ||
