@@ -24,8 +24,9 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int kPaWaves = 4;
 constexpr int kPaCus = 256; // of MI355X
-constexpr int kPaShort = 16; // pages up to which every task has a work-group of its own
-constexpr int kPaLeast = 4;  // pages of a share
+constexpr int kPaPerCu = 2; // work-groups of equal shares per CU
+constexpr int kPaLeast = 4; // pages of a share
+constexpr int kPaRound = 4;  // rounds of the wavefronts up to which a share is made a whole number of them
 constexpr float kLowest = -3.0e38f; // a running maximum that any score replaces
 
 // The pages of a sequence that hold visible cells: [0, ps) and [pw, pw + count - ps).
@@ -35,9 +36,9 @@ struct Span {
 };
 // Pages that a sequence has in the list: one at least, so that one without any is written (zeros) like the others.
 __device__ __forceinline__ int listed(const Span &s) { return max(1, s.count); }
-__device__ __forceinline__ Span span_of(const PagedAttnParams &P, int b) {
+__device__ __forceinline__ Span span_of(const PagedAttnParams &P, int len) {
     Span s;
-    s.n = max(0, min(P.len[b], P.max_len));
+    s.n = max(0, min(len, P.max_len));
     s.lo = P.window > 0 && s.n > P.window ? s.n - P.window : 0;
     s.sink = min(P.n_sink, s.lo);
     s.pw = s.lo / kPageCells;
@@ -52,6 +53,13 @@ __device__ __forceinline__ unsigned visible_cells(const Span &s, int i0) {
     return bits_below(s.n - i0) & (~bits_below(s.lo - i0) | bits_below(s.sink - i0));
 }
 
+// K and V are read once a call, with the non-temporal hint: 128 sequences (1.2 GB) 225 us without it, 205 with it on one of the
+// two, 200 on both; two of 100000 cells 89, 82 and 79.
+__device__ __forceinline__ uint4 read_once(const char *p) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
 __device__ __forceinline__ half8v halves(unsigned a, unsigned b, unsigned c, unsigned d) {
     return __builtin_bit_cast(half8v, make_uint4(a, b, c, d));
 }
@@ -73,36 +81,50 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
     return (int64_t) ((uint64_t) hi << 32 | lo);
 }
 
-// The share of work-group w in the list: from page j of task `task` of sequence b, `left` pages.
+// The share of a work-group in the list: `left` pages from page j of task `task` of sequence b on. The sequences' lengths and
+// first table entries stay in LDS where they fit, so that the way to the first page is one wait for them and not three.
+constexpr int kPaKept = kPaWaves * kWave;
 struct Share {
-    int b, task, j, w_of; // w_of: work-groups that have a share
-    int64_t left, total;  // total: pages of the list
+    int b, task, j;
+    int64_t left, each, total; // each: pages of a full share; total: of the list
 };
-__device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks) {
+struct Kept {
+    int len[kPaKept], first[kPaKept];
+};
+__device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, Kept &K) {
     __shared__ int64_t s_sum[kPaWaves], s_before;
     __shared__ int s_b;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
     int64_t sum = 0;
-    for (int b = tid; b < P.n_seq; b += kPaWaves * kWave) sum += listed(span_of(P, b));
+    int mine = 0; // pages of sequence tid, and of the last one of every kPaKept
+    for (int b = tid; b < P.n_seq; b += kPaKept) {
+        const int len = P.len[b];
+        if (P.n_seq <= kPaKept) {
+            K.len[tid] = len;
+            K.first[tid] = P.first[b];
+        }
+        mine = listed(span_of(P, len));
+        sum += mine;
+    }
     for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
     if (lane == 0) s_sum[wv] = sum;
     __syncthreads();
     Share s;
     s.total = 0;
     for (int w = 0; w < kPaWaves; w++) s.total += s_sum[w];
-    s.total *= tasks;
-    s.w_of = __builtin_amdgcn_readfirstlane((int) min((int64_t) gridDim.x, s.total));
-    const int w = blockIdx.x;
-    if (w >= s.w_of) {
-        s.left = 0;
-        return s;
-    }
-    const int64_t lo = s.total * w / s.w_of, hi = s.total * (w + 1) / s.w_of;
+    s.total = uniform(s.total * tasks);
+    // small shares are whole rounds of the wavefronts
+    s.each = (s.total + gridDim.x - 1) / gridDim.x;
+    if (s.each <= kPaRound * kPaWaves) s.each = (s.each + kPaWaves - 1) / kPaWaves * kPaWaves;
+    const int64_t lo = s.each * blockIdx.x;
+    s.each = uniform(s.each);
+    s.left = uniform(min(s.each, s.total - lo));
+    if (s.left <= 0) return s;
     // the sequence that page `lo` of the list is of
     int64_t before = 0; // of the sequences so far
-    for (int b0 = 0; b0 < P.n_seq; b0 += kPaWaves * kWave) {
+    for (int b0 = 0; b0 < P.n_seq; b0 += kPaKept) {
         const int b = b0 + tid;
-        const int64_t mine = b < P.n_seq ? listed(span_of(P, b)) : 0;
+        if (P.n_seq > kPaKept) mine = b < P.n_seq ? listed(span_of(P, P.len[b])) : 0;
         int64_t upto = mine;
         for (int d = 1; d < kWave; d *= 2) {
             const int64_t o = __shfl_up(upto, d, kWave);
@@ -123,11 +145,9 @@ __device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks) {
     __syncthreads();
     s.b = __builtin_amdgcn_readfirstlane(s_b);
     const int64_t into = lo - s_before * tasks;
-    const int count = listed(span_of(P, s.b));
+    const int count = listed(span_of(P, P.n_seq <= kPaKept ? K.len[s.b] : P.len[s.b]));
     s.task = __builtin_amdgcn_readfirstlane((int) (into / count));
-    s.j = __builtin_amdgcn_readfirstlane((int) (into % count));
-    s.left = uniform(hi - lo);
-    s.total = uniform(s.total);
+    s.j = __builtin_amdgcn_readfirstlane((int) (into - (int64_t) s.task * count));
     return s;
 }
 
@@ -139,10 +159,11 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
     __shared__ __align__(16) float s_o[kPaWaves][16][HD + 4];
     __shared__ uint4 s_q[NM][kWave];
     const int tasks = P.n_kv * P.n_rowblk;
+    __shared__ Kept K;
     Share share;
     if constexpr (SPLIT) {
-        share = share_of(P, tasks);
-        if (share.left == 0) return;
+        share = share_of(P, tasks, K);
+        if (share.left <= 0) return;
     } else {
         share.b = blockIdx.x / tasks;
         share.task = blockIdx.x % tasks;
@@ -153,7 +174,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
     const int grp = P.n_head / P.n_kv, rows = min(grp, 16);
     for (;;) {
         const int b = share.b, g = share.task % P.n_kv, rb = share.task / P.n_kv, row = rb * 16 + col;
-        const Span sp = span_of(P, b);
+        const bool kept = SPLIT && P.n_seq <= kPaKept;
+        const Span sp = span_of(P, kept ? __builtin_amdgcn_readfirstlane(K.len[b]) : P.len[b]);
         const int count = listed(sp), j0 = share.j, j1 = SPLIT ? (int) min((int64_t) count, j0 + share.left) : count;
 
         // the operand Q^T: head `col`, dims 16 i + 4 g4 .. + 3 of steps i = 2 m, 2 m + 1. Kept in LDS: in registers its 16 (head
@@ -173,7 +195,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         // range reads page 0 and shows nothing.
         const int begin = j0 + wv, end = min(j1, sp.count);
         const int n_page = end > begin ? (end - begin + kPaWaves - 1) / kPaWaves : 0;
-        const int64_t first = P.first[b];
+        const int64_t first = kept ? __builtin_amdgcn_readfirstlane(K.first[b]) : P.first[b];
         auto page_of = [&](int i) {
             const int j = begin + i * kPaWaves;
             return j < sp.ps ? j : sp.pw + (j - sp.ps);
@@ -193,7 +215,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         auto load_k = [&](int id) {
             const int64_t cell0 = (int64_t) max(id, 0) * kPageCells;
 #pragma unroll
-            for (int i = 0; i < NK; i++) k[i] = *reinterpret_cast<const uint4 *>(k_head + (cell0 + (int64_t) i * 4 * P.kv_size) * 8 + k_lane);
+            for (int i = 0; i < NK; i++) k[i] = read_once(k_head + (cell0 + (int64_t) i * 4 * P.kv_size) * 8 + k_lane);
             if (P.cell_seq) owner = P.cell_seq[cell0 + (lane & (kPageCells - 1))];
         };
         int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
@@ -204,8 +226,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
             uint4 v[NK];
 #pragma unroll
             for (int t = 0; t < NM; t++) {
-                v[2 * t] = *reinterpret_cast<const uint4 *>(v_head + cell0 * (HD * 2) + 256 * t + v_lane);
-                v[2 * t + 1] = *reinterpret_cast<const uint4 *>(v_head + cell0 * (HD * 2) + HD * 8 + 256 * t + v_lane);
+                v[2 * t] = read_once(v_head + cell0 * (HD * 2) + 256 * t + v_lane);
+                v[2 * t + 1] = read_once(v_head + cell0 * (HD * 2) + HD * 8 + 256 * t + v_lane);
             }
             unsigned see = id >= 0 ? visible_cells(sp, page_of(it) * kPageCells) : 0u;
             if (P.cell_seq) see &= (unsigned) __ballot(owner == seq);
@@ -327,9 +349,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         // where this part begins a task: how many other work-groups have the rest (the last is the one whose share holds the
         // task's last page)
         if (tid == 0 && j0 == 0) {
-            const int64_t upto = share.total * (blockIdx.x + 1) / share.w_of + (count - j1);
-            const int more = whole ? 0 : (int) ((upto * share.w_of + share.total - 1) / share.total) - 1 - (int) blockIdx.x;
-            P.split[(int64_t) b * tasks + share.task] = {(int) blockIdx.x, more};
+            const int64_t last = min(share.each * (blockIdx.x + 1), share.total) - share.left + count - 1;
+            P.split[(int64_t) b * tasks + share.task] = {(int) blockIdx.x, whole ? 0 : (int) (last / share.each) - (int) blockIdx.x};
         }
         share.left -= j1 - j0;
         if (share.left == 0) return;
@@ -454,9 +475,12 @@ size_t paged_attn_plan(PagedAttnParams &P) {
     if (P.window > 0) pages = std::min<int64_t>(all, (int64_t) P.window / kPageCells + 2 + ((int64_t) P.n_sink + kPageCells - 1) / kPageCells);
     const int64_t tasks = (int64_t) P.n_seq * P.n_kv * P.n_rowblk;
     P.n_wg = 0;
-    if (pages <= kPaShort || tasks == 0) return 0;
-    // equal shares: as many work-groups as the device holds at once, of kPaLeast pages or more
-    P.n_wg = (int) std::max<int64_t>(1, std::min<int64_t>(kPaCus * (P.hd == 64 ? 4 : P.hd == 128 ? 3 : 2), tasks * pages / kPaLeast));
+    // A work-group per task, in one launch, for sequences of up to 16 pages, and of up to 64 where there is a task for every CU:
+    // the equal shares cost some 10 us more (their way to the first page and the second launch). Us a call at 32 heads on 4:
+    // 64 sequences of 100 to 500 cells 12 and 22, 64 of 100 to 1000 18 and 26, one of 1000 15 and 14.
+    if (pages <= 16 || (pages <= 64 && tasks >= kPaCus) || tasks == 0) return 0;
+    // equal shares, of kPaLeast pages or more, for two work-groups a CU: all of them are there at once
+    P.n_wg = (int) std::max<int64_t>(1, std::min<int64_t>(kPaCus * kPaPerCu, tasks * pages / kPaLeast));
     return split_entries(P) * sizeof(PagedAttnSplit) + (size_t) P.n_wg * 2 * std::min(grp, 16) * (P.hd + 4) * sizeof(float);
 }
 
