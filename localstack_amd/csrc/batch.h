@@ -57,7 +57,7 @@ struct SampleParams {
     uint32_t *count;          // [n_rows][kSampleBins]
     uint32_t *n_list;         // [n_rows] entries of list
     uint32_t *n_done;         // [n_rows] work-groups of the last launch that are through
-    int *list;                // [n_rows][n_vocab] indices of the values in the bins where a cut may fall
+    unsigned long long *list; // [n_rows][n_vocab] (logit, index) of the values in the bins where a cut may fall
 };
 // Fills slices and slice, and the workspace pointers from `work`; returns the workspace's bytes.
 size_t sample_plan(SampleParams &P, void *work);

@@ -20,7 +20,8 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kSmThreads = 1024;
+constexpr int kSmThreads = 512;
+constexpr int kSmTarget = 512; // work-groups of a launch
 constexpr double kUnit = 0x1p44;
 // (x_max - x) / T that the bins cover; the last one starts at 31.2347, where the weight is 0.479 * 2^-44, so all that it
 // holds rounds to zero
@@ -400,13 +401,13 @@ __device__ __forceinline__ Cuts cuts_of(const Settings &how, const Sums &S, Sums
 // The search among the gathered values. Up to kSmKeep of them are sorted by place (larger first) once, with the running sum of
 // their weights; more are left in the list, and told apart there by digits.
 constexpr int kSmKeep = 1024;
-constexpr int kSmGather = 2 * kSmKeep; // indices that a work-group gathers before they go to the list together
+constexpr int kSmGather = kSmKeep; // places that a work-group gathers before they go to the list together
 struct Search {
     union {
         struct {
             u64 place[kSmKeep], before[kSmKeep]; // sorted, and the sum of the weights before each
         };
-        int gathered[kSmGather];
+        u64 gathered[kSmGather];
         struct {
             u64 digit_mass[256];
             uint32_t digit_count[256];
@@ -416,75 +417,80 @@ struct Search {
     };
     u64 wave_mass[kSmThreads / kWave];
     u64 found, mass0; // answer
-    u64 base;         // sum of the weights before the bin's first value
-    int first;        // and its index
+    int first;        // the bin's first value
 };
 struct Reached {
     u64 place; // of the value at which the running sum reaches the target
     u64 mass0; // running sum before it
 };
 
-// Sorts the places of `n` values (index_at(i), i < n <= kSmKeep) and sums their weights.
+// Sorts the places of `n` values (place(i), i < n <= kSmKeep) and sums their weights.
 template <typename F>
-__device__ __forceinline__ void sort_gathered(const Row &r, const float *x, Search &D, int n, F index_at) {
+__device__ __forceinline__ void sort_gathered(const Row &r, Search &D, int n, F place) {
+    constexpr int E = kSmKeep / kSmThreads; // entries of a thread
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
-    u64 mine = 0;
-    if (tid < n) {
-        const int at = index_at(tid);
-        mine = place_of(value_of(x[at]), (uint32_t) at);
-    }
-    __syncthreads(); // index_at may read what is written now
-    D.place[tid] = mine;
+    u64 mine[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) mine[e] = tid + e * kSmThreads < n ? place(tid + e * kSmThreads) : 0;
+    __syncthreads(); // place() may read what is written now
+#pragma unroll
+    for (int e = 0; e < E; e++) D.place[tid + e * kSmThreads] = mine[e];
     __syncthreads();
     int size = 1;
     while (size < n) size *= 2;
     for (int run = 2; run <= size; run *= 2) {
         for (int step = run / 2; step > 0; step /= 2) {
-            const int other = tid ^ step;
-            u64 a = 0;
-            if (tid < size) {
-                a = D.place[tid];
-                const u64 o = D.place[other];
-                const bool larger = ((tid & run) == 0) == (tid < other); // the larger of the two comes here
-                a = (o > a) == larger ? o : a;
+            for (int p = tid; p < size / 2; p += kSmThreads) {
+                const int i = 2 * p - (p & (step - 1)), j = i + step; // the pair's first and second place
+                const u64 a = D.place[i], o = D.place[j];
+                if ((a < o) == ((i & run) == 0)) {
+                    D.place[i] = o;
+                    D.place[j] = a;
+                }
             }
-            __syncthreads();
-            if (tid < size) D.place[tid] = a;
             __syncthreads();
         }
     }
-    mine = D.place[tid];
-    const u64 m = tid < n ? mass_of(r, of_key((uint32_t) (mine >> 32))) : 0;
-    u64 sum = m;
+    u64 m[E], sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int i = tid * E + e;
+        m[e] = i < n ? mass_of(r, of_key((uint32_t) (D.place[i] >> 32))) : 0;
+        sum += m[e];
+    }
+    u64 upto = sum;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-        const u64 o = __shfl_up(sum, d, kWave);
-        if (lane >= d) sum += o;
+        const u64 o = __shfl_up(upto, d, kWave);
+        if (lane >= d) upto += o;
     }
-    if (lane == kWave - 1) D.wave_mass[wv] = sum;
+    if (lane == kWave - 1) D.wave_mass[wv] = upto;
     __syncthreads();
-    sum -= m;
-    for (int w = 0; w < wv; w++) sum += D.wave_mass[w];
-    D.before[tid] = sum;
+    upto -= sum;
+    for (int w = 0; w < wv; w++) upto += D.wave_mass[w];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        D.before[tid * E + e] = upto;
+        upto += m[e];
+    }
     __syncthreads();
 }
 
 // The value of bin `f` at which the running sum of weights (BY_MASS) or of values reaches `target`, which lies in that bin.
 template <bool BY_MASS>
 __device__ __forceinline__ Reached reach_sorted(const Row &r, Search &D, const Found &f, int n, u64 target) {
-    const int tid = threadIdx.x;
-    const u64 place = tid < n ? D.place[tid] : 0;
-    const float x = of_key((uint32_t) (place >> 32));
-    const bool here = tid < n && bin_of(r, x) == f.bin;
-    if (here && (tid == 0 || bin_of(r, of_key((uint32_t) (D.place[tid - 1] >> 32))) != f.bin)) {
-        D.first = tid;
-        D.base = D.before[tid];
+    for (int i = threadIdx.x; i < n; i += kSmThreads) {
+        auto bin_at = [&](int at) { return bin_of(r, of_key((uint32_t) (D.place[at] >> 32))); };
+        if (bin_at(i) == f.bin && (i == 0 || bin_at(i - 1) != f.bin)) D.first = i;
     }
     __syncthreads();
-    if (here) {
-        const u64 mass0 = f.mass0 + D.before[tid] - D.base;
-        const u64 before = BY_MASS ? mass0 : f.count0 + (uint32_t) (tid - D.first);
-        if (before < target && target <= before + (BY_MASS ? mass_of(r, x) : 1)) {
+    const int first = D.first;
+    for (int i = threadIdx.x; i < n; i += kSmThreads) {
+        const u64 place = D.place[i];
+        const float x = of_key((uint32_t) (place >> 32));
+        const u64 mass0 = f.mass0 + D.before[i] - D.before[first];
+        const u64 before = BY_MASS ? mass0 : f.count0 + (uint32_t) (i - first);
+        if (i >= first && bin_of(r, x) == f.bin && before < target && target <= before + (BY_MASS ? mass_of(r, x) : 1)) {
             D.found = place;
             D.mass0 = mass0;
         }
@@ -499,14 +505,14 @@ __device__ __forceinline__ Reached reach_sorted(const Row &r, Search &D, const F
 // from the first bit in which they differ, by a histogram of those bits over the values still in question and the running sum
 // over it from the top.
 template <bool BY_MASS>
-__device__ __forceinline__ Reached reach_in_list(const Row &r, const float *x, const int *list, Search &D, const Found &f, uint32_t n,
+__device__ __forceinline__ Reached reach_in_list(const Row &r, const u64 *list, Search &D, const Found &f, uint32_t n,
                                                  u64 target) {
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     auto each = [&](auto &&take) {
         for (uint32_t i = tid; i < n; i += kSmThreads) {
-            const int at = ld_dev(list + i);
-            const float v = value_of(x[at]);
-            if (bin_of(r, v) == f.bin) take(place_of(v, (uint32_t) at), v);
+            const u64 p = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float v = of_key((uint32_t) (p >> 32));
+            if (bin_of(r, v) == f.bin) take(p, v);
         }
     };
     __syncthreads();
@@ -659,17 +665,19 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     const Sums S = sums_of(P.mass + (int64_t) b * kSampleBins, P.count + (int64_t) b * kSampleBins, L);
     const Row r = row_of(how, best);
     const Cuts c = cuts_of(how, S, L);
-    int *list = P.list + (int64_t) b * P.n_vocab;
+    u64 *list = P.list + (int64_t) b * P.n_vocab;
+    auto write_through = [&](uint32_t at, u64 p) { __hip_atomic_store(list + at, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     const Span drawn = span_of(r, c.d_lo, c.d_hi);
     const Span ranked = c.part ? span_of(r, c.cut.bin, c.cut.bin) : drawn, run = c.by_p ? span_of(r, c.p_lo, c.p_hi) : drawn;
     each_value(q, ahead, [&](float x, int i) {
         if (!(drawn.holds(x) || ranked.holds(x) || run.holds(x))) return;
-        const double below = bins_below(r, fminf(x, FLT_MAX));
+        x = fminf(x, FLT_MAX);
+        const double below = bins_below(r, x);
         const int bin = (int) below;
         if (!c.holds(bin) || mass_of(r, below, bin, edge_weight(bin)) == 0) return;
         const uint32_t at = atomicAdd(&s_n, 1u);
-        if (at < (uint32_t) kSmGather) D.gathered[at] = i;
-        else st_dev(list + atomicAdd(&P.n_list[b], 1u), i);
+        if (at < (uint32_t) kSmGather) D.gathered[at] = place_of(x, (uint32_t) i);
+        else write_through(atomicAdd(&P.n_list[b], 1u), place_of(x, (uint32_t) i));
     });
     // one place in the list for all that fitted (a global counter's answer takes a microsecond: one each, and a wavefront that
     // meets 20 such values takes 20)
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     const uint32_t mine = min(s_n, (uint32_t) kSmGather);
     if (tid == 0 && mine > 0) s_base = atomicAdd(&P.n_list[b], mine);
     __syncthreads();
-    for (uint32_t i = tid; i < mine; i += kSmThreads) st_dev(list + s_base + i, D.gathered[i]);
+    for (uint32_t i = tid; i < mine; i += kSmThreads) write_through(s_base + i, D.gathered[i]);
     // Hand-over without an L2 write-back: the entries are device-coherent stores, complete before the work-group counts itself
     // done, and read with device-coherent loads by the one that counts last.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -687,19 +695,19 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     const uint32_t n = s_n;
     if (n == UINT_MAX) return;
     if (n <= (uint32_t) kSmKeep) {
-        sort_gathered(r, q.x, D, (int) n, [&](int i) { return ld_dev(list + i); });
+        sort_gathered(r, D, (int) n, [&](int i) { return __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); });
         draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_sorted<by_mass>(r, D, f, (int) n, target); });
     } else {
-        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_in_list<by_mass>(r, q.x, list, D, f, n, target); });
+        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_in_list<by_mass>(r, list, D, f, n, target); });
     }
 }
 
 }  // namespace
 
 size_t sample_plan(SampleParams &P, void *work) {
-    // slices of at least 1024 quads, as many as bring the launches to 512 work-groups; a row out of line has a quad more
+    // slices of at least 1024 quads, as many as bring the launches to kSmTarget work-groups; a row out of line has a quad more
     const int quads = (P.n_vocab + 6) / 4;
-    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, 256 / std::max(1, P.n_rows)));
+    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, kSmTarget / std::max(1, P.n_rows)));
     P.slice = (quads + P.slices - 1) / P.slices;
     size_t off = 0;
     auto take = [&](auto *&p, size_t n) {
