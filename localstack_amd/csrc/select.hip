@@ -4,14 +4,19 @@
 //   a group's value is the sum of its `group_top` largest c; the best n_group_used groups stay; of their experts the k largest
 //   c are chosen (equal values: the lowest id), in that order;  w = s / max(sum of the chosen s, 2^-14) * scale
 //
-// Scores and choice values are held in 64 bits: two experts a 32-bit rounding apart would swap places with the compiler's
-// choice of instructions. The chosen weights are rounded once, to fp32.
+// Scores and choice values are those of 64 bits: two experts a 32-bit rounding apart would swap places with the compiler's
+// choice of instructions. But few are that close. So a wavefront first scores its tokens in 32 bits and takes the k largest and
+// a few more (choose_fast). Only these candidates' scores are computed in 64 bits, which gives their order and weights. The
+// 32-bit scores settle the rest where the last group that stays is further from the next, and the k-th candidate from all that
+// are none, than they can be off; a wavefront with a token where they are not does all of it in 64 bits (choose_exact). The
+// chosen weights are rounded once, to fp32.
 //
 // 16 lanes (a DPP row) take a token, so a wavefront takes four, and lane l the experts l, l + 16, ..: a row's maximum is four
-// DPP steps. A choice value carries its expert in its lowest 8 mantissa bits (2^-44 of it), so that the maximum says whose it
-// is and of equal values the lowest id is the largest. In each of the k rounds the lane that owned the maximum takes it out of
-// its values in LDS and finds its next one; the others keep theirs.
+// DPP steps. A choice value carries its expert in its lowest 8 bits, so that the maximum says whose it is and of equal values
+// the lowest id is the largest. In each of the k rounds the lane that owned the maximum takes it out of its values in LDS and
+// finds its next one; the others keep theirs.
 #include <cfloat>
+#include <type_traits>
 
 #include "batch.h"
 #include "device.h"
@@ -67,6 +72,25 @@ __device__ __forceinline__ double row_sum(double v) {
     return v + dpp_d<0x140>(v);
 }
 
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+    v = max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0xB1, 0xF, 0xF, false));
+    v = max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x4E, 0xF, 0xF, false));
+    v = max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x141, 0xF, 0xF, false));
+    return max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x140, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    return fmaxf(v, dpp_f<0x140>(v));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += dpp_f<0xB1>(v);
+    v += dpp_f<0x4E>(v);
+    v += dpp_f<0x141>(v);
+    return v + dpp_f<0x140>(v);
+}
+
 // A choice value with its expert: larger is earlier. -inf becomes a finite value below all others, so that it stays above what
 // may not be chosen at all (-inf here).
 __device__ __forceinline__ double tagged(double c, int e) {
@@ -79,48 +103,164 @@ __device__ __forceinline__ int expert_of(double t) {
     return (int) (u >> 63 ? u & 255u : 255u - (u & 255u));
 }
 
-// LDS of one wavefront: the choice values of each token, lane by lane (two more a lane against bank conflicts), the chosen
-// ids, and with groups their values and which of them stay.
-template <int V>
-__host__ __device__ constexpr size_t select_lds(int k, int groups) {
-    return kSelTokens * ((size_t) kSelLanes * (V + 2) * 8 + (size_t) groups * 8 + (groups ? 32 : 0) + (size_t) k * 4);
+// The same in 32 bits, as a whole number: the order-preserving key of c with the expert in place of its lowest 8 bits; 0 is
+// below all of them. value_below is at most 2^-14 |c| below c, and never above it.
+__device__ __forceinline__ unsigned tagged(float c, int e) {
+    const unsigned u = __float_as_uint(c), key = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return (key & ~255u) | (255u - (unsigned) e);
 }
+__device__ __forceinline__ float value_below(unsigned t) {
+    const unsigned key = t & ~255u;
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+// How far a 32-bit choice value near v can be from the 64-bit one. A sigmoid is off by less than 3e-7: its argument's rounding
+// |x| s (1 - s) 2^-23 < 3e-8, the exponential s (1 - s) 2^-23, 1 + t 2^-24, the inverse 2^-23 of s; a softmax score by less
+// than that too (its sum by 2^-23 and its exponentials' errors); the sum with the bias by 2^-24 of itself.
+__device__ __forceinline__ float margin(float v) { return 5e-7f * (1.0f + fabsf(v)); }
+constexpr int kSelMore = 3; // candidates beyond the k largest
+
+// What a wavefront knows of its lane's token.
+struct Lane {
+    const float *x;
+    int l;        // lane of the token
+    double *vals; // LDS: the token's choice values, lane by lane, in either width
+    double *s_g;  // with groups: their values, and which of them stay
+    uint32_t *s_keep;
+    int *s_id; // the chosen experts
+};
+
+// LDS of one wavefront: the choice values of each token, lane by lane, with groups their values and which of them stay, and the
+// chosen ids.
+template <int V>
+__host__ __device__ constexpr size_t select_lds(int groups) {
+    return kSelTokens * ((size_t) kSelLanes * (V + 2) * 8 + (size_t) groups * 8 + (groups ? 32 : 0) + kMaxK * 4);
+}
+// From one lane's choice values to the next's: two 64-bit or four 32-bit ones more than it has, against bank conflicts.
+template <int V, typename T>
+__host__ __device__ constexpr int stride_of() { return sizeof(T) == 8 ? V + 2 : V + 4; }
 // Orders a wavefront's LDS writes before its later reads by other lanes (they execute in order; the compiler has to as well).
 __device__ __forceinline__ void lds_in_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
 
-// V: experts per lane, 16 V >= E
-template <int V, bool SIGMOID, bool GROUPS>
-__global__ __launch_bounds__(kWave) void select_kernel(SelectParams P) {
-    extern __shared__ __align__(16) unsigned char s_all[];
-    const int l = threadIdx.x % kSelLanes, row = threadIdx.x / kSelLanes;
-    unsigned char *lds = s_all;
-    double *const s_c = reinterpret_cast<double *>(lds) + (row * kSelLanes) * (V + 2); // the token's values: lane's at (V + 2) l
-    double *const mine = s_c + l * (V + 2);
-    lds += kSelTokens * kSelLanes * (V + 2) * 8;
-    double *s_g = nullptr;
-    uint32_t *s_keep = nullptr;
-    if constexpr (GROUPS) {
-        s_g = reinterpret_cast<double *>(lds) + row * P.n_group;
-        lds += (size_t) kSelTokens * P.n_group * 8;
-        s_keep = reinterpret_cast<uint32_t *>(lds) + row * 8;
-        lds += kSelTokens * 32;
+// The two largest choice values of group g of a token, from LDS; lanes_per lanes (a power of two) take a group together.
+template <int V, typename T>
+__device__ __forceinline__ void best_two(const T *vals, int g, int per, int part, int lanes_per, T &a, T &b) {
+    a = b = -INFINITY;
+#pragma unroll 4
+    for (int j = part; j < per; j += lanes_per) {
+        const int e = g * per + j;
+        const T v = vals[(e % kSelLanes) * stride_of<V, T>() + e / kSelLanes];
+        const T low = a < v ? a : v;
+        b = b < low ? low : b;
+        a = a < v ? v : a;
     }
-    int *const s_id = reinterpret_cast<int *>(lds) + row * P.k;
-    const int64_t first = (int64_t) blockIdx.x * kSelTokens;
-    const int64_t t = min(first + row, (int64_t) P.T - 1); // rows past the last token compute it again and store nothing
-    const float *x = P.logits + t * P.ld;
-
-    float xv[V], bv[V];
+    auto join = [&](T oa, T ob) {
+        const T low = a < oa ? a : oa, high = b < ob ? ob : b;
+        a = a < oa ? oa : a;
+        b = low < high ? high : low;
+    };
+    auto dpp = [](T v, auto ctrl) {
+        if constexpr (sizeof(T) == 8) return dpp_d<decltype(ctrl)::value>(v);
+        else return dpp_f<decltype(ctrl)::value>(v);
+    };
+    if (lanes_per >= 2) join(dpp(a, std::integral_constant<int, 0xB1>()), dpp(b, std::integral_constant<int, 0xB1>()));
+    if (lanes_per >= 4) join(dpp(a, std::integral_constant<int, 0x4E>()), dpp(b, std::integral_constant<int, 0x4E>()));
+    if (lanes_per >= 8) join(dpp(a, std::integral_constant<int, 0x141>()), dpp(b, std::integral_constant<int, 0x141>()));
+    if (lanes_per >= 16) join(dpp(a, std::integral_constant<int, 0x140>()), dpp(b, std::integral_constant<int, 0x140>()));
+}
+// Which of the lane's experts may not be chosen (bit i: expert l + 16 i), from the choice values c. stays(values, g): whether
+// group g stays, 1 or 0, or -1 where that is not settled; settled then becomes false.
+template <int V, typename T, typename F>
+__device__ __forceinline__ unsigned left_out(const SelectParams &P, const Lane &L, const T (&c)[V], bool &settled, F stays) {
+    const int per = P.E / P.n_group;
+    const unsigned inv = (65536u + per - 1) / per; // e / per = e * inv >> 16 for e < 256
+    T *const vals = reinterpret_cast<T *>(L.vals), *const values = reinterpret_cast<T *>(L.s_g);
+    lds_in_order();
+#pragma unroll
+    for (int i = 0; i < V; i++) vals[L.l * stride_of<V, T>() + i] = c[i];
+    if (L.l < 8) L.s_keep[L.l] = 0;
+    lds_in_order();
+    int lanes_per = 1;
+    while (lanes_per * 2 * P.n_group <= kSelLanes) lanes_per *= 2;
+    const int at_once = kSelLanes / lanes_per;
+    for (int g0 = 0; g0 < P.n_group; g0 += at_once) { // all lanes stay in step for the DPP joins
+        const int g = g0 + L.l / lanes_per;
+        T a, b;
+        best_two<V>(vals, min(g, P.n_group - 1), per, L.l % lanes_per, lanes_per, a, b);
+        const T v = P.group_top == 2 ? a + b : a;
+        if (g < P.n_group && L.l % lanes_per == 0) values[g] = v != v ? (T) -INFINITY : v;
+    }
+    lds_in_order();
+    for (int g = L.l; g < P.n_group; g += kSelLanes) {
+        const int s = stays(values, g);
+        if (s > 0) atomicOr(&L.s_keep[g / 32], 1u << (g % 32));
+        settled = settled && s >= 0;
+    }
+    lds_in_order();
+    unsigned out = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const int e = l + kSelLanes * i;
-        xv[i] = e < P.E ? x[e] : -INFINITY;
-        bv[i] = P.bias && e < P.E ? P.bias[e] : 0.0f;
+        const unsigned g = (L.l + kSelLanes * i) * inv >> 16;
+        out |= (~L.s_keep[g / 32] >> (g % 32) & 1u) << i;
     }
-    double c[V], top = 0.0, scale = 1.0; // softmax: e^(x - top) * scale
+    return out;
+}
+
+// The k largest of the tagged values t (the lanes' own, `none` for one that may not be chosen), into s_id; returns the next.
+template <int V, typename T, typename F>
+__device__ __forceinline__ T take_largest(const Lane &L, const T (&t)[V], T none, int k, F expert) {
+    T *const mine = reinterpret_cast<T *>(L.vals) + L.l * stride_of<V, T>();
+    lds_in_order();
+    T best = none;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        mine[i] = t[i];
+        best = best < t[i] ? t[i] : best;
+    }
+    for (int j = 0; j < k; j++) {
+        const int e = expert(row_max(best));
+        if (L.l == e % kSelLanes) {
+            L.s_id[j] = e;
+            mine[e / kSelLanes] = none;
+            T v[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = mine[i];
+            best = v[0];
+#pragma unroll
+            for (int i = 1; i < V; i++) best = best < v[i] ? v[i] : best;
+        }
+    }
+    lds_in_order();
+    return row_max(best);
+}
+
+// The lane's logits and biases; -inf past the last expert.
+template <int V>
+__device__ __forceinline__ void load_lane(const SelectParams &P, const Lane &L, float (&xv)[V], float (&bv)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        xv[i] = L.x[min(L.l + kSelLanes * i, P.E - 1)];
+        bv[i] = 0.0f;
+    }
+    if (P.bias) {
+#pragma unroll
+        for (int i = 0; i < V; i++) bv[i] = P.bias[min(L.l + kSelLanes * i, P.E - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        if (L.l + kSelLanes * i >= P.E) xv[i] = -INFINITY;
+}
+
+// All in 64 bits: s_id gets the chosen experts in order. A softmax's scores are e^(x - top) scale.
+template <int V, bool SIGMOID, bool GROUPS>
+__device__ __forceinline__ void choose_exact(const SelectParams &P, const Lane &L, double &top, double &scale) {
+    float xv[V], bv[V];
+    load_lane(P, L, xv, bv);
+    double c[V];
+    top = 0.0;
+    scale = 1.0;
     if constexpr (SIGMOID) {
 #pragma unroll
         for (int i = 0; i < V; i++) c[i] = sigmoid(value_of(xv[i]));
@@ -141,89 +281,195 @@ __global__ __launch_bounds__(kWave) void select_kernel(SelectParams P) {
 #pragma unroll
         for (int i = 0; i < V; i++) c[i] *= scale;
     }
+    unsigned out = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         c[i] += (double) bv[i];
         if (c[i] != c[i]) c[i] = -INFINITY;
+        out |= (L.l + kSelLanes * i < P.E ? 0u : 1u) << i;
     }
-    unsigned out = 0; // bit i: expert l + 16 i may not be chosen
-#pragma unroll
-    for (int i = 0; i < V; i++) out |= (l + kSelLanes * i < P.E ? 0u : 1u) << i;
     if constexpr (GROUPS) {
-        const int per = P.E / P.n_group;
-        const unsigned inv = (65536u + per - 1) / per; // e / per = e * inv >> 16 for e < 256
-#pragma unroll
-        for (int i = 0; i < V; i++) mine[i] = c[i];
-        if (l < 8) s_keep[l] = 0;
-        lds_in_order();
-        for (int g = l; g < P.n_group; g += kSelLanes) {
-            double a = -INFINITY, b = -INFINITY; // the two largest
-            for (int j = 0; j < per; j++) {
-                const int e = g * per + j;
-                const double v = s_c[(e % kSelLanes) * (V + 2) + e / kSelLanes];
-                b = fmax(b, fmin(a, v));
-                a = fmax(a, v);
-            }
-            const double v = P.group_top == 2 ? a + b : a;
-            s_g[g] = v != v ? -INFINITY : v;
-        }
-        lds_in_order();
-        for (int g = l; g < P.n_group; g += kSelLanes) {
-            const double v = s_g[g];
+        bool settled = true;
+        out |= left_out<V>(P, L, c, settled, [&](const double *v, int g) {
+            const double mine = v[g];
             int rank = 0;
-            for (int j = 0; j < P.n_group; j++) {
-                const double o = s_g[j];
-                rank += o > v || (o == v && j < g);
-            }
-            if (rank < P.n_group_used) atomicOr(&s_keep[g / 32], 1u << (g % 32));
-        }
-        lds_in_order();
+            for (int j = 0; j < P.n_group; j++) rank += v[j] > mine || (v[j] == mine && j < g);
+            return rank < P.n_group_used ? 1 : 0;
+        });
+    }
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const unsigned g = (l + kSelLanes * i) * inv >> 16;
-            out |= (~s_keep[g / 32] >> (g % 32) & 1u) << i;
+    for (int i = 0; i < V; i++) c[i] = out >> i & 1u ? -INFINITY : tagged(c[i], L.l + kSelLanes * i);
+    take_largest<V>(L, c, (double) -INFINITY, P.k, [](double t) { return expert_of(t); });
+}
+
+// In 32 bits: s_id gets the n largest, in no order that counts; returns whether what stays by groups is settled, and a bound of
+// all choice values that are none of the n (in units of 1 / sum for a softmax with groups, of logits for one without). For
+// sigmoid scores, and for softmax ones without bias that are renormalised (the weights then need no exact sum over all).
+struct Fast {
+    bool settled;
+    float rest, most, sum; // most, sum: a softmax's largest logit and sum of e^(x - most)
+};
+template <int V, bool SIGMOID, bool GROUPS>
+__device__ __forceinline__ Fast choose_fast(const SelectParams &P, const Lane &L, int n) {
+    float xv[V], bv[V];
+    load_lane(P, L, xv, bv);
+    constexpr float kLog2e = 1.44269504088896341f;
+    float c[V], most = 0.0f, sum = 1.0f;
+    bool settled = true;
+    if constexpr (SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(xv[i] * -kLog2e)) + bv[i];
+    } else {
+        most = xv[0];
+#pragma unroll
+        for (int i = 1; i < V; i++) most = fmaxf(most, xv[i]);
+        most = row_max(most);
+        settled = fabsf(most) < 1e30f;
+        if constexpr (GROUPS) {
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                c[i] = __builtin_amdgcn_exp2f((xv[i] - most) * kLog2e);
+                sum += c[i];
+            }
+            sum = row_sum(sum);
+            const float inv = 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i] *= inv;
+        } else {
+            // the order of the logits is that of the scores
+#pragma unroll
+            for (int i = 0; i < V; i++) c[i] = xv[i];
         }
     }
-    double best = -INFINITY;
+    unsigned out = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const double v = out >> i & 1u ? -INFINITY : tagged(c[i], l + kSelLanes * i);
-        mine[i] = v;
-        best = fmax(best, v);
+        const bool in = L.l + kSelLanes * i < P.E;
+        out |= (in ? 0u : 1u) << i;
+        settled = settled && (c[i] < 1e30f || !in); // no NaN, nothing too large for the margins
     }
-    for (int j = 0; j < P.k; j++) {
-        const int e = expert_of(row_max(best));
-        if (l == e % kSelLanes) {
-            s_id[j] = e;
-            mine[e / kSelLanes] = -INFINITY;
-            double v[V];
+    if constexpr (GROUPS) {
+        out |= left_out<V>(P, L, c, settled, [&](const float *v, int g) {
+            const float mine = v[g];
+            int above = 0, near = 0;
+            for (int j = 0; j < P.n_group; j++) {
+                const float m = 2.0f * (margin(mine) + margin(v[j])); // each may be a sum of two
+                above += v[j] > mine + m;
+                near += !(v[j] < mine - m);
+            }
+            return near <= P.n_group_used ? 1 : above >= P.n_group_used ? 0 : -1; // `near` counts the group itself
+        });
+    }
+    unsigned t[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) v[i] = mine[i];
-            best = v[0];
+    for (int i = 0; i < V; i++) t[i] = out >> i & 1u ? 0u : tagged(c[i], L.l + kSelLanes * i);
+    const unsigned next = take_largest<V>(L, t, 0u, n, [](unsigned v) { return (int) (255u - (v & 255u)); });
+    const float v = value_below(next);
+    return {settled, next == 0 ? -INFINITY : v + fabsf(v) * 0x1p-14f + 2.0f * margin(v), most, sum};
+}
+
+// The candidates' scores and their ranks by 64-bit choice value; lane l's are s_id[l], s_id[l + 16], ..
+template <int MOST>
+struct Ranked {
+    double s[MOST], sum; // sum: of the k best of the token
+    int rank[MOST];
+};
+template <bool SIGMOID, int MOST>
+__device__ __forceinline__ Ranked<MOST> rank_candidates(const SelectParams &P, const Lane &L, int n, double top, double scale) {
+    Ranked<MOST> r;
+    lds_in_order();
 #pragma unroll
-            for (int i = 1; i < V; i++) best = fmax(best, v[i]);
+    for (int q = 0; q < MOST; q++) {
+        const int j = L.l + kSelLanes * q;
+        if (j < n) {
+            const int e = L.s_id[j];
+            const double v = value_of(L.x[e]);
+            if constexpr (SIGMOID) r.s[q] = sigmoid(v);
+            else r.s[q] = exp_of(fmax(v - top, -800.0)) * scale;
+            L.vals[j] = tagged(P.bias ? r.s[q] + (double) P.bias[e] : r.s[q], e);
         }
+        if (kSelLanes * (q + 1) >= n) break;
     }
     lds_in_order();
-    // the chosen experts' scores, 16 at a time
     double sum = 0.0;
-    auto score = [&](int j) {
-        const double v = value_of(x[s_id[j]]);
-        if constexpr (SIGMOID) return sigmoid(v);
-        else return exp_of(fmax(v - top, -800.0)) * scale;
-    };
-    for (int j = l; j < P.k; j += kSelLanes) {
-        const double s = score(j);
-        sum += s;
-        mine[j / kSelLanes] = s;
+#pragma unroll
+    for (int q = 0; q < MOST; q++) {
+        const int j = L.l + kSelLanes * q;
+        if (j < n) {
+            r.rank[q] = 0;
+            const double mine = L.vals[j];
+            for (int i = 0; i < n; i++) r.rank[q] += L.vals[i] > mine;
+            if (r.rank[q] < P.k) sum += r.s[q];
+        }
+        if (kSelLanes * (q + 1) >= n) break;
     }
-    sum = row_sum(sum);
-    if (first + row >= P.T) return;
-    const double f = (P.renorm ? 1.0 / fmax(sum, 0x1p-14) : 1.0) * (double) P.scale;
-    for (int j = l; j < P.k; j += kSelLanes) {
-        P.ids[t * P.k + j] = s_id[j];
-        P.weights[t * P.k + j] = (float) (mine[j / kSelLanes] * f);
+    r.sum = row_sum(sum);
+    return r;
+}
+template <int MOST>
+__device__ __forceinline__ void write_out(const SelectParams &P, const Lane &L, const Ranked<MOST> &r, int64_t t, int n, double f) {
+    f *= (double) P.scale;
+#pragma unroll
+    for (int q = 0; q < MOST; q++) {
+        const int j = L.l + kSelLanes * q;
+        if (j < n && r.rank[q] < P.k) {
+            P.ids[t * P.k + r.rank[q]] = L.s_id[j];
+            P.weights[t * P.k + r.rank[q]] = (float) (r.s[q] * f);
+        }
+        if (kSelLanes * (q + 1) >= n) break;
     }
+}
+
+// V: experts per lane, 16 V >= E
+template <int V, bool SIGMOID, bool GROUPS>
+__global__ __launch_bounds__(kWave) void select_kernel(SelectParams P) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    constexpr int kMost = kMaxK / kSelLanes; // candidates of a lane
+    const int l = threadIdx.x % kSelLanes, row = threadIdx.x / kSelLanes, groups = GROUPS ? P.n_group : 0;
+    Lane L;
+    L.l = l;
+    unsigned char *at = lds;
+    L.vals = reinterpret_cast<double *>(at) + row * kSelLanes * (V + 2);
+    at += kSelTokens * kSelLanes * (V + 2) * 8;
+    L.s_g = reinterpret_cast<double *>(at) + row * groups;
+    at += (size_t) kSelTokens * groups * 8;
+    L.s_keep = reinterpret_cast<uint32_t *>(at) + row * 8;
+    at += GROUPS ? kSelTokens * 32 : 0;
+    L.s_id = reinterpret_cast<int *>(at) + row * kMaxK;
+    const int64_t first = (int64_t) blockIdx.x * kSelTokens, t = min(first + row, (int64_t) P.T - 1);
+    const bool live = first + row < P.T; // rows past the last token compute it again and store nothing
+    L.x = P.logits + t * P.ld;
+
+    Ranked<kMost> r;
+    if (SIGMOID || (P.renorm && !P.bias)) {
+        const int n = min(min(P.k + kSelMore, kMaxK), GROUPS ? P.n_group_used * (P.E / P.n_group) : P.E);
+        const Fast F = choose_fast<V, SIGMOID, GROUPS>(P, L, n);
+        r = rank_candidates<SIGMOID, kMost>(P, L, n, (double) F.most, 1.0);
+        bool settled = F.settled;
+#pragma unroll
+        for (int q = 0; q < kMost; q++) {
+            const int j = l + kSelLanes * q;
+            if (j < n && r.rank[q] == P.k - 1 && n < P.E) {
+                // the last one that stays, against all that are no candidates
+                float v = SIGMOID ? (float) L.vals[j] : GROUPS ? (float) r.s[q] * (1.0f / F.sum) : L.x[L.s_id[j]];
+                settled = settled && v - margin(v) > F.rest;
+                // of a softmax also: not so small that 64 bits make it the same as others
+                if constexpr (!SIGMOID) settled = settled && r.s[q] > 1e-290;
+            }
+            if (kSelLanes * (q + 1) >= n) break;
+        }
+        // the scores' sum is held above 2^-14, which a softmax's best k without groups always are (k / E at least)
+        if constexpr (!SIGMOID && GROUPS) settled = settled && r.sum > (double) (0x1p-12f * F.sum);
+        if (__all(settled)) {
+            if (live) write_out(P, L, r, t, n, P.renorm ? 1.0 / (SIGMOID ? fmax(r.sum, 0x1p-14) : r.sum) : 1.0);
+            return;
+        }
+    }
+    double top, scale;
+    choose_exact<V, SIGMOID, GROUPS>(P, L, top, scale);
+    r = rank_candidates<SIGMOID, kMost>(P, L, P.k, top, scale);
+    if (live) write_out(P, L, r, t, P.k, P.renorm ? 1.0 / fmax(r.sum, 0x1p-14) : 1.0);
 }
 
 template <int V>
@@ -231,7 +477,7 @@ hipError_t launch_select_v(const SelectParams &P, hipStream_t st, const LaunchTi
     const bool groups = P.n_group_used < P.n_group;
     // one wavefront per work-group: with four, 60000 tokens take the same 71 us and 512 take 10.6 instead of 10.2
     const dim3 grid((P.T + kSelTokens - 1) / kSelTokens), block(kWave);
-    const size_t lds = select_lds<V>(P.k, groups ? P.n_group : 0);
+    const size_t lds = select_lds<V>(groups ? P.n_group : 0);
     if (P.sigmoid)
         return groups ? launch(select_kernel<V, true, true>, grid, block, lds, st, tm, P) : launch(select_kernel<V, true, false>, grid, block, lds, st, tm, P);
     return groups ? launch(select_kernel<V, false, true>, grid, block, lds, st, tm, P) : launch(select_kernel<V, false, false>, grid, block, lds, st, tm, P);
