@@ -114,7 +114,8 @@ int lstk_model_forward(lstk_model *model, int32_t seq, int n_tokens, int32_t n_c
  * 1 <= n_seq <= n_batch. With window > 0 each token attends its sequence's last `window` cells and first n_sink cells, else
  * all of them (lstk_attn_paged); prompts run through lstk_model_decode attend everything. d_trace, when not NULL, receives the
  * router's ids [n_layer][n_seq][n_expert_used]; a trace file (lstk_model_set_trace) gets the step like any other.
- * Nothing is appended when the arguments are rejected or the cache has no room for all of them. */
+ * Nothing is appended when the arguments are rejected or the cache has no room for all of them. The cache may have at most
+ * 2^27 cells. */
 int lstk_model_decode_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int window, int n_sink,
                             float *d_logits, int32_t *d_trace, lstk_stream_t stream);
 /* The same in two halves, like lstk_model_prepare / lstk_model_forward. prepare_batch returns the longest sequence's cells in

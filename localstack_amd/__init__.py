@@ -672,7 +672,12 @@ class Qwen3Model:
 
     def _batch_logits(self, n, logits):
         import torch
-        return torch.empty(n, self.hp["n_vocab"], dtype=torch.float32, device=self.device) if logits is None else logits
+        if logits is None:
+            return torch.empty(n, self.hp["n_vocab"], dtype=torch.float32, device=self.device)
+        if hasattr(logits, "numel") and (logits.dtype != torch.float32 or logits.numel() < n * self.hp["n_vocab"] or
+                                         not logits.is_contiguous()):
+            raise LstkError(E_INVALID, "logits must be a contiguous float32 tensor with a row of n_vocab per sequence")
+        return logits
 
     def decode_batch(self, seqs, tokens, window=0, n_sink=0, trace=None, logits=None, stream=None):
         """Appends tokens[i] to sequence seqs[i] (distinct), all in one step; returns the device logits [n_seq][n_vocab].

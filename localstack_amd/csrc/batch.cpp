@@ -23,7 +23,6 @@ bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % 
 // A launch has fewer than 2^32 threads along x, in work-groups of up to 1024.
 constexpr int64_t kMostGrid = (int64_t(1) << 22) - 1;
 constexpr int kMostHeads = 65535;
-constexpr int64_t kMostCells = int64_t(1) << 27; // of a cache: the kernel's 32-bit offsets
 constexpr int kMostTokens = 1 << 24;
 
 // Shapes of a paged attention call, checked, and its plan.
@@ -63,7 +62,7 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
     size_t bytes = 0;
     const int rc = paged_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
     if (rc != LSTK_OK) return rc;
-    if (cache->kv_size < lstk::kPageCells || cache->kv_size % lstk::kPageCells || cache->kv_size > kMostCells)
+    if (cache->kv_size < lstk::kPageCells || cache->kv_size % lstk::kPageCells || cache->kv_size > lstk::kPagedMaxCells)
         return bad("kv_size must be a positive multiple of 32, at most 2^27");
     if (seqs->n_table < 0) return bad("n_table must be >= 0");
     if (!std::isfinite(scale)) return bad("scale must be finite");

@@ -11,6 +11,7 @@
 
 namespace lstk {
 
+constexpr int64_t kPagedMaxCells = int64_t(1) << 27; // of a cache: the attention kernel's 32-bit offsets
 constexpr int kPageCells = 32; // cells of a page: the cache's block (KvCache::block_size, src/kv_cache.h:27)
 
 // Attention of one query token per sequence over one layer's cache in the cell layouts of forward.h. Logical cell i of

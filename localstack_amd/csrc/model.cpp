@@ -767,6 +767,7 @@ int check_batch(const lstk_model *M, int n_seq, const int32_t *seqs, const int32
     if (n_seq < 1 || n_seq > M->n_batch) return set_error(LSTK_E_INVALID, "n_seq must be in [1, n_batch]");
     std::vector<int32_t> sorted(seqs, seqs + n_seq);
     std::sort(sorted.begin(), sorted.end());
+    if ((int64_t) M->kv.size > lstk::kPagedMaxCells) return set_error(LSTK_E_INVALID, "batch steps take a cache of at most 2^27 cells");
     if (sorted[0] < 0) return set_error(LSTK_E_INVALID, "seq must be >= 0");
     if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
         return set_error(LSTK_E_INVALID, "a sequence is in the batch twice");

@@ -220,7 +220,9 @@ __device__ __forceinline__ T take_largest(const Lane &L, const T (&t)[V], T none
         best = best < t[i] ? t[i] : best;
     }
     for (int j = 0; j < k; j++) {
-        const int e = expert(row_max(best));
+        // (where groups are not settled there may be none left: expert 0 stands in, and choose_exact does it over)
+        const T top = row_max(best);
+        const int e = top == none ? 0 : expert(top);
         if (L.l == e % kSelLanes) {
             L.s_id[j] = e;
             mine[e / kSelLanes] = none;

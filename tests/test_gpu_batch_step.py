@@ -272,6 +272,9 @@ def test_errors(lstk, dev):
     refused(lambda: m.decode_batch(range(5), range(5)))
     refused(lambda: m.decode_batch([0], [1], window=5, n_sink=-1))
     refused(lambda: m.forward_batch(1, 10))
+    import torch
+    refused(lambda: m.decode_batch([0, 1], [1, 2], logits=torch.empty(1, 1024, device=dev)))
+    refused(lambda: m.decode_batch([0, 1], [1, 2], logits=torch.empty(2, 1024, device=dev).half()))
     n = m.prepare_batch([0, 1], [1, 2])
     assert n == 4
     refused(lambda: m.forward_batch(1, 10))

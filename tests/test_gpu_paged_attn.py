@@ -157,6 +157,19 @@ def test_many_sequences(lstk, dev):
     check(lstk, make(torch, dev, rng, 4, 2, 64, rng.integers(0, 200, 300).tolist()))
 
 
+@pytest.mark.parametrize("n,longest", [(300, 5000), (257, 3000), (1000, 2500)])
+def test_many_sequences_beside_a_long_one(lstk, dev, n, longest):
+    """More sequences than a work-group looks up at once, in equal shares of the list of pages."""
+    import torch
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 90, n).tolist()
+    lens[n // 2], lens[-1], lens[0] = longest, 2100, 0
+    c = make(torch, dev, rng, 4, 2, 64, lens)
+    assert lstk.paged_attention_work_bytes(n, 4, 2, 64, longest) > 0
+    check(lstk, c)
+    check(lstk, c, window=1000, n_sink=3)
+
+
 def test_pages_out_of_range_are_not_visible(lstk, dev):
     """Block numbers outside the cache, and table indices outside the table, hide their cells."""
     import torch
