@@ -52,7 +52,8 @@ struct SampleParams {
     const float *top_p, *min_p, *u;
     int32_t *tokens;
     float *probs;
-    int slices, slice; // work-groups per row and 16-byte quads per slice (sample_plan)
+    bool by_row;       // one work-group per row, one launch (sample_plan)
+    int slices, slice; // work-groups per row and 16-byte quads per slice
     unsigned long long *best; // [n_rows][slices] largest (logit, lowest index) of a slice
     unsigned long long *mass; // [n_rows][kSampleBins]
     uint32_t *count;          // [n_rows][kSampleBins]

@@ -22,6 +22,7 @@ typedef unsigned long long u64;
 
 constexpr int kSmThreads = 512;
 constexpr int kSmTarget = 512; // work-groups of a launch
+constexpr int kSmHeld = 24;    // quads of a thread where a row takes one work-group: up to 49149 values
 constexpr double kUnit = 0x1p44;
 // (x_max - x) / T that the bins cover; the last one starts at 31.2347, where the weight is 0.479 * 2^-44, so all that it
 // holds rounds to zero
@@ -722,12 +723,115 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
     }
 }
 
+// A row by one work-group, in one launch: the same steps with the histogram in LDS and the row, up to kSmHeld quads a thread,
+// in registers, so that it is read once. Bound by the 64-bit steps of the weights, which only two wavefronts a SIMD share: 0.7
+// us per 1000 values.
+__global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SampleParams P) {
+    __shared__ u64 s_mass[kSampleBins];
+    __shared__ uint32_t s_count[kSampleBins];
+    __shared__ double s_edge[kSampleBins];
+    __shared__ SumsLds L;
+    __shared__ Search D;
+    __shared__ uint32_t s_n;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
+    const Settings how = settings_of(P, b);
+    const Quads q = quads_of(P, b, 0);
+    float4 held[kSmHeld];
+#pragma unroll
+    for (int i = 0; i < kSmHeld; i++) {
+        const int j = tid + i * kSmThreads;
+        held[i] = j < q.end ? quad_at(q, j) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    }
+    auto all_values = [&](auto &&f) {
+#pragma unroll
+        for (int i = 0; i < kSmHeld; i++) {
+            if (i * kSmThreads >= q.end) break;
+            const int at = 4 * (tid + i * kSmThreads) - q.off;
+            f(held[i].x, at);
+            f(held[i].y, at + 1);
+            f(held[i].z, at + 2);
+            f(held[i].w, at + 3);
+        }
+    };
+    for (int i = tid; i < kSampleBins; i += kSmThreads) {
+        s_mass[i] = 0;
+        s_count[i] = 0;
+        s_edge[i] = edge_weight(i);
+    }
+    if (tid == 0) s_n = 0;
+
+    float top = -INFINITY;
+    int top_at = 0;
+    all_values([&](float x, int i) {
+        x = x > FLT_MAX ? FLT_MAX : x;
+        if (x > top) { // (a NaN is not)
+            top = x;
+            top_at = i;
+        }
+    });
+    u64 best = wave_max_u64(top > -INFINITY ? place_of(top, top_at) : 0);
+    if (lane == 0) L.wave_mass[wv] = best;
+    __syncthreads();
+    for (int w = 0; w < kSmThreads / kWave; w++) best = L.wave_mass[w] > best ? L.wave_mass[w] : best;
+    __syncthreads();
+    if (best == 0 || how.greedy) {
+        if (tid == 0) {
+            P.tokens[b] = best == 0 ? -1 : (int32_t) ~(uint32_t) best;
+            if (P.probs) P.probs[b] = best == 0 ? 0.0f : 1.0f;
+        }
+        return;
+    }
+    const Row r = row_of(how, best);
+    const bool ranked = how.k != UINT_MAX;
+    all_values([&](float x, int) {
+        if (!(x >= r.least)) return;
+        const double below = bins_below(r, fminf(x, FLT_MAX));
+        const int bin = (int) below;
+        const u64 m = mass_of(r, below, bin, s_edge[bin]);
+        if (m == 0) return;
+        atomicAdd(&s_mass[bin], m);
+        if (ranked) atomicAdd(&s_count[bin], 1u);
+    });
+    __syncthreads();
+    const Sums S = sums_of(s_mass, s_count, L);
+    const Cuts c = cuts_of(how, S, L);
+    u64 *const list = P.list + (int64_t) b * P.n_vocab;
+    auto write_through = [&](uint32_t at, u64 p) { __hip_atomic_store(list + at, p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const Span drawn = span_of(r, c.d_lo, c.d_hi);
+    const Span cut = c.part ? span_of(r, c.cut.bin, c.cut.bin) : drawn, run = c.by_p ? span_of(r, c.p_lo, c.p_hi) : drawn;
+    all_values([&](float x, int i) {
+        if (!(drawn.holds(x) || cut.holds(x) || run.holds(x))) return;
+        x = fminf(x, FLT_MAX);
+        const double below = bins_below(r, x);
+        const int bin = (int) below;
+        if (!c.holds(bin) || mass_of(r, below, bin, s_edge[bin]) == 0) return;
+        const uint32_t at = atomicAdd(&s_n, 1u);
+        if (at < (uint32_t) kSmGather) D.gathered[at] = place_of(x, (uint32_t) i);
+        else write_through(at, place_of(x, (uint32_t) i));
+    });
+    __syncthreads();
+    const uint32_t n = s_n;
+    if (n <= (uint32_t) kSmKeep) {
+        sort_gathered(r, D, (int) n, [&](int i) { return D.gathered[i]; });
+        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_sorted<by_mass>(r, D, f, (int) n, target); });
+    } else {
+        for (int i = tid; i < kSmGather; i += kSmThreads) write_through(i, D.gathered[i]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        draw(P, how, b, r, c, S, L, [&](auto by_mass, const Found &f, u64 target) { return reach_in_list<by_mass>(r, list, D, f, n, target); });
+    }
+}
+
 }  // namespace
 
 size_t sample_plan(SampleParams &P, void *work) {
     // slices of at least 1024 quads, as many as bring the launches to kSmTarget work-groups; a row out of line has a quad more
     const int quads = (P.n_vocab + 6) / 4;
-    P.slices = std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, kSmTarget / std::max(1, P.n_rows)));
+    // One work-group a row, in one launch, for rows of up to 16384 values, and where there are many for all that it can hold. Us
+    // a call, so and in slices: one row of 1000 values 12 and 19, of 8192 16 and 21, of 32768 30 and 22; 256 rows of 5000 15 and
+    // 30; 64 rows of 32768 32 and 31; 250 of 38000 40 and 50.
+    P.by_row = quads <= kSmHeld * kSmThreads && (P.n_vocab <= 16384 || P.n_rows >= 96);
+    P.slices = P.by_row ? 1 : std::max(1, std::min((quads + kSmThreads - 1) / kSmThreads, kSmTarget / std::max(1, P.n_rows)));
     P.slice = (quads + P.slices - 1) / P.slices;
     size_t off = 0;
     auto take = [&](auto *&p, size_t n) {
@@ -747,6 +851,7 @@ size_t sample_plan(SampleParams &P, void *work) {
 hipError_t launch_sample(const SampleParams &P, hipStream_t st) {
     if (P.n_rows <= 0) return hipSuccess;
     const dim3 all((unsigned) (P.n_rows * P.slices)), block(kSmThreads);
+    if (P.by_row) return launch(sample_row_kernel, all, block, 0, st, nullptr, P);
     hipError_t e;
     if ((e = launch(sample_max_kernel, all, block, 0, st, nullptr, P)) != hipSuccess) return e;
     if ((e = launch(sample_bins_kernel, all, block, 0, st, nullptr, P)) != hipSuccess) return e;

@@ -111,6 +111,20 @@ def test_equal_values(lstk, dev):
     check(lstk, dev, x, [0.0], k=[3], borders=True)
 
 
+@pytest.mark.parametrize("n,V", [(3, 1024), (3, 1025), (2, 16384), (2, 16385), (97, 40000), (96, 49149), (96, 49150)])
+def test_many_equal_values_in_one_row(lstk, dev, n, V):
+    """More values where a cut falls than are sorted, with one work-group to a row and with several, at the sizes where that and
+    the row's place in registers change."""
+    rng = np.random.default_rng(V)
+    x = np.zeros((n, V), np.float32)
+    x[::2] = (rng.integers(0, 3, V) / 7).astype(np.float32)
+    x[0] = 2.2 * rng.standard_normal(V).astype(np.float32)
+    u = rng.random(n).astype(np.float32)
+    check(lstk, dev, x, u, borders=True)
+    check(lstk, dev, x, u, k=[V // 2 + 3] * n, p=[0.625] * n, borders=True)
+    check(lstk, dev, x, u, p=[0.5] * n, m=[0.25] * n, borders=True)
+
+
 def test_special_values(lstk, dev):
     inf, nan = np.inf, np.nan
     rows = [[-inf] * 6, [nan] * 6, [-inf, nan, -inf, 3.0, nan, -inf], [1, nan, 2, -inf, 0, 1], [inf, 1, 2, inf, 3, -inf], [FMAX, inf, -FMAX, 0, 1, 2],
