@@ -39,9 +39,10 @@ int paged_plan(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, 
     P.max_len = max_len;
     P.window = window > 0 ? window : 0;
     P.n_sink = n_sink;
-    bytes = lstk::paged_attn_plan(P);
-    if (n_head > kMostHeads || (int64_t) n_seq * n_head_kv * P.n_rowblk > kMostGrid)
+    const int row_blocks = (n_head / n_head_kv - 1) / 16 + 1;
+    if (n_head > kMostHeads || (int64_t) n_seq * n_head_kv * row_blocks > kMostGrid)
         return bad("too many sequences or heads for one launch");
+    bytes = lstk::paged_attn_plan(P);
     return LSTK_OK;
 }
 

@@ -39,6 +39,8 @@ struct Span {
     int n, lo, sink; // cells; first cell of the window; sink cells
     int ps, pw, count;
 };
+// Pages of n cells; n may be the largest 32-bit number.
+__device__ __forceinline__ int pages_of(int n) { return n / kPageCells + (n % kPageCells != 0); }
 // Pages that a sequence has in the list: one at least, so that one without any is written (zeros) like the others.
 __device__ __forceinline__ int listed(const Span &s) { return max(1, s.count); }
 __device__ __forceinline__ Span span_of(const PagedAttnParams &P, int len) {
@@ -47,8 +49,8 @@ __device__ __forceinline__ Span span_of(const PagedAttnParams &P, int len) {
     s.lo = P.window > 0 && s.n > P.window ? s.n - P.window : 0;
     s.sink = min(P.n_sink, s.lo);
     s.pw = s.lo / kPageCells;
-    s.ps = min((s.sink + kPageCells - 1) / kPageCells, s.pw);
-    s.count = s.ps + (s.n + kPageCells - 1) / kPageCells - s.pw;
+    s.ps = min(pages_of(s.sink), s.pw);
+    s.count = s.ps + pages_of(s.n) - s.pw;
     return s;
 }
 

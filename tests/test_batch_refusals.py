@@ -111,3 +111,11 @@ def test_tensors_on_the_host_are_refused(lstk):
         with pytest.raises(lstk.LstkError) as e:
             f()
         assert e.value.code == lstk.E_INVALID
+
+
+def test_attention_counts_tasks_before_it_plans(lstk):
+    """Sequences times heads times pages past 2^63: refused, with no workspace, from the number of tasks alone."""
+    big = dict(n_seq=2 ** 31 - 1, n_head=65535, n_kv=65535, max_len=2 ** 31 - 1)
+    assert attn(lstk, **big, work=P, work_bytes=2 ** 62) == lstk.E_INVALID
+    assert b"too many" in lstk.lib().lstk_last_error()
+    assert lstk.paged_attention_work_bytes(2 ** 31 - 1, 65535, 65535, 64, 2 ** 31 - 1) == 0

@@ -343,3 +343,17 @@ def test_refusals_of_tensors(lstk, dev):
         lstk.paged_attention(**{**ok, "max_len": 100000, "work": torch.empty(16, dtype=torch.uint8, device=dev)})
     empty = lstk.paged_attention(c["qd"][:0], c["kc"], c["vc"], c["lens"][:0], c["first"][:0], c["blocks"], 60)
     assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("n_sink", [0, 5])
+def test_the_longest_length(lstk, dev, n_sink):
+    """A sequence of 2^31 - 1 cells whose window's two pages are the only ones in the table (its list starts before it)."""
+    import torch
+    c = make(torch, dev, np.random.default_rng(18), 32, 4, 128, [64, 64])
+    n, window = 2 ** 31 - 1, 40
+    c["max_len"] = n
+    c["lens"].fill_(n)
+    c["first"].copy_(torch.tensor([2 * b - (2 ** 26 - 2) for b in range(2)], dtype=torch.int32))
+    c["rows"] = [r[:63] for r in c["rows"]]  # the second page's last cell would be the one after
+    vis = [np.arange(63) >= 63 - window for _ in range(2)]
+    check(lstk, c, visible=vis, window=window, n_sink=n_sink)
