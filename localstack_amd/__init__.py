@@ -328,19 +328,31 @@ def _on_device(dev, stream, call):
         handle = torch._C._cuda_getCurrentRawStream(dev)
     else:
         handle = stream if isinstance(stream, int) else stream.cuda_stream
+        if getattr(stream, "device_index", dev) != dev:
+            raise LstkError(E_INVALID, f"the stream is of GPU {stream.device_index}, the tensors of GPU {dev}")
     if torch.cuda.current_device() == dev:
         return call(handle)
     with torch.cuda.device(dev):
         return call(handle)
 
 
-def _work(given, nbytes, dev, stream):
-    """(tensor, pointer, bytes) of the caller's workspace, or of a new one that lives until `stream` is done with it."""
+def _empty(shape, dtype, dev, stream):
+    """A new tensor for the work of `stream`: of that stream's memory, since what the current stream has freed may still be in use
+    by what it has queued."""
     import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=dev)
+
+
+def _work(given, nbytes, dev, stream):
+    """(tensor, pointer, bytes) of the caller's workspace, or of a new one."""
     if given is None:
-        given = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        if stream is not None:
-            given.record_stream(torch.cuda.ExternalStream(stream, device=dev) if isinstance(stream, int) else stream)
+        import torch
+        given = _empty(nbytes, torch.uint8, dev, stream)
     elif not hasattr(given, "data_ptr") or given.get_device() != dev or not given.is_contiguous():
         raise LstkError(E_INVALID, f"work must be a contiguous tensor on GPU {dev}")
     return given, given.data_ptr(), given.numel() * given.element_size()
@@ -367,9 +379,9 @@ def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, s
     k = int(n_expert_used)
     shape = (T, k)
     if ids is None:
-        ids = torch.empty(T, max(k, 0), dtype=torch.int32, device=dev)
+        ids = _empty((T, max(k, 0)), torch.int32, dev, stream)
     if weights is None:
-        weights = torch.empty(T, max(k, 0), dtype=torch.float32, device=dev)
+        weights = _empty((T, max(k, 0)), torch.float32, dev, stream)
     ip, wp = _tensor(ids, "ids", torch.int32, shape, dev), _tensor(weights, "weights", torch.float32, shape, dev)
     _check(_on_device(dev, stream, lambda st: lib().lstk_moe_select(ctypes.byref(rule.c), p, ld, b, T, E, k, ip, wp, st)))
     return ids, weights
@@ -401,7 +413,7 @@ def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0,
     s = PagedSeqs(n, int(max_len), _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table,
                   blocks.numel(), None if seqs is None else _tensor(seqs, "seqs", i32, (n,), dev))
     if out is None:
-        out = torch.empty_like(q)
+        out = _empty(shape, f16, dev, stream)
     op = _tensor(out, "out", f16, shape, dev)
     need = 0 if work is not None else lib().lstk_attn_paged_work_bytes(n, H, kv, hd, s.max_len, int(window), int(n_sink))
     wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
@@ -429,9 +441,9 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
                    None if min_p is None else _tensor(min_p, "min_p", f32, shape, dev))
     up = _tensor(u, "u", f32, shape, dev)
     if tokens is None:
-        tokens = torch.empty(n, dtype=i32, device=dev)
+        tokens = _empty(n, i32, dev, stream)
     if probs is None:
-        probs = torch.empty(n, dtype=f32, device=dev)
+        probs = _empty(n, f32, dev, stream)
     tp, pp = _tensor(tokens, "tokens", i32, shape, dev), _tensor(probs, "probs", f32, shape, dev)
     wt, wp, wn = _work(work, lib().lstk_sample_work_bytes(n, V) if work is None else 0, dev, stream)
     _check(_on_device(dev, stream, lambda st: lib().lstk_sample(p, ld, n, V, ctypes.byref(how), up, tp, pp, wp, wn, st)))
@@ -670,10 +682,10 @@ class Qwen3Model:
                                         _stream(stream)))
         return out
 
-    def _batch_logits(self, n, logits):
+    def _batch_logits(self, n, logits, stream):
         import torch
         if logits is None:
-            return torch.empty(n, self.hp["n_vocab"], dtype=torch.float32, device=self.device)
+            return _empty((n, self.hp["n_vocab"]), torch.float32, self.device, stream)
         if hasattr(logits, "numel") and (logits.dtype != torch.float32 or logits.numel() < n * self.hp["n_vocab"] or
                                          not logits.is_contiguous()):
             raise LstkError(E_INVALID, "logits must be a contiguous float32 tensor with a row of n_vocab per sequence")
@@ -686,7 +698,7 @@ class Qwen3Model:
         s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
         if s.size != tok.size:
             raise LstkError(E_INVALID, "one token per sequence")
-        out = self._batch_logits(s.size, logits)
+        out = self._batch_logits(s.size, logits, stream)
         _check(lib().lstk_model_decode_batch(self._h, s.size, s.ctypes.data, tok.ctypes.data, int(window), int(n_sink), _ptr(out),
                                              _ptr(trace), _stream(stream)))
         return out
@@ -702,7 +714,7 @@ class Qwen3Model:
 
     def forward_batch(self, n_seq, max_len, window=0, n_sink=0, trace=None, logits=None, stream=None):
         """Second half of a batch step (capturable; replays after each prepare_batch of n_seq sequences up to max_len)."""
-        out = self._batch_logits(n_seq, logits)
+        out = self._batch_logits(n_seq, logits, stream)
         _check(lib().lstk_model_forward_batch(self._h, int(n_seq), int(max_len), int(window), int(n_sink), _ptr(out), _ptr(trace),
                                               _stream(stream)))
         return out

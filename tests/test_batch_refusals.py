@@ -113,6 +113,16 @@ def test_tensors_on_the_host_are_refused(lstk):
         assert e.value.code == lstk.E_INVALID
 
 
+def test_a_stream_of_another_gpu_is_refused(lstk):
+    """Before the call is made; the stream stands for one of GPU 1, the tensors' is GPU 0."""
+    class Other:
+        cuda_stream, device_index = P, 1
+    called = []
+    with pytest.raises(lstk.LstkError) as e:
+        lstk._on_device(0, Other(), called.append)
+    assert e.value.code == lstk.E_INVALID and not called
+
+
 def test_attention_counts_tasks_before_it_plans(lstk):
     """Sequences times heads times pages past 2^63: refused, with no workspace, from the number of tasks alone."""
     big = dict(n_seq=2 ** 31 - 1, n_head=65535, n_kv=65535, max_len=2 ** 31 - 1)

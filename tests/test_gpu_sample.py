@@ -232,3 +232,24 @@ def test_refusals_of_tensors(lstk, dev):
         assert e.value.code == lstk.E_INVALID, kw
     t, p = lstk.sample(x[:0], u[:0])
     assert t.numel() == 0 and p.numel() == 0
+
+
+def test_new_tensors_are_of_the_given_stream(lstk, dev):
+    """What a call allocates for another stream is not memory that the current stream has just freed (its kernels may still be
+    at work there), whether the stream comes as an object or as a handle."""
+    import torch
+    x, u = torch.zeros(4, 20000, device=dev), torch.zeros(4, device=dev)
+    sizes = (lstk.sample_work_bytes(4, 20000), 16, 16)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream):
+        freed = [torch.empty(n, dtype=torch.uint8, device=dev) for n in sizes for _ in range(2)]
+        at = {t.data_ptr() for t in freed}
+        del freed
+        work = lstk._work(None, sizes[0], 0, stream)[0]
+        tokens, probs = lstk.sample(x, u, work=work, stream=stream)
+        side.synchronize()
+        assert not at & {t.data_ptr() for t in (work, tokens, probs)}
+        assert (tokens == 0).all()
+    work = lstk._work(None, sizes[0], 0, 0)[0]  # the null stream's handle
+    assert (lstk.sample(x, u, work=work, stream=0)[0].cpu() == 0).all()
