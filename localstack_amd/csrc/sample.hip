@@ -10,8 +10,9 @@
 // counts and weights over kSampleBins equal steps of (x_max - x) / T says in which bins the three cuts fall; only those
 // bins' values are looked at one by one. Weights that round to zero cannot be drawn and take no part.
 //
-// Measured on MI355X: 64 rows of 151936 values (39 MB) 58 us in three launches of 9 (reading at 4.3 TB/s), 17 (the 64-bit steps of
-// the weights) and 32 us (waits in turn: histogram, cuts, the row again, the row's last work-group); one such row 22 us.
+// Measured on MI355X: 64 rows of 151936 values (39 MB) 58 us in three launches of 9 (reading at 4.3 TB/s), 17 (the vector units
+// are busy for 39% of it, mostly with the weights; the rest are waits, LDS atomics among them) and 32 us (18%; waits in turn:
+// histogram, cuts, the row again, the row's last work-group); one such row 22 us.
 
 #include <cfloat>
 #include <type_traits>
@@ -728,8 +729,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_pick_kernel(SampleParams P)
 }
 
 // A row by one work-group, in one launch: the same steps with the histogram in LDS and the row, up to kSmHeld quads a thread,
-// in registers, so that it is read once. Bound by the 64-bit steps of the weights, which only two wavefronts a SIMD share: 0.7
-// us per 1000 values.
+// in registers, so that it is read once. 0.7 us per 1000 values: two wavefronts a SIMD do not cover each other's waits.
 __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SampleParams P) {
     __shared__ u64 s_mass[kSampleBins];
     __shared__ uint32_t s_count[kSampleBins];
