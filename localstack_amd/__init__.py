@@ -600,6 +600,7 @@ class Qwen3Model:
     def __init__(self, hp, weights, store, kv_size, n_batch, device="cuda", join_qkv=True):
         import torch
         self.hp = dict(hp)
+        self.n_batch = int(n_batch)
         self.store = store
         self.device = torch.device(device)
         self._keep = []
@@ -728,6 +729,10 @@ class Qwen3Model:
         n, V = len(seqs), self.hp["n_vocab"]
         if n == 0 or n_new <= 0:
             return {s: [] for s in seqs}
+        if n > self.n_batch:
+            raise LstkError(E_INVALID, f"{n} sequences in a model of {self.n_batch} tokens a step")
+        if any(len(p) == 0 for p in prompts.values()):
+            raise LstkError(E_INVALID, "an empty prompt")
 
         def setting(v, dtype):
             v = torch.as_tensor(v, dtype=dtype).flatten()

@@ -319,3 +319,16 @@ def test_trace_file(lstk, dev, tmp_path):
     np.testing.assert_array_equal(v[1:9].reshape(2, 2, 2), tr.cpu().numpy())
     v = v[9:]
     assert v[0] == 1 and len(v) == 5 and (v[1:] >= 0).all()
+
+
+def test_generate_refuses_before_it_appends(lstk, dev):
+    hp, w = weights("tiny")
+    store, m = build(lstk, dev, hp, w, n_batch=2)
+    for prompts in ({0: [1], 1: [2], 2: [3]}, {0: [1, 2], 1: []}):
+        with pytest.raises(lstk.LstkError) as e:
+            m.generate(prompts, 3)
+        assert e.value.code == lstk.E_INVALID
+        assert [m.seq_len(s) for s in range(3)] == [0, 0, 0]
+    assert [len(t) for t in m.generate({0: [1], 1: [2]}, 3).values()] == [3, 3]
+    m.close()
+    store.close()
