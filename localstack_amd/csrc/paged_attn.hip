@@ -13,8 +13,9 @@
 // at 64 on 4 (410 MB) 75 us. Short calls are bound by the way to the first page (length, first table entry, block number, K:
 // four waits on memory, 4.4 us in all) and, split, by the second launch (4 to 6 us).
 //
-// A page (32 cells) costs a wavefront 2 HD / 32 16 x 16 x 32 fp16 matrix instructions for S^T = K Q^T and as many for
-// O^T += V^T P^T, every operand as the cache holds it: a lane's 16-byte load of K is 4 dims of two neighbouring cells, so one
+// A page (32 cells) costs a wavefront 2 HD / 32 16 x 16 x 32 fp16 matrix instructions for S^T = K Q^T and twice as many for
+// O^T += V^T P^T (P as a sum of two fp16 parts, like the attention of steps of one sequence: 0.2% of the time of 128 sequences,
+// 4% of 64 short ones'), every operand as the cache holds it: a lane's 16-byte load of K is 4 dims of two neighbouring cells, so one
 // load feeds the tile of the even and that of the odd cells, and the two results leave a lane with 8 consecutive cells of one
 // query head, which is its share of the second product's operand P. Nothing goes through LDS between the products. V
 // likewise: 4 cells of two neighbouring dims.
@@ -33,6 +34,11 @@ constexpr int kPaPerCu = 2; // work-groups of equal shares per CU
 constexpr int kPaLeast = 4; // pages of a share
 constexpr int kPaRound = 4;  // rounds of the wavefronts up to which a share is made a whole number of them
 constexpr float kLowest = -3.0e38f; // a running maximum that any score replaces
+// The running maximum m that is kept lies 15 below the largest score, so that weights reach 2^15 and fp16 holds those down to
+// 2^-29 of the largest as normal numbers. Scores so large that the difference would be rounded by more than 2^-4 stay as they
+// are (a weight of 2^16 would be an infinity).
+constexpr float kBelow = 15.0f, kExactTo = 0x1p20f;
+__device__ __forceinline__ float maximum_kept(float top) { return fabsf(top) < kExactTo ? top - kBelow : top; }
 
 // The pages of a sequence that hold visible cells: [0, ps) and [pw, pw + count - ps).
 struct Span {
@@ -276,24 +282,32 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
             float top = s[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
-            top = fmaxf(m_run, across_groups_max(top));
+            top = fmaxf(m_run, maximum_kept(across_groups_max(top)));
             const float f = __builtin_amdgcn_exp2f(m_run - top);
             m_run = top;
             l_run *= f;
 #pragma unroll
             for (int t = 0; t < 2 * NM; t++) o[t] *= f;
-            // p rounded to fp16 for the matrix product (half a step, 2^-11 of each weight), and summed as rounded, so that the
-            // weights used add up to the sum divided by
-            half8v p;
+            // p = hi + lo in fp16 for the matrix products, to 2^-22 of each weight, or to 2^-40 of the largest where lo leaves
+            // fp16's normal numbers; the sum takes p itself
+            half8v hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                p[e] = (_Float16) __builtin_amdgcn_exp2f(s[e] - m_run);
-                l_run += (float) p[e];
+                const float p = __builtin_amdgcn_exp2f(s[e] - m_run);
+                hi[e] = (_Float16) p;
+                lo[e] = (_Float16) (p - (float) hi[e]);
+                l_run += p;
+            }
+            __builtin_amdgcn_sched_barrier(0); // (registers: without it four spill at head size 128)
+#pragma unroll
+            for (int t = 0; t < NM; t++) {
+                o[2 * t] = mfma(halves(v[2 * t].x, v[2 * t].y, v[2 * t + 1].x, v[2 * t + 1].y), lo, o[2 * t]);
+                o[2 * t + 1] = mfma(halves(v[2 * t].z, v[2 * t].w, v[2 * t + 1].z, v[2 * t + 1].w), lo, o[2 * t + 1]);
             }
 #pragma unroll
             for (int t = 0; t < NM; t++) {
-                o[2 * t] = mfma(halves(v[2 * t].x, v[2 * t].y, v[2 * t + 1].x, v[2 * t + 1].y), p, o[2 * t]);
-                o[2 * t + 1] = mfma(halves(v[2 * t].z, v[2 * t].w, v[2 * t + 1].z, v[2 * t + 1].w), p, o[2 * t + 1]);
+                o[2 * t] = mfma(halves(v[2 * t].x, v[2 * t].y, v[2 * t + 1].x, v[2 * t + 1].y), hi, o[2 * t]);
+                o[2 * t + 1] = mfma(halves(v[2 * t].z, v[2 * t].w, v[2 * t + 1].z, v[2 * t + 1].w), hi, o[2 * t + 1]);
             }
         }
 
