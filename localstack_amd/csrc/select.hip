@@ -12,9 +12,9 @@
 // chosen weights are rounded once, to fp32.
 //
 // 16 lanes (a DPP row) take a token, so a wavefront takes four, and lane l the experts l, l + 16, ..: a row's maximum is four
-// DPP steps. A choice value carries its expert in its lowest 8 bits, so that the maximum says whose it is and of equal values
-// the lowest id is the largest. In each of the k rounds the lane that owned the maximum takes it out of its values in LDS and
-// finds its next one; the others keep theirs.
+// DPP steps. A 32-bit choice value carries its expert in its lowest 8 bits, so that the maximum says whose it is; 64-bit ones keep
+// all their bits, and a second maximum finds the lowest id among equal ones. In each of the k rounds the lane that owned the
+// maximum takes it out of its values in LDS and finds its next one; the others keep theirs.
 //
 // Bound by vector instructions, 1450 a wavefront (the units are busy for 75% of the time), not by the 65 MB of 60000 tokens over
 // 256 experts, which take 49 us with sigmoid scores, bias and 4 of 8 groups on MI355X; 512 such tokens take 7 us, or 15 where
@@ -82,6 +82,12 @@ __device__ __forceinline__ unsigned row_max(unsigned v) {
     v = max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x141, 0xF, 0xF, false));
     return max(v, (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x140, 0xF, 0xF, false));
 }
+__device__ __forceinline__ unsigned row_sum(unsigned v) {
+    v += (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0xB1, 0xF, 0xF, false);
+    v += (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x4E, 0xF, 0xF, false);
+    v += (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x141, 0xF, 0xF, false);
+    return v + (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, 0x140, 0xF, 0xF, false);
+}
 __device__ __forceinline__ float row_max(float v) {
     v = fmaxf(v, dpp_f<0xB1>(v));
     v = fmaxf(v, dpp_f<0x4E>(v));
@@ -95,20 +101,12 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + dpp_f<0x140>(v);
 }
 
-// A choice value with its expert: larger is earlier. -inf becomes a finite value below all others, so that it stays above what
-// may not be chosen at all (-inf here).
-__device__ __forceinline__ double tagged(double c, int e) {
-    c = fmin(fmax(c, -0x1p1023), 0x1p1023); // (a NaN becomes -2^1023)
-    const unsigned long long u = __builtin_bit_cast(unsigned long long, c);
-    return __builtin_bit_cast(double, (u & ~255ull) | (u >> 63 ? (unsigned) e : 255u - (unsigned) e));
-}
-__device__ __forceinline__ int expert_of(double t) {
-    const unsigned long long u = __builtin_bit_cast(unsigned long long, t);
-    return (int) (u >> 63 ? u & 255u : 255u - (u & 255u));
-}
+// A choice value as it is ordered: -inf and NaN become a finite value below all others, so that they stay above what may not be
+// chosen at all (-inf here).
+__device__ __forceinline__ double ordered(double c) { return fmax(c, -0x1p1000); }
 
-// The same in 32 bits, as a whole number: the order-preserving key of c with the expert in place of its lowest 8 bits; 0 is
-// below all of them. value_below is at most 2^-14 |c| below c, and never above it.
+// A 32-bit choice value with its expert, as a whole number: the order-preserving key of c with the expert in place of its lowest 8
+// bits; 0 is below all of them. value_below is at most 2^-14 |c| below c, and never above it.
 __device__ __forceinline__ unsigned tagged(float c, int e) {
     const unsigned u = __float_as_uint(c), key = u & 0x80000000u ? ~u : u | 0x80000000u;
     return (key & ~255u) | (255u - (unsigned) e);
@@ -212,12 +210,12 @@ __device__ __forceinline__ unsigned left_out(const SelectParams &P, const Lane &
     return out;
 }
 
-// The k largest of the tagged values t (the lanes' own, `none` for one that may not be chosen), into s_id; returns the next.
-template <int V, typename T, typename F>
-__device__ __forceinline__ T take_largest(const Lane &L, const T (&t)[V], T none, int k, F expert) {
-    T *const mine = reinterpret_cast<T *>(L.vals) + L.l * stride_of<V, T>();
+// The k largest of the tagged values t (the lanes' own, 0 for one that may not be chosen), into s_id; returns the next.
+template <int V>
+__device__ __forceinline__ unsigned take_largest(const Lane &L, const unsigned (&t)[V], int k) {
+    unsigned *const mine = reinterpret_cast<unsigned *>(L.vals) + L.l * stride_of<V, unsigned>();
     lds_in_order();
-    T best = none;
+    unsigned best = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         mine[i] = t[i];
@@ -225,12 +223,12 @@ __device__ __forceinline__ T take_largest(const Lane &L, const T (&t)[V], T none
     }
     for (int j = 0; j < k; j++) {
         // (where groups are not settled there may be none left: expert 0 stands in, and choose_exact does it over)
-        const T top = row_max(best);
-        const int e = top == none ? 0 : expert(top);
+        const unsigned top = row_max(best);
+        const int e = top == 0 ? 0 : (int) (255u - (top & 255u));
         if (L.l == e % kSelLanes) {
             L.s_id[j] = e;
-            mine[e / kSelLanes] = none;
-            T v[V];
+            mine[e / kSelLanes] = 0;
+            unsigned v[V];
 #pragma unroll
             for (int i = 0; i < V; i++) v[i] = mine[i];
             best = v[0];
@@ -240,6 +238,36 @@ __device__ __forceinline__ T take_largest(const Lane &L, const T (&t)[V], T none
     }
     lds_in_order();
     return row_max(best);
+}
+
+// The k largest of the 64-bit values c (ordered(); -inf for one that may not be chosen), of equal ones the lowest id first, into
+// s_id in that order. The ids stand apart from the values: in their lowest 8 bits they would make values 2^-45 of themselves apart
+// equal, as saturated sigmoids are.
+template <int V>
+__device__ __forceinline__ void take_largest(const Lane &L, const double (&c)[V], int k) {
+    double *const mine = L.vals + L.l * stride_of<V, double>();
+    lds_in_order();
+    double v[V], best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        mine[i] = v[i] = c[i];
+        best = fmax(best, c[i]);
+    }
+    for (int j = 0; j < k; j++) {
+        const double top = row_max(best);
+        int at = V; // the lane's first value that is the largest
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--) at = v[i] == top ? i : at;
+        const int e = 255 - (int) row_max(at < V ? 255u - (unsigned) (L.l + kSelLanes * at) : 0u);
+        if (L.l == e % kSelLanes) {
+            L.s_id[j] = e;
+            mine[e / kSelLanes] = -INFINITY;
+            best = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < V; i++) best = fmax(best, v[i] = mine[i]);
+        }
+    }
+    lds_in_order();
 }
 
 // The lane's logits and biases; -inf past the last expert.
@@ -304,8 +332,8 @@ __device__ __forceinline__ void choose_exact(const SelectParams &P, const Lane &
         });
     }
 #pragma unroll
-    for (int i = 0; i < V; i++) c[i] = out >> i & 1u ? -INFINITY : tagged(c[i], L.l + kSelLanes * i);
-    take_largest<V>(L, c, (double) -INFINITY, P.k, [](double t) { return expert_of(t); });
+    for (int i = 0; i < V; i++) c[i] = out >> i & 1u ? -INFINITY : ordered(c[i]);
+    take_largest<V>(L, c, P.k);
 }
 
 // In 32 bits: s_id gets the n largest, in no order that counts; returns whether what stays by groups is settled, and a bound of
@@ -370,7 +398,7 @@ __device__ __forceinline__ Fast choose_fast(const SelectParams &P, const Lane &L
     unsigned t[V];
 #pragma unroll
     for (int i = 0; i < V; i++) t[i] = out >> i & 1u ? 0u : tagged(c[i], L.l + kSelLanes * i);
-    const unsigned next = take_largest<V>(L, t, 0u, n, [](unsigned v) { return (int) (255u - (v & 255u)); });
+    const unsigned next = take_largest<V>(L, t, n);
     const float v = value_below(next);
     return {settled, next == 0 ? -INFINITY : v + fabsf(v) * 0x1p-14f + 2.0f * margin(v), most, sum};
 }
@@ -393,12 +421,12 @@ __device__ __forceinline__ Ranked<MOST> rank_candidates(const SelectParams &P, c
             const double v = value_of(L.x[e]);
             if constexpr (SIGMOID) r.s[q] = sigmoid(v);
             else r.s[q] = exp_of(fmax(v - top, -800.0)) * scale;
-            L.vals[j] = tagged(P.bias ? r.s[q] + (double) P.bias[e] : r.s[q], e);
+            L.vals[j] = ordered(P.bias ? r.s[q] + (double) P.bias[e] : r.s[q]);
         }
         if (kSelLanes * (q + 1) >= n) break;
     }
     lds_in_order();
-    double sum = 0.0;
+    unsigned ranks = 0;
 #pragma unroll
     for (int q = 0; q < MOST; q++) {
         const int j = L.l + kSelLanes * q;
@@ -406,8 +434,28 @@ __device__ __forceinline__ Ranked<MOST> rank_candidates(const SelectParams &P, c
             r.rank[q] = 0;
             const double mine = L.vals[j];
             for (int i = 0; i < n; i++) r.rank[q] += L.vals[i] > mine;
-            if (r.rank[q] < P.k) sum += r.s[q];
+            ranks += (unsigned) r.rank[q];
         }
+        if (kSelLanes * (q + 1) >= n) break;
+    }
+    // of equal values the lowest id is first; there are some where the ranks add up to less than 0 + 1 + .. + n - 1 (comparing ids
+    // with every value costs 60000 tokens 5 us)
+    if (__any(row_sum(ranks) != (unsigned) (n * (n - 1) / 2))) {
+#pragma unroll
+        for (int q = 0; q < MOST; q++) {
+            const int j = L.l + kSelLanes * q;
+            if (j < n) {
+                const double mine = L.vals[j];
+                const int e = L.s_id[j];
+                for (int i = 0; i < n; i++) r.rank[q] += L.vals[i] == mine && L.s_id[i] < e;
+            }
+            if (kSelLanes * (q + 1) >= n) break;
+        }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < MOST; q++) {
+        if (L.l + kSelLanes * q < n && r.rank[q] < P.k) sum += r.s[q];
         if (kSelLanes * (q + 1) >= n) break;
     }
     r.sum = row_sum(sum);
