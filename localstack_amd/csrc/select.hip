@@ -117,7 +117,8 @@ __device__ __forceinline__ float value_below(unsigned t) {
 }
 // How far a 32-bit choice value near v can be from the 64-bit one. A sigmoid is off by less than 3e-7: its argument's rounding
 // |x| s (1 - s) 2^-23 < 3e-8, the exponential s (1 - s) 2^-23, 1 + t 2^-24, the inverse 2^-23 of s; a softmax score by less
-// than that too (its sum by 2^-23 and its exponentials' errors); the sum with the bias by 2^-24 of itself.
+// than that too (its sum by 2^-23 and its exponentials' errors); the sum with the bias by 2^-24 of itself. The rest, 2e-7 and
+// 4e-7 |v|, covers the roundings of a group's sum and of the comparisons.
 __device__ __forceinline__ float margin(float v) { return 5e-7f * (1.0f + fabsf(v)); }
 constexpr int kSelMore = 3; // candidates beyond the k largest
 
@@ -126,7 +127,7 @@ struct Lane {
     const float *x;
     int l;        // lane of the token
     double *vals; // LDS: the token's choice values, lane by lane, in either width
-    double *s_g;  // with groups: their values, and which of them stay
+    double *s_g;  // with groups: their values (in 32 bits margins too), and which of them stay
     uint32_t *s_keep;
     int *s_id; // the chosen experts
 };
@@ -173,7 +174,8 @@ __device__ __forceinline__ void best_two(const T *vals, int g, int per, int part
     if (lanes_per >= 16) join(dpp(a, std::integral_constant<int, 0x140>()), dpp(b, std::integral_constant<int, 0x140>()));
 }
 // Which of the lane's experts may not be chosen (bit i: expert l + 16 i), from the choice values c. stays(values, g): whether
-// group g stays, 1 or 0, or -1 where that is not settled; settled then becomes false.
+// group g stays, 1 or 0, or -1 where that is not settled; settled then becomes false. Behind 32-bit values stand how far they can be
+// off: the margins of their summands, which may be far larger than their sum.
 template <int V, typename T, typename F>
 __device__ __forceinline__ unsigned left_out(const SelectParams &P, const Lane &L, const T (&c)[V], bool &settled, F stays) {
     const int per = P.E / P.n_group;
@@ -192,7 +194,10 @@ __device__ __forceinline__ unsigned left_out(const SelectParams &P, const Lane &
         T a, b;
         best_two<V>(vals, min(g, P.n_group - 1), per, L.l % lanes_per, lanes_per, a, b);
         const T v = P.group_top == 2 ? a + b : a;
-        if (g < P.n_group && L.l % lanes_per == 0) values[g] = v != v ? (T) -INFINITY : v;
+        if (g < P.n_group && L.l % lanes_per == 0) {
+            values[g] = v != v ? (T) -INFINITY : v;
+            if constexpr (sizeof(T) == 4) values[P.n_group + g] = P.group_top == 2 ? margin(a) + margin(b) : margin(a);
+        }
     }
     lds_in_order();
     for (int g = L.l; g < P.n_group; g += kSelLanes) {
@@ -385,10 +390,10 @@ __device__ __forceinline__ Fast choose_fast(const SelectParams &P, const Lane &L
     }
     if constexpr (GROUPS) {
         out |= left_out<V>(P, L, c, settled, [&](const float *v, int g) {
-            const float mine = v[g];
+            const float mine = v[g], mine_m = v[P.n_group + g];
             int above = 0, near = 0;
             for (int j = 0; j < P.n_group; j++) {
-                const float m = 2.0f * (margin(mine) + margin(v[j])); // each may be a sum of two
+                const float m = mine_m + v[P.n_group + j];
                 above += v[j] > mine + m;
                 near += !(v[j] < mine - m);
             }
