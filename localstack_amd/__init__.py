@@ -230,6 +230,15 @@ def _stream(stream):
     return stream.cuda_stream
 
 
+def _current_device():
+    """torch's current GPU, -1 without one."""
+    try:
+        import torch
+    except ImportError:
+        return -1
+    return torch.cuda.current_device() if torch.cuda.is_available() else -1
+
+
 def matrix_bytes(type_, rows, cols):
     return lib().lstk_matrix_bytes(type_, rows, cols)
 
@@ -319,6 +328,25 @@ def _rows(t, name, dtype):
     if (m > 1 and one != 1) or (n > 1 and ld < m):
         raise LstkError(E_INVALID, f"{name} must have contiguous rows that do not overlap")
     return t.data_ptr(), ld if n > 1 else m, n, m, dev
+
+
+def _buffer(t, name, dtype, least, dev):
+    """Pointer of a contiguous tensor on GPU `dev` with at least `least` elements of this dtype (None: bytes of any), for calls
+    that also take raw device pointers (integers) and None."""
+    if t is None or isinstance(t, int):
+        return t
+    try:
+        fits = (dtype is None or t.dtype is dtype) and t.is_contiguous()
+        room = t.numel() * (t.element_size() if dtype is None else 1)
+        on = t.get_device()
+    except AttributeError:
+        raise LstkError(E_INVALID, f"{name} must be a tensor or a device pointer, got {type(t)}") from None
+    if not fits or room < least:
+        raise LstkError(E_INVALID, f"{name} must be a contiguous tensor of at least {least} " +
+                        (f"bytes, got {room}" if dtype is None else f"{dtype} elements, got {t.dtype} {tuple(t.shape)}"))
+    if on < 0 or on != dev:
+        raise LstkError(E_INVALID, f"{name} is on {t.device}" + (f", not on GPU {dev}" if dev >= 0 else ", not on the GPU"))
+    return t.data_ptr()
 
 
 def _on_device(dev, stream, call):
@@ -486,6 +514,7 @@ class ExpertStore:
         _check(lib().lstk_pool_create(ctypes.byref(self.dims), ctypes.cast(arr, ctypes.c_void_p), int(pool_bytes),
                                       int(min_slots), flags, ctypes.byref(h)))
         self._h = h
+        self._dev = -1 if dry else _current_device()  # the pool lives on it
         self._keep = None  # the pool copied what it needs
         self._destroy = lib().lstk_pool_destroy  # held, so that closing works during interpreter shutdown
         _stores.add(self)
@@ -546,10 +575,17 @@ class ExpertStore:
                                     _stream(stream)))
 
     def route_by(self, layer, rule, hnorm, gate_inp, gate_type, ids, weights, bias=None, n_tokens=None, stream=None):
-        """route() by a RouterRule; bias: f32 [n_expert] or None."""
-        T = hnorm.shape[0] if n_tokens is None else n_tokens
-        _check(lib().lstk_moe_route_by(self._h, layer, ctypes.byref(rule.c), _ptr(hnorm), T, _ptr(gate_inp), gate_type, _ptr(bias),
-                                       _ptr(ids), _ptr(weights), _stream(stream)))
+        """route() by a RouterRule; bias: f32 [n_expert] or None. Tensors are checked for their type, size and device."""
+        import torch
+        T = hnorm.shape[0] if n_tokens is None else int(n_tokens)
+        d, dev, rows = self.dims, self._dev, max(T, 0)
+        x = _buffer(hnorm, "hnorm", torch.float32, rows * d.n_embd, dev)
+        gate = _buffer(gate_inp, "gate_inp", None, d.n_expert * d.n_embd * (4 if gate_type == TYPE_F32 else 2), dev)
+        b = _buffer(bias, "bias", torch.float32, d.n_expert, dev)
+        i = _buffer(ids, "ids", torch.int32, rows * d.n_expert_used, dev)
+        w = _buffer(weights, "weights", torch.float32, rows * d.n_expert_used, dev)
+        call = lambda st: lib().lstk_moe_route_by(self._h, layer, ctypes.byref(rule.c), x, T, gate, gate_type, b, i, w, st)
+        _check(_on_device(dev, stream, call) if dev >= 0 else call(None))
 
     def ffn(self, layer, hnorm, slots, weights, resid, out, n_tokens=None, stream=None):
         T = hnorm.shape[0] if n_tokens is None else n_tokens
@@ -683,13 +719,17 @@ class Qwen3Model:
                                         _stream(stream)))
         return out
 
-    def _batch_logits(self, n, logits, stream):
+    def _batch_call(self, n, logits, trace, stream, call):
+        """The step's logits; call(logits pointer, trace pointer, stream handle) on the model's device, after a look at what the
+        kernels will write to."""
         import torch
+        dev, hp = self.logits.get_device(), self.hp
+        rows = max(int(n), 0)
+        tr = _buffer(trace, "trace", torch.int32, hp["n_layer"] * rows * hp["n_expert_used"], dev)
         if logits is None:
-            return _empty((n, self.hp["n_vocab"]), torch.float32, self.device, stream)
-        if hasattr(logits, "numel") and (logits.dtype != torch.float32 or logits.numel() < n * self.hp["n_vocab"] or
-                                         not logits.is_contiguous()):
-            raise LstkError(E_INVALID, "logits must be a contiguous float32 tensor with a row of n_vocab per sequence")
+            logits = _empty((rows, hp["n_vocab"]), torch.float32, self.logits.device, stream)
+        out = _buffer(logits, "logits", torch.float32, rows * hp["n_vocab"], dev)
+        _check(_on_device(dev, stream, lambda st: call(out, tr, st)))
         return logits
 
     def decode_batch(self, seqs, tokens, window=0, n_sink=0, trace=None, logits=None, stream=None):
@@ -699,10 +739,8 @@ class Qwen3Model:
         s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
         if s.size != tok.size:
             raise LstkError(E_INVALID, "one token per sequence")
-        out = self._batch_logits(s.size, logits, stream)
-        _check(lib().lstk_model_decode_batch(self._h, s.size, s.ctypes.data, tok.ctypes.data, int(window), int(n_sink), _ptr(out),
-                                             _ptr(trace), _stream(stream)))
-        return out
+        return self._batch_call(s.size, logits, trace, stream, lambda out, tr, st: lib().lstk_model_decode_batch(
+            self._h, s.size, s.ctypes.data, tok.ctypes.data, int(window), int(n_sink), out, tr, st))
 
     def prepare_batch(self, seqs, tokens, stream=None):
         """First half of a batch step; returns the longest sequence's cells."""
@@ -710,15 +748,14 @@ class Qwen3Model:
         if s.size != tok.size:
             raise LstkError(E_INVALID, "one token per sequence")
         n = ctypes.c_int32()
-        _check(lib().lstk_model_prepare_batch(self._h, s.size, s.ctypes.data, tok.ctypes.data, ctypes.byref(n), _stream(stream)))
+        _check(_on_device(self.logits.get_device(), stream, lambda st: lib().lstk_model_prepare_batch(
+            self._h, s.size, s.ctypes.data, tok.ctypes.data, ctypes.byref(n), st)))
         return n.value
 
     def forward_batch(self, n_seq, max_len, window=0, n_sink=0, trace=None, logits=None, stream=None):
         """Second half of a batch step (capturable; replays after each prepare_batch of n_seq sequences up to max_len)."""
-        out = self._batch_logits(n_seq, logits, stream)
-        _check(lib().lstk_model_forward_batch(self._h, int(n_seq), int(max_len), int(window), int(n_sink), _ptr(out), _ptr(trace),
-                                              _stream(stream)))
-        return out
+        return self._batch_call(n_seq, logits, trace, stream, lambda out, tr, st: lib().lstk_model_forward_batch(
+            self._h, int(n_seq), int(max_len), int(window), int(n_sink), out, tr, st))
 
     def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0):
         """Continues several sequences together: prompts is {seq: token ids}, each is decoded (appended to what seq holds), then
