@@ -293,6 +293,38 @@ def unpack_matrix(type_, rows, cols, packed):
 
 
 # ---- operators of a step over many sequences -------------------------------------------------------
+_MOST = 2 ** 31 - 1
+
+
+def _i32(v, name):
+    """v as a number that the library's 32-bit arguments hold (ctypes would drop its upper bits)."""
+    try:
+        i = int(v)
+    except (TypeError, ValueError, OverflowError):
+        raise LstkError(E_INVALID, f"{name} must be a whole number, got {v!r}") from None
+    if not -_MOST - 1 <= i <= _MOST:
+        raise LstkError(E_INVALID, f"{name} must fit 32 bits, got {i}")
+    return i
+
+
+def _check_i32(**named):
+    for name, v in named.items():
+        _i32(v, name)
+
+
+def _ids32(a, name):
+    """An int32 array of these host numbers; numpy would drop their upper bits or fractions."""
+    v = np.asarray(a)
+    try:
+        with np.errstate(invalid="ignore"):
+            i = np.ascontiguousarray(v, dtype=np.int32).ravel()
+    except (TypeError, ValueError, OverflowError):
+        i = None
+    if i is None or not np.array_equal(i, v.ravel()):
+        raise LstkError(E_INVALID, f"{name} must be whole numbers of 32 bits")
+    return i
+
+
 # A call that takes the device a few microseconds is bound by what Python does around it, so the checks below look at each
 # tensor once, in the cheapest order, and build a message only when one fails.
 
@@ -394,8 +426,9 @@ class RouterRule:
     def __init__(self, score="softmax", n_group=1, n_group_used=None, group_top=1, renorm=True, scale=1.0):
         if score not in ("softmax", "sigmoid"):
             raise LstkError(E_INVALID, f"unknown score function {score!r}")
-        self.c = CRouterRule(SCORE_SIGMOID if score == "sigmoid" else SCORE_SOFTMAX, int(n_group),
-                             int(n_group if n_group_used is None else n_group_used), int(group_top), 1 if renorm else 0, float(scale))
+        self.c = CRouterRule(SCORE_SIGMOID if score == "sigmoid" else SCORE_SOFTMAX, _i32(n_group, "n_group"),
+                             _i32(n_group if n_group_used is None else n_group_used, "n_group_used"), _i32(group_top, "group_top"),
+                             1 if renorm else 0, float(scale))
 
 
 def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, stream=None):
@@ -405,6 +438,8 @@ def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, s
     p, ld, T, E, dev = _rows(logits, "logits", torch.float32)
     b = None if bias is None else _tensor(bias, "bias", torch.float32, (E,), dev)
     k = int(n_expert_used)
+    if max(T, E, k) > _MOST or k < 0:
+        _check_i32(n_tokens=T, n_expert=E, n_expert_used=k)
     shape = (T, k)
     if ids is None:
         ids = _empty((T, max(k, 0)), torch.int32, dev, stream)
@@ -416,8 +451,9 @@ def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, s
 
 
 def paged_attention_work_bytes(n_seq, n_head, n_head_kv, head_dim, max_len, window=0, n_sink=0):
-    return lib().lstk_attn_paged_work_bytes(int(n_seq), int(n_head), int(n_head_kv), int(head_dim), int(max_len), int(window),
-                                            int(n_sink))
+    return lib().lstk_attn_paged_work_bytes(_i32(n_seq, "n_seq"), _i32(n_head, "n_head"), _i32(n_head_kv, "n_head_kv"),
+                                            _i32(head_dim, "head_dim"), _i32(max_len, "max_len"), _i32(window, "window"),
+                                            _i32(n_sink, "n_sink"))
 
 
 def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0, n_sink=0, scale=None, cell_seq=None, seqs=None,
@@ -430,6 +466,7 @@ def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0,
     n_sink. cell_seq (int32 [kv_size]) with seqs (int32 [n_seq]): cells of other owners are not visible. Returns out, like q."""
     import torch
     i32, f16 = torch.int32, torch.float16
+    max_len, window, n_sink = int(max_len), int(window), int(n_sink)
     qp = _tensor(q, "q", f16, (None, None, None))
     dev = q.get_device()
     n, H, hd = shape = q.shape
@@ -438,21 +475,23 @@ def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0,
     cache = PagedCache(kp, _tensor(v_cache, "v_cache", f16, (kv, size // 4, hd, 4), dev), size, kv, hd,
                        None if cell_seq is None else _tensor(cell_seq, "cell_seq", i32, (size,), dev))
     table = _tensor(blocks, "blocks", i32, (None,), dev)
-    s = PagedSeqs(n, int(max_len), _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table,
+    if max(max_len, window, n_sink, n, H, kv, blocks.numel()) > _MOST or min(max_len, window, n_sink) < 0:
+        _check_i32(max_len=max_len, window=window, n_sink=n_sink, n_seq=n, n_head=H, n_head_kv=kv, n_table=blocks.numel())
+    s = PagedSeqs(n, max_len, _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table,
                   blocks.numel(), None if seqs is None else _tensor(seqs, "seqs", i32, (n,), dev))
     if out is None:
         out = _empty(shape, f16, dev, stream)
     op = _tensor(out, "out", f16, shape, dev)
-    need = 0 if work is not None else lib().lstk_attn_paged_work_bytes(n, H, kv, hd, s.max_len, int(window), int(n_sink))
+    need = 0 if work is not None else lib().lstk_attn_paged_work_bytes(n, H, kv, hd, max_len, window, n_sink)
     wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
     f = float(hd ** -0.5 if scale is None else scale)
-    _check(_on_device(dev, stream, lambda st: lib().lstk_attn_paged(ctypes.byref(cache), ctypes.byref(s), qp, H, int(window),
-                                                                    int(n_sink), f, op, wp, wn, st)))
+    _check(_on_device(dev, stream, lambda st: lib().lstk_attn_paged(ctypes.byref(cache), ctypes.byref(s), qp, H, window, n_sink, f,
+                                                                    op, wp, wn, st)))
     return out
 
 
 def sample_work_bytes(n_rows, n_vocab):
-    return lib().lstk_sample_work_bytes(int(n_rows), int(n_vocab))
+    return lib().lstk_sample_work_bytes(_i32(n_rows, "n_rows"), _i32(n_vocab, "n_vocab"))
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None, work=None, stream=None):
@@ -462,6 +501,8 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     import torch
     f32, i32 = torch.float32, torch.int32
     p, ld, n, V, dev = _rows(logits, "logits", f32)
+    if max(n, V) > _MOST:
+        _check_i32(n_rows=n, n_vocab=V)
     shape = (n,)
     how = Sampling(None if temperature is None else _tensor(temperature, "temperature", f32, shape, dev),
                    None if top_k is None else _tensor(top_k, "top_k", i32, shape, dev),
@@ -577,7 +618,8 @@ class ExpertStore:
     def route_by(self, layer, rule, hnorm, gate_inp, gate_type, ids, weights, bias=None, n_tokens=None, stream=None):
         """route() by a RouterRule; bias: f32 [n_expert] or None. Tensors are checked for their type, size and device."""
         import torch
-        T = hnorm.shape[0] if n_tokens is None else int(n_tokens)
+        T = _i32(hnorm.shape[0] if n_tokens is None else n_tokens, "n_tokens")
+        layer, gate_type = _i32(layer, "layer"), _i32(gate_type, "gate_type")
         d, dev, rows = self.dims, self._dev, max(T, 0)
         x = _buffer(hnorm, "hnorm", torch.float32, rows * d.n_embd, dev)
         gate = _buffer(gate_inp, "gate_inp", None, d.n_expert * d.n_embd * (4 if gate_type == TYPE_F32 else 2), dev)
@@ -724,7 +766,7 @@ class Qwen3Model:
         kernels will write to."""
         import torch
         dev, hp = self.logits.get_device(), self.hp
-        rows = max(int(n), 0)
+        rows = max(n, 0)
         tr = _buffer(trace, "trace", torch.int32, hp["n_layer"] * rows * hp["n_expert_used"], dev)
         if logits is None:
             logits = _empty((rows, hp["n_vocab"]), torch.float32, self.logits.device, stream)
@@ -736,15 +778,16 @@ class Qwen3Model:
         """Appends tokens[i] to sequence seqs[i] (distinct), all in one step; returns the device logits [n_seq][n_vocab].
         window > 0: each token attends its sequence's last `window` cells and first n_sink. trace: as decode's, with a row for
         every sequence."""
-        s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
+        s, tok = _ids32(seqs, "sequences"), _ids32(tokens, "tokens")
         if s.size != tok.size:
             raise LstkError(E_INVALID, "one token per sequence")
+        window, n_sink = _i32(window, "window"), _i32(n_sink, "n_sink")
         return self._batch_call(s.size, logits, trace, stream, lambda out, tr, st: lib().lstk_model_decode_batch(
-            self._h, s.size, s.ctypes.data, tok.ctypes.data, int(window), int(n_sink), out, tr, st))
+            self._h, s.size, s.ctypes.data, tok.ctypes.data, window, n_sink, out, tr, st))
 
     def prepare_batch(self, seqs, tokens, stream=None):
         """First half of a batch step; returns the longest sequence's cells."""
-        s, tok = (np.ascontiguousarray(a, dtype=np.int32).ravel() for a in (seqs, tokens))
+        s, tok = _ids32(seqs, "sequences"), _ids32(tokens, "tokens")
         if s.size != tok.size:
             raise LstkError(E_INVALID, "one token per sequence")
         n = ctypes.c_int32()
@@ -754,8 +797,10 @@ class Qwen3Model:
 
     def forward_batch(self, n_seq, max_len, window=0, n_sink=0, trace=None, logits=None, stream=None):
         """Second half of a batch step (capturable; replays after each prepare_batch of n_seq sequences up to max_len)."""
+        n_seq, max_len, window, n_sink = (_i32(v, n) for v, n in ((n_seq, "n_seq"), (max_len, "max_len"), (window, "window"),
+                                                                  (n_sink, "n_sink")))
         return self._batch_call(n_seq, logits, trace, stream, lambda out, tr, st: lib().lstk_model_forward_batch(
-            self._h, int(n_seq), int(max_len), int(window), int(n_sink), out, tr, st))
+            self._h, n_seq, max_len, window, n_sink, out, tr, st))
 
     def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0):
         """Continues several sequences together: prompts is {seq: token ids}, each is decoded (appended to what seq holds), then
