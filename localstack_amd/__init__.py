@@ -805,34 +805,62 @@ class Qwen3Model:
     def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0):
         """Continues several sequences together: prompts is {seq: token ids}, each is decoded (appended to what seq holds), then
         n_new tokens are sampled for all of them, a batch step each. Returns {seq: the n_new tokens}; the last is not appended.
-        The settings are numbers, or sequences with one per prompt; generator: a torch generator on the model's device."""
+        The settings are numbers, or sequences with one per prompt; generator: a torch generator on the model's device. Arguments
+        are checked before anything is appended; where a later step fails (no room in the cache, a sequence without a finite
+        logit) every sequence is cut back to what it held before."""
         import torch
-        seqs = [int(s) for s in prompts]
+        seqs = _ids32(list(prompts), "sequences").tolist()
         n, V = len(seqs), self.hp["n_vocab"]
         if n == 0 or n_new <= 0:
             return {s: [] for s in seqs}
         if n > self.n_batch:
             raise LstkError(E_INVALID, f"{n} sequences in a model of {self.n_batch} tokens a step")
-        if any(len(p) == 0 for p in prompts.values()):
-            raise LstkError(E_INVALID, "an empty prompt")
+        if min(seqs) < 0:
+            raise LstkError(E_INVALID, "a sequence below 0")
+        window, n_sink = _i32(window, "window"), _i32(n_sink, "n_sink")
+        if n_sink < 0:
+            raise LstkError(E_INVALID, "n_sink must be >= 0")
+        tokens = {s: _ids32(prompts[s], f"the tokens of sequence {s}") for s in seqs}
+        for s, t in tokens.items():
+            if t.size == 0:
+                raise LstkError(E_INVALID, f"sequence {s}: an empty prompt")
+            if t.min() < 0 or t.max() >= V:
+                raise LstkError(E_INVALID, f"sequence {s}: token id out of range")
 
         def setting(v, dtype):
-            v = torch.as_tensor(v, dtype=dtype).flatten()
+            v = torch.as_tensor(v).flatten()
             if v.numel() not in (1, n):
                 raise LstkError(E_INVALID, "a setting is one number, or one per prompt")
-            return v.expand(n).contiguous().to(self.device)
+            w = v.to(dtype)
+            if dtype is torch.int32 and not torch.equal(w.to(v.dtype), v):
+                raise LstkError(E_INVALID, "top_k must be whole numbers of 32 bits")
+            return w.expand(n).contiguous().to(self.device)
 
         how = dict(temperature=setting(temperature, torch.float32), top_k=setting(top_k, torch.int32),
                    top_p=setting(top_p, torch.float32), min_p=setting(min_p, torch.float32))
-        logits = torch.empty(n, V, dtype=torch.float32, device=self.device)
-        for i, s in enumerate(seqs):
-            self.decode(s, prompts[s], logits=logits[i])
-        got = []
-        for i in range(n_new):
-            u = torch.rand(n, device=self.device, generator=generator)
-            got.append(sample(logits, u, **how)[0].cpu().numpy())
-            if i + 1 < n_new:
-                self.decode_batch(seqs, got[-1], window=window, n_sink=n_sink, logits=logits)
+        before = {s: self.seq_len(s) for s in seqs}
+        try:
+            with torch.cuda.device(self.logits.device):
+                logits = torch.empty(n, V, dtype=torch.float32, device=self.device)
+                for i, s in enumerate(seqs):
+                    self.decode(s, tokens[s], logits=logits[i])
+                got = []
+                for i in range(n_new):
+                    u = torch.rand(n, device=self.device, generator=generator)
+                    t = sample(logits, u, **how)[0].cpu().numpy()
+                    if t.min() < 0:
+                        raise LstkError(E_INVALID, f"sequence {seqs[int(t.argmin())]} has no finite logit at new token {i}")
+                    got.append(t)
+                    if i + 1 < n_new:
+                        self.decode_batch(seqs, t, window=window, n_sink=n_sink, logits=logits)
+        except BaseException:
+            for s, length in before.items():
+                try:
+                    if self.seq_len(s) > length:
+                        self.truncate_seq(s, length)
+                except LstkError:
+                    pass  # the first error is the one to report
+            raise
         return {s: [int(t[i]) for t in got] for i, s in enumerate(seqs)}
 
     def fill_context(self, seq, n_cells, seed=0, stream=None):
