@@ -101,6 +101,7 @@ int lstk_model_decode(lstk_model *model, int32_t seq, const int32_t *tokens, int
  *   n_tokens and n_cells (n_cells changes only when the sequence crosses a multiple of 256 cells),
  *   wherever the new cells lie: while the stream is capturing, attention covers cells [0, n_cells)
  *   (an eager forward starts at the sequence's lowest cache block instead).
+ *   Where the step last prepared is a batch step (below) it is refused, unless it is being captured.
  *   With a streaming pool it synchronises the stream once per layer (the router's ids go to the host),
  *   unless the pool was created with LSTK_POOL_DEVICE_LRU: then the experts are acquired on the device
  *   (lstk_pool_acquire_device), nothing waits on the host and the forward may be captured too. */

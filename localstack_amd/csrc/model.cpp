@@ -837,7 +837,16 @@ int lstk_model_forward(lstk_model *model, int32_t seq, int n_tokens, int32_t n_c
     if (!model || !d_logits) return set_error(LSTK_E_INVALID, "null argument");
     if (seq < 0 || n_tokens < 1 || n_tokens > model->n_batch || n_cells < 1 || n_cells > (int32_t) model->kv.size)
         return set_error(LSTK_E_INVALID, "seq must be >= 0, n_tokens in [1, n_batch], n_cells in [1, kv_size]");
-    return forward(model, seq, n_tokens, n_cells, d_logits, d_trace, static_cast<hipStream_t>(stream));
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (model->batch_n > 0) {
+        // the inputs are a batch step's; a capture does not run on them
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        const hipError_t e = hipStreamIsCapturing(st, &capturing);
+        if (e != hipSuccess) return hip_fail(e, "hipStreamIsCapturing");
+        if (capturing == hipStreamCaptureStatusNone)
+            return set_error(LSTK_E_INVALID, "the step last prepared is a batch step (lstk_model_forward_batch)");
+    }
+    return forward(model, seq, n_tokens, n_cells, d_logits, d_trace, st);
 }
 
 int lstk_model_decode_batch(lstk_model *model, int n_seq, const int32_t *seqs, const int32_t *tokens, int window, int n_sink,
