@@ -126,7 +126,9 @@ __device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, K
     s.total = 0;
     for (int w = 0; w < kPaWaves; w++) s.total += s_sum[w];
     s.total = uniform(s.total * tasks);
-    // small shares are whole rounds of the wavefronts
+    // Small shares are whole rounds of the wavefronts, so that few sequences have fewer parts to join. Us a call so and without, with
+    // room for 131072 cells: one sequence of 5000 cells 14.1 and 15.9, four of 200 to 3000 at 64 heads on 4 13.8 and 15.8; but 24
+    // of 100 to 1500 18.4 and 16.8, 24 of 45 to 500 at 16 on 2 of 256 17.1 and 14.5; larger calls differ by 2% or less.
     s.each = (s.total + gridDim.x - 1) / gridDim.x;
     if (s.each <= kPaRound * kPaWaves) s.each = (s.each + kPaWaves - 1) / kPaWaves * kPaWaves;
     const int64_t lo = s.each * blockIdx.x;
