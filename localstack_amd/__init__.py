@@ -314,8 +314,8 @@ def _check_i32(**named):
 
 def _ids32(a, name):
     """An int32 array of these host numbers; numpy would drop their upper bits or fractions."""
-    v = np.asarray(a)
     try:
+        v = np.asarray(a)
         with np.errstate(invalid="ignore"):
             i = np.ascontiguousarray(v, dtype=np.int32).ravel()
     except (TypeError, ValueError, OverflowError):

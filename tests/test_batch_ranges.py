@@ -93,6 +93,6 @@ def test_ids_of_every_kind(lstk):
         got = lstk._ids32(a, "x")
         assert got.dtype == np.int32 and got.tolist() == [1, 2] and got.flags.c_contiguous
     assert lstk._ids32([], "x").size == 0
-    for a in ([1.5], [float("nan")], [float("inf")], ["a"], [None], np.array([3e9])):
+    for a in ([1.5], [float("nan")], [float("inf")], ["a"], [None], np.array([3e9]), [[1], [2, 3]], iter([1])):
         with pytest.raises(lstk.LstkError):
             lstk._ids32(a, "x")
