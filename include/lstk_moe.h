@@ -166,7 +166,7 @@ int lstk_moe_route(lstk_pool *pool, int layer, const float *d_hnorm, int n_token
  *   n_group_used best groups stay (equal values: the lower group);
  *   of their experts the n_expert_used largest c are chosen (equal values: the lower id), written in that order;
  *   weight = s (without bias), divided by max(sum of the chosen s, 2^-14) if renorm, times scale.
- * A token whose logits are all -inf has softmax scores 0. Scores and choice values are held in 64 bits. */
+ * A token whose logits are all -inf has softmax scores 0. Scores and choice values are held in 64 bits, and ordered by all of them. */
 #define LSTK_SCORE_SOFTMAX 0
 #define LSTK_SCORE_SIGMOID 1
 typedef struct lstk_router_rule {

@@ -137,7 +137,8 @@ int lstk_model_forward_batch(lstk_model *model, int n_seq, int32_t max_len, int 
  * the first n_sink (counted in cells the row holds). A page whose table index (outside [0, n_table)) or block number (outside the cache) is out of range is
  * not visible; with d_cell_seq [kv_size] and d_seq [n_seq] given (both or neither), nor is a cell whose d_cell_seq entry is
  * not d_seq[b]. What the cache holds in cells that are not visible is never used, whatever it is; a row with no visible cell
- * gets zeros. */
+ * gets zeros. A NaN or an infinity in a visible cell can make its head's output NaN. Sums are fp32; a weight enters them as two fp16
+ * parts, good to 2^-22 (to 2^-40 of the largest where it is below 2^-18 of it). */
 typedef struct lstk_paged_cache {
     const uint16_t *d_k, *d_v;
     int64_t kv_size;
@@ -167,6 +168,8 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
  *   of those the shortest run from the top that holds top_p of their sum (>= 1: all; the largest always);
  *   the token is the first whose running sum exceeds u times the sum of what stays, u in [0, 1); its probability is w over
  *   that sum. temperature <= 0 or NaN: the largest value, probability 1.
+ * w is held as a whole multiple of 2^-44 (from a series good to 1.8e-14), so that sums are exact and the same in any order: a value
+ * whose w is below 2^-45 is never drawn.
  * A row with nothing above -inf gives token -1 and probability 0. The four setting arrays are on the device, [n_rows] each;
  * a NULL one means temperature 1 / no cut; a NaN top_p or min_p means no cut. Row r of the logits is at
  * d_logits + r * ld_logits; n_vocab < 2^20. d_probs may be NULL. The workspace is as lstk_attn_paged's. */
