@@ -438,7 +438,7 @@ def moe_select(logits, n_expert_used, rule, bias=None, ids=None, weights=None, s
     p, ld, T, E, dev = _rows(logits, "logits", torch.float32)
     b = None if bias is None else _tensor(bias, "bias", torch.float32, (E,), dev)
     k = int(n_expert_used)
-    if max(T, E, k) > _MOST or k < 0:
+    if not (T <= _MOST and E <= _MOST and 0 <= k <= _MOST):
         _check_i32(n_tokens=T, n_expert=E, n_expert_used=k)
     shape = (T, k)
     if ids is None:
@@ -475,8 +475,9 @@ def paged_attention(q, k_cache, v_cache, lens, first, blocks, max_len, window=0,
     cache = PagedCache(kp, _tensor(v_cache, "v_cache", f16, (kv, size // 4, hd, 4), dev), size, kv, hd,
                        None if cell_seq is None else _tensor(cell_seq, "cell_seq", i32, (size,), dev))
     table = _tensor(blocks, "blocks", i32, (None,), dev)
-    if max(max_len, window, n_sink, n, H, kv, blocks.numel()) > _MOST or min(max_len, window, n_sink) < 0:
-        _check_i32(max_len=max_len, window=window, n_sink=n_sink, n_seq=n, n_head=H, n_head_kv=kv, n_table=blocks.numel())
+    # (the other sizes are those of tensors that would not fit the device)
+    if not (0 <= max_len <= _MOST and 0 <= window <= _MOST and 0 <= n_sink <= _MOST and blocks.numel() <= _MOST):
+        _check_i32(max_len=max_len, window=window, n_sink=n_sink, n_table=blocks.numel())
     s = PagedSeqs(n, max_len, _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table,
                   blocks.numel(), None if seqs is None else _tensor(seqs, "seqs", i32, (n,), dev))
     if out is None:
@@ -501,7 +502,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     import torch
     f32, i32 = torch.float32, torch.int32
     p, ld, n, V, dev = _rows(logits, "logits", f32)
-    if max(n, V) > _MOST:
+    if not (n <= _MOST and V <= _MOST):
         _check_i32(n_rows=n, n_vocab=V)
     shape = (n,)
     how = Sampling(None if temperature is None else _tensor(temperature, "temperature", f32, shape, dev),
