@@ -182,6 +182,65 @@ size_t lstk_sample_work_bytes(int n_rows, int n_vocab);
 int lstk_sample(const float *d_logits, int64_t ld_logits, int n_rows, int n_vocab, const lstk_sampling *how, const float *d_u,
                 int32_t *d_tokens, float *d_probs, void *d_work, size_t work_bytes, lstk_stream_t stream);
 
+/* A cache whose K and V are held in 8 bits: blocks of 32 dims of a cell with a scale each (8.5 bits a value, as Q8_0). d is the
+ * smallest fp16 number that is no less than a block's largest magnitude over 127, q = value / d to the nearest whole number (halves to
+ * the even one), and what the cache holds is d q: no value is off by more than d / 2. A block with a NaN, an infinity or a magnitude
+ * above 127 * 65504 holds NaN.
+ * d_pages is [n_pages][n_head_kv] records of 68 head_dim bytes, one for a page (32 cells) and KV head, 16-byte aligned; n_pages is at
+ * most 2^22, head_dim 64, 128 or 256. A record is, one after the other, K's q, int8 [head_dim / 32][4][4][4][2][8], where [m][a][b][c][t][j]
+ * is cell 8 b + 4 t + c, dim 32 m + 8 a + j; K's d, fp16 [head_dim / 32][32 cells]; V's q, int8 [head_dim / 32][4][16][2][8], where
+ * [m][a][r][t][c] is cell 8 a + c, dim 32 m + 16 t + r; V's d, as K's. Scales that a caller writes itself must not be negative. */
+typedef struct lstk_q8_cache {
+    uint8_t *d_pages;
+    int64_t n_pages;
+    int32_t n_head_kv, head_dim;
+    const int32_t *d_cell_seq; /* [32 n_pages] or NULL; read by attention, as lstk_paged_cache's */
+} lstk_q8_cache;
+/* store: quantises n_rows (at most 2^24) rows of K and V, [n_rows][n_head_kv][head_dim] of type LSTK_TYPE_F16 or LSTK_TYPE_F32, as they
+ * are written to the cells d_cells [n_rows]. load: reads the rows of these cells back, rounded to fp16, or exact in f32. Row r is at
+ * d_k + r * ld_k and d_v + r * ld_v (in values; multiples of 8; pointers 16-byte aligned). A cell outside the cache is left alone by
+ * store, its row zeros in load. The cells of one store must differ: a cell that several rows name holds bytes of more than one of
+ * them afterwards. Other cells keep every bit. */
+int lstk_cache_q8_store(const lstk_q8_cache *cache, const void *d_k, const void *d_v, int type, int64_t ld_k, int64_t ld_v,
+                        const int32_t *d_cells, int n_rows, lstk_stream_t stream);
+int lstk_cache_q8_load(const lstk_q8_cache *cache, void *d_k, void *d_v, int type, int64_t ld_k, int64_t ld_v, const int32_t *d_cells,
+                       int n_rows, lstk_stream_t stream);
+/* lstk_attn_paged over such a cache: the result of the values d q, with the same rules for lengths, pages, windows, owners and the
+ * workspace. A weight enters its sums times a scale of V, as two fp16 parts. */
+size_t lstk_attn_paged_q8_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink);
+int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head, int window, int n_sink,
+                       float scale, uint16_t *d_out, void *d_work, size_t work_bytes, lstk_stream_t stream);
+
+/* Attention of one new token per sequence over cells that all sequences see, the prefix (a prompt that many answers go out from), and
+ * the sequence's own cells behind it, as one softmax: what lstk_attn_paged gives where every row's list begins with the same pages
+ * (whole ones), but the prefix is read once for all rows. The prefix is the first *d_len cells (held in [0, max_len]) of the pages
+ * d_blocks [n_table] of an fp16 cache; pages out of range are not visible. seqs describes the sequences' own cells, in an fp16 cache
+ * (the same or another one) or a quantised one, by the rules of lstk_attn_paged without a window; prefix->cache->d_cell_seq must be NULL.
+ * A row without a visible cell gets zeros. Over the prefix a weight is rounded to one fp16 part, good to 2^-11 (to 2^-37 of the
+ * largest where it is below 2^-26 of it); sums are fp32. */
+typedef struct lstk_prefix {
+    const lstk_paged_cache *cache;
+    int32_t max_len;         /* bound of the length: sizes the launch and the workspace */
+    const int32_t *d_len;    /* one number */
+    const int32_t *d_blocks; /* [n_table] block numbers */
+    int32_t n_table;
+} lstk_prefix;
+size_t lstk_attn_shared_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int max_prefix);
+int lstk_attn_shared(const lstk_prefix *prefix, const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head,
+                     float scale, uint16_t *d_out, void *d_work, size_t work_bytes, lstk_stream_t stream);
+int lstk_attn_shared_q8(const lstk_prefix *prefix, const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head,
+                        float scale, uint16_t *d_out, void *d_work, size_t work_bytes, lstk_stream_t stream);
+
+/* For each row of logits (as lstk_sample's: NaN counts as -inf, +inf as the largest float): d_logprobs [n_rows], the natural logarithm of
+ * the probability that softmax gives d_tokens[r]; d_entropy [n_rows] (or NULL), -sum p ln p; and the n_top (at most 32) largest values'
+ * ids and log probabilities, d_top_ids and d_top_logprobs [n_rows][n_top], in descending order, equal ones by id. A token outside the
+ * vocabulary, or one at -inf, has -inf; a row with fewer than n_top values above -inf has id -1 and -inf in the other places, one with
+ * none of them entropy 0. n_vocab is at most 2^20 - 16; the workspace is as lstk_attn_paged's. */
+size_t lstk_token_logprobs_work_bytes(int n_rows, int n_vocab, int n_top);
+int lstk_token_logprobs(const float *d_logits, int64_t ld_logits, int n_rows, int n_vocab, const int32_t *d_tokens, int n_top,
+                        float *d_logprobs, float *d_entropy, int32_t *d_top_ids, float *d_top_logprobs, void *d_work, size_t work_bytes,
+                        lstk_stream_t stream);
+
 /* KvCache::remove_seq / truncate_seq / length (src/kv_cache.cpp:97-150, src/engine.h:75-80). */
 int lstk_model_remove_seq(lstk_model *model, int32_t seq);
 int lstk_model_truncate_seq(lstk_model *model, int32_t seq, int32_t keep);

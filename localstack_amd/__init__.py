@@ -12,7 +12,9 @@ ctypes view of that ABI that mirrors the reference's interface for the path:
                        (src/engine.cpp:250-278) over qwen3_build_graph (src/qwen3.cpp:223-259)
                        with the KvCache block table (src/kv_cache.cpp:59-150); decode_batch and generate
                        step many sequences at once
-  paged_attention, sample, moe_select   the operators of such a step on plain tensors
+  paged_attention, sample, moe_select   the operators of such a step on plain tensors; beside them
+                       store_q8, load_q8, paged_attention_q8 (a cache in 8 bits), shared_attention,
+                       shared_attention_q8 (a prefix that the sequences share) and token_logprobs
 
 Device buffers are torch tensors on a ROCm device (or raw integer device pointers); torch is used
 only to own device memory and streams. There is no CPU fallback: every compute call runs the HIP
@@ -94,6 +96,16 @@ class PagedSeqs(ctypes.Structure):
                 ("d_seq", ctypes.c_void_p)]
 
 
+class Q8Cache(ctypes.Structure):
+    _fields_ = [("d_pages", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("n_head_kv", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("d_cell_seq", ctypes.c_void_p)]
+
+
+class Prefix(ctypes.Structure):
+    _fields_ = [("cache", ctypes.POINTER(PagedCache)), ("max_len", ctypes.c_int32), ("d_len", ctypes.c_void_p),
+                ("d_blocks", ctypes.c_void_p), ("n_table", ctypes.c_int32)]
+
+
 class Sampling(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("d_temperature", "d_top_k", "d_top_p", "d_min_p")]
 
@@ -162,6 +174,17 @@ SIGNATURES = {
                              _P]),
     "lstk_sample_work_bytes": (_SZ, [_I, _I]),
     "lstk_sample": (_I, [_P, ctypes.c_int64, _I, _I, ctypes.POINTER(Sampling), _P, _P, _P, _P, _SZ, _P]),
+    "lstk_cache_q8_store": (_I, [ctypes.POINTER(Q8Cache), _P, _P, _I, ctypes.c_int64, ctypes.c_int64, _P, _I, _P]),
+    "lstk_cache_q8_load": (_I, [ctypes.POINTER(Q8Cache), _P, _P, _I, ctypes.c_int64, ctypes.c_int64, _P, _I, _P]),
+    "lstk_attn_paged_q8_work_bytes": (_SZ, [_I] * 7),
+    "lstk_attn_paged_q8": (_I, [ctypes.POINTER(Q8Cache), ctypes.POINTER(PagedSeqs), _P, _I, _I, _I, ctypes.c_float, _P, _P, _SZ, _P]),
+    "lstk_attn_shared_work_bytes": (_SZ, [_I] * 6),
+    "lstk_attn_shared": (_I, [ctypes.POINTER(Prefix), ctypes.POINTER(PagedCache), ctypes.POINTER(PagedSeqs), _P, _I, ctypes.c_float, _P,
+                              _P, _SZ, _P]),
+    "lstk_attn_shared_q8": (_I, [ctypes.POINTER(Prefix), ctypes.POINTER(Q8Cache), ctypes.POINTER(PagedSeqs), _P, _I, ctypes.c_float, _P,
+                                 _P, _SZ, _P]),
+    "lstk_token_logprobs_work_bytes": (_SZ, [_I] * 3),
+    "lstk_token_logprobs": (_I, [_P, ctypes.c_int64, _I, _I, _P, _I, _P, _P, _P, _P, _P, _SZ, _P]),
     "lstk_model_decode_batch": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
     "lstk_model_prepare_batch": (_I, [_P, _I, _P, _P, ctypes.POINTER(ctypes.c_int32), _P]),
     "lstk_model_forward_batch": (_I, [_P, _I, ctypes.c_int32, _I, _I, _P, _P, _P]),
@@ -518,6 +541,233 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     wt, wp, wn = _work(work, lib().lstk_sample_work_bytes(n, V) if work is None else 0, dev, stream)
     _check(_on_device(dev, stream, lambda st: lib().lstk_sample(p, ld, n, V, ctypes.byref(how), up, tp, pp, wp, wn, st)))
     return tokens, probs
+
+
+def q8_cache_shape(n_cells, n_head_kv, head_dim):
+    """Shape of the uint8 tensor that holds n_cells cells (rounded up to whole pages of 32) of K and V in 8 bits (lstk_q8_cache,
+    include/lstk_qwen3.h)."""
+    return -(-int(n_cells) // 32), int(n_head_kv), 68 * int(head_dim)
+
+
+def _q8(cache, dev=None, cell_seq=None):
+    """(Q8Cache, device) of a cache tensor; its head size is the last dimension's over 68."""
+    import torch
+    p = _tensor(cache, "cache", torch.uint8, (None, None, None), dev)
+    dev = cache.get_device()
+    pages, kv, record = cache.shape
+    if record % 68:
+        raise LstkError(E_INVALID, f"cache must be a uint8 tensor of q8_cache_shape(), got {tuple(cache.shape)}")
+    if kv > _MOST or record > _MOST:
+        _check_i32(n_head_kv=kv, head_dim=record // 68)
+    return Q8Cache(p, pages, kv, record // 68,
+                   None if cell_seq is None else _tensor(cell_seq, "cell_seq", torch.int32, (32 * pages,), dev)), dev
+
+
+def _cache_rows(t, name, n, kv, hd, dtype, dev):
+    """(pointer, values between rows) of rows [n][kv][hd] whose heads and dims are contiguous."""
+    try:
+        shape, stride, on = tuple(t.shape), t.stride(), t.get_device()
+    except AttributeError:
+        raise LstkError(E_INVALID, f"{name} must be a tensor, got {type(t)}") from None
+    if t.dtype is not dtype or shape != (n, kv, hd) or (n and ((kv > 1 and stride[1] != hd) or stride[2] != 1)):
+        raise LstkError(E_INVALID, f"{name} must be a {dtype} tensor of shape {n}x{kv}x{hd} whose rows are contiguous, got {t.dtype} "
+                                   f"{shape} of strides {stride}")
+    if on != dev:
+        raise LstkError(E_INVALID, f"{name} is on {t.device}, not on GPU {dev}")
+    return t.data_ptr(), stride[0] if n > 1 else kv * hd
+
+
+def _rows_type(dtype):
+    import torch
+    if dtype is torch.float16:
+        return TYPE_F16
+    if dtype is torch.float32:
+        return TYPE_F32
+    raise LstkError(E_INVALID, f"rows must be float16 or float32, not {dtype}")
+
+
+def store_q8(cache, k, v, cells, stream=None):
+    """Quantises rows of K and V (fp16 or f32 [n][n_head_kv][head_dim], rows may be strided) as they are written to the cells (int32
+    [n], all different; one outside the cache is left alone) of a cache tensor of q8_cache_shape(): lstk_cache_q8_store."""
+    import torch
+    c, dev = _q8(cache)
+    at = _tensor(cells, "cells", torch.int32, (None,), dev)
+    n = cells.shape[0]
+    if n > _MOST:
+        _check_i32(n_rows=n)
+    dtype = getattr(k, "dtype", None)
+    kind = _rows_type(dtype)
+    kp, ldk = _cache_rows(k, "k", n, c.n_head_kv, c.head_dim, dtype, dev)
+    vp, ldv = _cache_rows(v, "v", n, c.n_head_kv, c.head_dim, dtype, dev)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_cache_q8_store(ctypes.byref(c), kp, vp, kind, ldk, ldv, at, n, st)))
+
+
+def load_q8(cache, cells, dtype=None, k=None, v=None, stream=None):
+    """The rows of these cells (int32 [n]; zeros for one outside the cache) as (k, v), each [n][n_head_kv][head_dim] of `dtype`
+    (float16, or float32, which is exact): lstk_cache_q8_load. k, v: where they go, rows may be strided."""
+    import torch
+    c, dev = _q8(cache)
+    at = _tensor(cells, "cells", torch.int32, (None,), dev)
+    n = cells.shape[0]
+    if n > _MOST:
+        _check_i32(n_rows=n)
+    if dtype is None:
+        dtype = torch.float16 if k is None else getattr(k, "dtype", None)
+    kind = _rows_type(dtype)
+    shape = (n, c.n_head_kv, c.head_dim)
+    if k is None:
+        k = _empty(shape, dtype, dev, stream)
+    if v is None:
+        v = _empty(shape, dtype, dev, stream)
+    kp, ldk = _cache_rows(k, "k", *shape, dtype, dev)
+    vp, ldv = _cache_rows(v, "v", *shape, dtype, dev)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_cache_q8_load(ctypes.byref(c), kp, vp, kind, ldk, ldv, at, n, st)))
+    return k, v
+
+
+def _own_seqs(n, lens, first, blocks, max_len, seqs, dev):
+    import torch
+    i32 = torch.int32
+    table = _tensor(blocks, "blocks", i32, (None,), dev)
+    max_len = int(max_len)
+    if not (0 <= max_len <= _MOST and blocks.numel() <= _MOST):
+        _check_i32(max_len=max_len, n_table=blocks.numel())
+    return PagedSeqs(n, max_len, _tensor(lens, "lens", i32, (n,), dev), _tensor(first, "first", i32, (n,), dev), table, blocks.numel(),
+                     None if seqs is None else _tensor(seqs, "seqs", i32, (n,), dev))
+
+
+def paged_attention_q8_work_bytes(n_seq, n_head, n_head_kv, head_dim, max_len, window=0, n_sink=0):
+    return lib().lstk_attn_paged_q8_work_bytes(_i32(n_seq, "n_seq"), _i32(n_head, "n_head"), _i32(n_head_kv, "n_head_kv"),
+                                               _i32(head_dim, "head_dim"), _i32(max_len, "max_len"), _i32(window, "window"),
+                                               _i32(n_sink, "n_sink"))
+
+
+def paged_attention_q8(q, cache, lens, first, blocks, max_len, window=0, n_sink=0, scale=None, cell_seq=None, seqs=None, out=None,
+                       work=None, stream=None):
+    """paged_attention over a cache in 8 bits (uint8, q8_cache_shape()): lstk_attn_paged_q8, include/lstk_qwen3.h. The other arguments are
+    paged_attention's."""
+    import torch
+    qp = _tensor(q, "q", torch.float16, (None, None, None))
+    n, H, hd = shape = q.shape
+    c, dev = _q8(cache, q.get_device(), cell_seq)
+    if c.head_dim != hd:
+        raise LstkError(E_INVALID, f"the cache is of head size {c.head_dim}, q of {hd}")
+    window, n_sink = int(window), int(n_sink)
+    if not (0 <= window <= _MOST and 0 <= n_sink <= _MOST):
+        _check_i32(window=window, n_sink=n_sink)
+    s = _own_seqs(n, lens, first, blocks, max_len, seqs, dev)
+    if out is None:
+        out = _empty(shape, torch.float16, dev, stream)
+    op = _tensor(out, "out", torch.float16, shape, dev)
+    need = 0 if work is not None else lib().lstk_attn_paged_q8_work_bytes(n, H, c.n_head_kv, hd, s.max_len, window, n_sink)
+    wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
+    f = float(hd ** -0.5 if scale is None else scale)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_attn_paged_q8(ctypes.byref(c), ctypes.byref(s), qp, H, window, n_sink, f, op, wp,
+                                                                       wn, st)))
+    return out
+
+
+class SharedPrefix:
+    """Cells that all sequences of a call see (lstk_prefix, include/lstk_qwen3.h): the first `length` (int32 [1] on the device) cells of the
+    pages `blocks` (int32) of an fp16 cache in paged_attention's layouts. max_len bounds the length. The tensors are looked at here, once,
+    and held."""
+
+    def __init__(self, k_cache, v_cache, length, blocks, max_len):
+        import torch
+        i32, f16 = torch.int32, torch.float16
+        kp = _tensor(k_cache, "k_cache", f16, (None, None, None, 4))
+        self.device = dev = k_cache.get_device()
+        kv, quads, size, _ = k_cache.shape
+        self._held = (k_cache, v_cache, length, blocks)
+        self.cache = PagedCache(kp, _tensor(v_cache, "v_cache", f16, (kv, size // 4, 4 * quads, 4), dev), size, kv, 4 * quads, None)
+        table = _tensor(blocks, "blocks", i32, (None,), dev)
+        self.c = Prefix(ctypes.pointer(self.cache), _i32(max_len, "max_len"), _tensor(length, "length", i32, (1,), dev), table,
+                        _i32(blocks.numel(), "n_table"))
+
+
+def shared_attention_work_bytes(n_seq, n_head, n_head_kv, head_dim, max_len, max_prefix):
+    return lib().lstk_attn_shared_work_bytes(_i32(n_seq, "n_seq"), _i32(n_head, "n_head"), _i32(n_head_kv, "n_head_kv"),
+                                             _i32(head_dim, "head_dim"), _i32(max_len, "max_len"), _i32(max_prefix, "max_prefix"))
+
+
+def _shared(call, q, qp, prefix, cache, s, scale, out, work, stream):
+    import torch
+    if not isinstance(prefix, SharedPrefix):
+        raise LstkError(E_INVALID, f"prefix must be a SharedPrefix, got {type(prefix)}")
+    n, H, hd = shape = q.shape
+    dev = q.get_device()
+    if prefix.device != dev:
+        raise LstkError(E_INVALID, f"the prefix is on GPU {prefix.device}, q on GPU {dev}")
+    if out is None:
+        out = _empty(shape, torch.float16, dev, stream)
+    op = _tensor(out, "out", torch.float16, shape, dev)
+    need = 0 if work is not None else lib().lstk_attn_shared_work_bytes(n, H, cache.n_head_kv, hd, s.max_len, prefix.c.max_len)
+    wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
+    f = float(hd ** -0.5 if scale is None else scale)
+    _check(_on_device(dev, stream, lambda st: call(ctypes.byref(prefix.c), ctypes.byref(cache), ctypes.byref(s), qp, H, f, op, wp, wn, st)))
+    return out
+
+
+def shared_attention(q, prefix, k_cache, v_cache, lens, first, blocks, max_len, scale=None, cell_seq=None, seqs=None, out=None, work=None,
+                     stream=None):
+    """Attention of one new token per sequence over a SharedPrefix and, behind it, the sequence's own cells (the other arguments are
+    paged_attention's; a length may be 0): lstk_attn_shared, include/lstk_qwen3.h. The prefix is read once for all sequences."""
+    import torch
+    f16 = torch.float16
+    qp = _tensor(q, "q", f16, (None, None, None))
+    n, H, hd = q.shape
+    dev = q.get_device()
+    kp = _tensor(k_cache, "k_cache", f16, (None, hd // 4, None, 4), dev)
+    kv, _, size, _ = k_cache.shape
+    cache = PagedCache(kp, _tensor(v_cache, "v_cache", f16, (kv, size // 4, hd, 4), dev), size, kv, hd,
+                       None if cell_seq is None else _tensor(cell_seq, "cell_seq", torch.int32, (size,), dev))
+    return _shared(lib().lstk_attn_shared, q, qp, prefix, cache, _own_seqs(n, lens, first, blocks, max_len, seqs, dev), scale, out, work,
+                   stream)
+
+
+def shared_attention_q8(q, prefix, cache, lens, first, blocks, max_len, scale=None, cell_seq=None, seqs=None, out=None, work=None,
+                        stream=None):
+    """shared_attention with the sequences' own cells in 8 bits (uint8, q8_cache_shape()): lstk_attn_shared_q8."""
+    import torch
+    qp = _tensor(q, "q", torch.float16, (None, None, None))
+    n, H, hd = q.shape
+    c, dev = _q8(cache, q.get_device(), cell_seq)
+    if c.head_dim != hd:
+        raise LstkError(E_INVALID, f"the cache is of head size {c.head_dim}, q of {hd}")
+    return _shared(lib().lstk_attn_shared_q8, q, qp, prefix, c, _own_seqs(n, lens, first, blocks, max_len, seqs, dev), scale, out, work,
+                   stream)
+
+
+def token_logprobs_work_bytes(n_rows, n_vocab, n_top=0):
+    return lib().lstk_token_logprobs_work_bytes(_i32(n_rows, "n_rows"), _i32(n_vocab, "n_vocab"), _i32(n_top, "n_top"))
+
+
+def token_logprobs(logits, tokens, n_top=0, logprobs=None, entropy=None, top_ids=None, top_logprobs=None, work=None, stream=None):
+    """The log probability of tokens[r] (int32 [n]) in row r of logits (f32 [n][n_vocab], rows may be strided), the rows' entropies, and
+    the ids and log probabilities of their n_top largest values: lstk_token_logprobs, include/lstk_qwen3.h. Returns (logprobs f32 [n],
+    entropy f32 [n], top_ids int32 [n][n_top], top_logprobs f32 [n][n_top])."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    p, ld, n, V, dev = _rows(logits, "logits", f32)
+    n_top = int(n_top)
+    if not (n <= _MOST and V <= _MOST and 0 <= n_top <= _MOST):
+        _check_i32(n_rows=n, n_vocab=V, n_top=n_top)
+    tp = _tensor(tokens, "tokens", i32, (n,), dev)
+    shape, tops = (n,), (n, max(n_top, 0))
+    if logprobs is None:
+        logprobs = _empty(n, f32, dev, stream)
+    if entropy is None:
+        entropy = _empty(n, f32, dev, stream)
+    if top_ids is None:
+        top_ids = _empty(tops, i32, dev, stream)
+    if top_logprobs is None:
+        top_logprobs = _empty(tops, f32, dev, stream)
+    lp, ep = _tensor(logprobs, "logprobs", f32, shape, dev), _tensor(entropy, "entropy", f32, shape, dev)
+    ip, ap = _tensor(top_ids, "top_ids", i32, tops, dev), _tensor(top_logprobs, "top_logprobs", f32, tops, dev)
+    need = 0 if work is not None else lib().lstk_token_logprobs_work_bytes(n, V, n_top)
+    wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
+    _check(_on_device(dev, stream, lambda st: lib().lstk_token_logprobs(p, ld, n, V, tp, n_top, lp, ep, ip, ap, wp, wn, st)))
+    return logprobs, entropy, top_ids, top_logprobs
 
 
 _stores = weakref.WeakSet()  # stores not yet freed

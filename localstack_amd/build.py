@@ -3,8 +3,9 @@
 The library is the product: the MoE kernels (csrc/kernels.hip, grouped.hip, fused.hip), the HBM
 expert pool and the MoE C ABI (csrc/pool.cpp, include/lstk_moe.h), the host repacker
 (csrc/repack.cpp), the forward pass around the MoE block (csrc/forward.hip, csrc/model.cpp,
-include/lstk_qwen3.h), the operators of a step over many sequences (csrc/paged_attn.hip, sample.hip,
-select.hip, batch.cpp) and the GGUF reader (csrc/gguf.cpp, include/lstk_gguf.h).
+include/lstk_qwen3.h), the operators of a step over many sequences (csrc/paged_attn.hip, paged_attn_q8.hip,
+prefix_attn.hip, cache_q8.hip, sample.hip, logp.hip, select.hip, batch.cpp) and the GGUF reader
+(csrc/gguf.cpp, include/lstk_gguf.h).
 """
 import os
 import shutil
@@ -15,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblstk_moe.so")
-SOURCES = ["kernels.hip", "grouped.hip", "grouped_rows.hip", "fused.hip", "forward.hip", "paged_attn.hip", "sample.hip", "select.hip", "pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp", "tier.hip", "batch.cpp"]
+SOURCES = ["kernels.hip", "grouped.hip", "grouped_rows.hip", "fused.hip", "forward.hip", "paged_attn.hip", "paged_attn_q8.hip", "prefix_attn.hip", "cache_q8.hip", "sample.hip", "logp.hip", "select.hip", "pool.cpp", "repack.cpp", "model.cpp", "gguf.cpp", "tier.hip", "batch.cpp"]
 ARCH = os.environ.get("LSTK_OFFLOAD_ARCH", "gfx950")
 
 
@@ -29,7 +30,7 @@ def hipcc():
 # Per-source extra flags. The MFMA kernels keep their accumulators in VGPRs (the VALU epilogue and the
 # attention's rescale then read them without v_accvgpr_read moves). In forward.hip only the attention
 # kernels change by it: fewer instructions at the same registers, steps of 1 to 63 tokens 1% faster.
-EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for s in ("grouped.hip", "grouped_rows.hip", "forward.hip", "paged_attn.hip")}
+EXTRA = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for s in ("grouped.hip", "grouped_rows.hip", "forward.hip", "paged_attn.hip", "paged_attn_q8.hip", "prefix_attn.hip")}
 COMMON = ["-O3", "-std=c++20", "-fPIC",
           # packed-FP32 instructions off for all device code
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -32,13 +32,66 @@ struct PagedAttnParams {
     PagedAttnSplit *split; // [n_seq][n_kv * n_rowblk], a task each
     float *part;           // [n_wg][2][min(16, heads per KV head)][hd + 4]: max, sum, 2 unused, unnormalised output of a part of a task
     uint16_t *out;         // [n_seq][n_head][hd] fp16
+    const uint8_t *q8 = nullptr;  // in place of kc and vc: the records of a quantised cache (cache_q8.h), kv_size / 32 pages
+    const float *pre = nullptr;   // [n_pre][n_seq][n_head][hd + 4]: what parts of a prefix left, in the form of `part`
+    int n_pre = 0;
 };
 // Fills n_rowblk and n_wg; returns the bytes of workspace (16-byte aligned) that calls of these shapes with this max_len or a
 // smaller one take (0 where every task has a work-group), which paged_attn_work points at.
 size_t paged_attn_plan(PagedAttnParams &P);
 void paged_attn_work(PagedAttnParams &P, void *work);
 hipError_t launch_paged_attn(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm);
+hipError_t launch_paged_attn_q8(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm);
 hipError_t launch_paged_attn_join(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm);
+
+// Attention of the query tokens of all sequences over one list of pages that they share: what each of n_chunk shares of the list
+// leaves, [n_chunk][n_seq * n_head][hd + 4] (max, sum, 2 unused, unnormalised output), for PagedAttnParams::pre.
+struct PrefixAttnParams {
+    const uint16_t *q; // [n_seq][n_head][hd] fp16
+    const uint16_t *kc, *vc;
+    const int32_t *len, *blocks; // len: one number, cells of the prefix
+    int64_t kv_size;
+    int n_seq, n_head, n_kv, hd, n_table, max_len;
+    float scale; // of the scores, times log2(e)
+    int n_chunk, n_rowblk; // prefix_attn_plan
+    bool shared;           // the wavefronts of a work-group share pages; otherwise each takes its own
+    float *part;
+};
+// Fills n_chunk, n_rowblk and shared; returns the bytes of `part` (0: no prefix).
+size_t prefix_attn_plan(PrefixAttnParams &P);
+hipError_t launch_prefix_attn(const PrefixAttnParams &P, hipStream_t st, const LaunchTiming *tm);
+
+// Rows into and out of a quantised cache (cache_q8.hip).
+struct CacheRowsParams {
+    uint8_t *cache;
+    int64_t n_cells; // of the cache
+    int n_kv, hd;
+    const int32_t *cells; // [n] cell of each row; one outside the cache is left alone (read: zeros)
+    int n;
+    bool f32;        // rows are f32, otherwise fp16
+    const void *k, *v; // [n][n_kv][hd], rows ld_k and ld_v values apart; written to when reading back
+    int64_t ld_k, ld_v;
+};
+hipError_t launch_cache_store(const CacheRowsParams &P, hipStream_t st);
+hipError_t launch_cache_load(const CacheRowsParams &P, hipStream_t st);
+
+// Log probabilities of one token per row of logits, entropy and the largest values.
+constexpr int kLogpMaxTop = 32;
+constexpr int kLogpMaxVocab = (1 << 20) - 16; // 64 slices of what a work-group holds
+struct LogpParams {
+    const float *logits;
+    int64_t ld;
+    int n_rows, n_vocab, n_top;
+    const int32_t *tokens;
+    float *logp, *entropy; // entropy may be null
+    int32_t *top_ids;      // [n_rows][n_top]
+    float *top_logp;
+    int slices, slice;     // work-groups per row and values per slice (logp_plan)
+    float *sums;           // [n_rows][slices][4]: max, sum of e^(x - max), sum of (x - max) e^(x - max), unused
+    unsigned long long *best; // [n_rows][slices][n_top] (value, lowest index), largest first
+};
+size_t logp_plan(LogpParams &P, void *work);
+hipError_t launch_logp(const LogpParams &P, hipStream_t st);
 
 // Sampling of one token per row of logits.
 constexpr int kSampleBins = 2048;

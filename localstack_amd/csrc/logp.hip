@@ -1,0 +1,261 @@
+// logp.hip - log probabilities of a given token per row of logits, the row's entropy and its largest values.
+//
+//   m = max x,  l = sum e^(x - m),  t = sum (x - m) e^(x - m)
+//   log p(i) = x_i - m - ln l,  entropy = ln l - t / l
+//
+// A row is read once: a work-group holds a slice of it in registers (kLpThreads * HELD quads), so the maximum is known before the
+// sums are taken, and the largest values can be looked for afterwards. The n-th largest of the threads' own maxima is a bound
+// that the n largest values of the slice reach and few others do; those are gathered in LDS and put in order by counting. A row of
+// several slices is joined by a second launch, a wavefront a row.
+#include <cfloat>
+#include <type_traits>
+
+#include "batch.h"
+#include "device.h"
+
+namespace lstk {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave;
+constexpr int kLpHeld = 16, kLpFew = 4; // quads of a thread
+constexpr int kLpSlices = 64;           // of a row: a lane each in the join
+constexpr int kLpList = 1024;
+constexpr int kLpTarget = 512;          // work-groups of a launch
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kFar = -1000.0f;        // e^kFar is 0: x - m of -inf, so that 0 times it stays 0
+
+__device__ __forceinline__ float counted(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); } // NaN: -inf
+__device__ __forceinline__ unsigned key_of(float x) { // order-preserving
+    const unsigned u = __float_as_uint(x + 0.0f);     // -0 and 0 are equal values
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ u64 place_of(float x, unsigned i) { return (u64) key_of(x) << 32 | (unsigned) ~i; } // larger is earlier; 0: none
+
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ unsigned dpp_u(unsigned v) {
+    return (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+    v = max(v, dpp_u<0xB1>(v));
+    v = max(v, dpp_u<0x4E>(v));
+    v = max(v, dpp_u<0x141>(v));
+    v = max(v, dpp_u<0x140>(v));
+    v = max(v, dpp_u<kDppRowBcast15, 0xA>(v));
+    v = max(v, dpp_u<kDppRowBcast31, 0x8>(v));
+    return (unsigned) __builtin_amdgcn_readlane((int) v, 63);
+}
+__device__ __forceinline__ u64 wave_place_max(u64 p) {
+    const unsigned hi = wave_umax((unsigned) (p >> 32)), lo = wave_umax((unsigned) (p >> 32) == hi ? (unsigned) p : 0u);
+    return (u64) hi << 32 | lo;
+}
+// wave_max gives rows that a DPP step leaves out a 0; here the maxima may be below it
+__device__ __forceinline__ float wave_top(float v) { return of_key(wave_umax(key_of(v))); }
+
+// A row's answers from its sums (m: its largest value).
+__device__ __forceinline__ void answer(const LogpParams &P, int row, float m, double l, double t, double &lse) {
+    lse = m > -INFINITY ? log(l) : 0.0;
+    const float *x = P.logits + (int64_t) row * P.ld;
+    const int token = P.tokens[row];
+    float v = -INFINITY;
+    if (token >= 0 && token < P.n_vocab) v = counted(x[token]);
+    P.logp[row] = v > -INFINITY ? (float) ((double) v - (double) m - lse) : -INFINITY;
+    if (P.entropy) P.entropy[row] = m > -INFINITY ? (float) (lse - t / l) : 0.0f;
+}
+__device__ __forceinline__ void alternative(const LogpParams &P, int row, int r, u64 place, float m, double lse) {
+    const int64_t at = (int64_t) row * P.n_top + r;
+    P.top_ids[at] = place == 0 ? -1 : (int32_t) ~(unsigned) place;
+    P.top_logp[at] = place == 0 ? -INFINITY : (float) ((double) of_key((unsigned) (place >> 32)) - (double) m - lse);
+}
+
+template <int HELD>
+__global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
+    __shared__ float s_max[kLpThreads], s_l[kLpWaves], s_t[kLpWaves];
+    __shared__ unsigned s_bound, s_n;
+    __shared__ u64 s_list[kLpList], s_best[kLogpMaxTop], s_place[kLpWaves];
+    const int row = blockIdx.x / P.slices, slice = blockIdx.x % P.slices, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
+    const float *x = P.logits + (int64_t) row * P.ld;
+    // quads by the memory's alignment: value i of the row is place i + off of them
+    const int off = (int) (reinterpret_cast<uintptr_t>(x) / 4 % 4), quads = (P.n_vocab + off + 3) / 4;
+    const int q0 = slice * P.slice, q1 = min(quads, q0 + P.slice);
+    float v[HELD][4];
+    auto index = [&](int h, int e) { return 4 * (q0 + h * kLpThreads + tid) + e - off; };
+#pragma unroll
+    for (int h = 0; h < HELD; h++) {
+        const int i = index(h, 0);
+        if (q0 + h * kLpThreads + tid < q1 && i >= 0 && i + 4 <= P.n_vocab) {
+            const float4 f = *reinterpret_cast<const float4 *>(x + i);
+            v[h][0] = f.x;
+            v[h][1] = f.y;
+            v[h][2] = f.z;
+            v[h][3] = f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[h][e] = q0 + h * kLpThreads + tid < q1 && i + e >= 0 && i + e < P.n_vocab ? x[i + e] : -INFINITY;
+        }
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < HELD; h++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[h][e] = counted(v[h][e]);
+            most = fmaxf(most, v[h][e]);
+        }
+    s_max[tid] = most;
+    if (tid == 0) s_n = 0;
+    const float wave_most = wave_top(most);
+    if (lane == 0) s_l[wv] = wave_most;
+    __syncthreads();
+    float m = s_l[0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) m = fmaxf(m, s_l[w]);
+    __syncthreads();
+    float l = 0.0f, t = 0.0f;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int h = 0; h < HELD; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float d = fmaxf(v[h][e] - m, kFar), w = __builtin_amdgcn_exp2f(d * kLog2e);
+                l += w;
+                t = fmaf(d, w, t);
+            }
+    }
+    l = wave_sum_tree(l);
+    t = wave_sum_tree(t);
+    if (lane == 0) {
+        s_l[wv] = l;
+        s_t[wv] = t;
+    }
+    if (P.n_top > 0 && wv == 0) {
+        // the n-th largest of the threads' maxima, bit by bit
+        unsigned key[kLpWaves], bound = 0;
+#pragma unroll
+        for (int w = 0; w < kLpWaves; w++) key[w] = key_of(s_max[w * kWave + lane]);
+        for (int bit = 31; bit >= 0; bit--) {
+            const unsigned c = bound | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < kLpWaves; w++) n += __popcll(__ballot(key[w] >= c));
+            if (n >= P.n_top) bound = c;
+        }
+        if (lane == 0) s_bound = bound;
+    }
+    __syncthreads();
+    double L = 0.0, T = 0.0;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; w++) {
+        L += s_l[w];
+        T += s_t[w];
+    }
+    const int64_t part = (int64_t) row * P.slices + slice;
+    double lse = 0.0;
+    if (tid == 0) {
+        if (P.slices > 1) *reinterpret_cast<float4 *>(P.sums + 4 * part) = make_float4(m, (float) L, (float) T, 0.0f);
+        else answer(P, row, m, L, T, lse);
+    }
+    if (P.n_top == 0) return;
+    const float bound = of_key(s_bound);
+#pragma unroll
+    for (int h = 0; h < HELD; h++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (v[h][e] >= bound && v[h][e] > -INFINITY) {
+                const unsigned at = atomicAdd(&s_n, 1u);
+                if (at < (unsigned) kLpList) s_list[at] = place_of(v[h][e], (unsigned) index(h, e));
+            }
+    if (tid < P.n_top) s_best[tid] = 0;
+    __syncthreads();
+    const int n = (int) s_n;
+    if (n <= kLpList) {
+        for (int i = tid; i < n; i += kLpThreads) {
+            const u64 mine = s_list[i];
+            int before = 0;
+            for (int j = 0; j < n; j++) before += s_list[j] > mine;
+            if (before < P.n_top) s_best[before] = mine;
+        }
+    } else {
+        // many values alike: one after the other
+        u64 last = ~0ull;
+        for (int r = 0; r < P.n_top; r++) {
+            u64 top = 0;
+#pragma unroll
+            for (int h = 0; h < HELD; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const u64 p = place_of(v[h][e], (unsigned) index(h, e));
+                    if (v[h][e] > -INFINITY && p < last && p > top) top = p;
+                }
+            top = wave_place_max(top);
+            if (lane == 0) s_place[wv] = top;
+            __syncthreads();
+            last = 0;
+#pragma unroll
+            for (int w = 0; w < kLpWaves; w++) last = max(last, s_place[w]);
+            if (tid == 0) s_best[r] = last;
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    if (tid >= P.n_top) return;
+    if (P.slices > 1) P.best[part * P.n_top + tid] = s_best[tid];
+    else alternative(P, row, tid, s_best[tid], m, m > -INFINITY ? log(L) : 0.0);
+}
+
+__global__ __launch_bounds__(kWave) void logp_join_kernel(LogpParams P) {
+    const int row = blockIdx.x, lane = threadIdx.x;
+    const int64_t part = (int64_t) row * P.slices + lane;
+    float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    if (lane < P.slices) s = *reinterpret_cast<const float4 *>(P.sums + 4 * part);
+    const float m = wave_top(s.x);
+    double l = 0.0, t = 0.0;
+    if (s.x > -INFINITY) {
+        const double d = (double) s.x - (double) m, w = exp(d);
+        l = w * s.y;
+        t = w * s.z + d * l;
+    }
+    l = wave_sum_d(l);
+    t = wave_sum_d(t);
+    double lse = m > -INFINITY ? log(l) : 0.0;
+    if (lane == 0) answer(P, row, m, l, t, lse);
+    // the largest of the slices' next ones, one after the other
+    int at = 0;
+    u64 head = lane < P.slices && P.n_top > 0 ? P.best[part * P.n_top] : 0;
+    for (int r = 0; r < P.n_top; r++) {
+        const u64 top = wave_place_max(head);
+        if (lane == 0) alternative(P, row, r, top, m, lse);
+        if (head == top && top != 0) {
+            at++;
+            head = at < P.n_top ? P.best[part * P.n_top + at] : 0;
+        }
+    }
+}
+
+}  // namespace
+
+size_t logp_plan(LogpParams &P, void *work) {
+    const int quads = (P.n_vocab + 6) / 4; // a row out of line has one more
+    const int least = (quads + kLpHeld * kLpThreads - 1) / (kLpHeld * kLpThreads);
+    const int want = std::min(kLpTarget / std::max(1, P.n_rows), quads / (kLpFew * kLpThreads));
+    P.slices = std::min(kLpSlices, std::max({1, least, want}));
+    P.slice = (quads + P.slices - 1) / P.slices;
+    if (P.slices == 1) return 0;
+    const size_t parts = (size_t) P.n_rows * P.slices;
+    P.sums = static_cast<float *>(work);
+    P.best = reinterpret_cast<unsigned long long *>(static_cast<uint8_t *>(work) + parts * 16);
+    return parts * (16 + 8 * (size_t) P.n_top);
+}
+
+hipError_t launch_logp(const LogpParams &P, hipStream_t st) {
+    if (P.n_rows <= 0) return hipSuccess;
+    const dim3 all((unsigned) (P.n_rows * P.slices)), block(kLpThreads);
+    const hipError_t e = P.slice <= kLpFew * kLpThreads ? launch(logp_slice_kernel<kLpFew>, all, block, 0, st, nullptr, P)
+                                                        : launch(logp_slice_kernel<kLpHeld>, all, block, 0, st, nullptr, P);
+    if (e != hipSuccess || P.slices == 1) return e;
+    return launch(logp_join_kernel, dim3((unsigned) P.n_rows), dim3(kWave), 0, st, nullptr, P);
+}
+
+}  // namespace lstk

@@ -19,155 +19,13 @@
 // load feeds the tile of the even and that of the odd cells, and the two results leave a lane with 8 consecutive cells of one
 // query head, which is its share of the second product's operand P. Nothing goes through LDS between the products. V
 // likewise: 4 cells of two neighbouring dims.
-#include "batch.h"
-#include "device.h"
+#include "paged_parts.h"
 
 namespace lstk {
 namespace {
 
-typedef _Float16 half8v __attribute__((ext_vector_type(8)));
-typedef float float4v __attribute__((ext_vector_type(4)));
-
-constexpr int kPaWaves = 4;
-constexpr int kPaCus = 256; // of MI355X
-constexpr int kPaPerCu = 2; // work-groups of equal shares per CU
-constexpr int kPaLeast = 4; // pages of a share
-constexpr int kPaRound = 4;  // rounds of the wavefronts up to which a share is made a whole number of them
-constexpr float kLowest = -3.0e38f; // a running maximum that any score replaces
-// The running maximum m that is kept lies 15 below the largest score, so that weights reach 2^15 and fp16 holds those down to
-// 2^-29 of the largest as normal numbers. Scores so large that the difference would be rounded by more than 2^-4 stay as they
-// are (a weight of 2^16 would be an infinity).
-constexpr float kBelow = 15.0f, kExactTo = 0x1p20f;
-__device__ __forceinline__ float maximum_kept(float top) { return fabsf(top) < kExactTo ? top - kBelow : top; }
-
-// The pages of a sequence that hold visible cells: [0, ps) and [pw, pw + count - ps).
-struct Span {
-    int n, lo, sink; // cells; first cell of the window; sink cells
-    int ps, pw, count;
-};
-// Pages of n cells; n may be the largest 32-bit number.
-__device__ __forceinline__ int pages_of(int n) { return n / kPageCells + (n % kPageCells != 0); }
-// Pages that a sequence has in the list: one at least, so that one without any is written (zeros) like the others.
-__device__ __forceinline__ int listed(const Span &s) { return max(1, s.count); }
-__device__ __forceinline__ Span span_of(const PagedAttnParams &P, int len) {
-    Span s;
-    s.n = max(0, min(len, P.max_len));
-    s.lo = P.window > 0 && s.n > P.window ? s.n - P.window : 0;
-    s.sink = min(P.n_sink, s.lo);
-    s.pw = s.lo / kPageCells;
-    s.ps = min(pages_of(s.sink), s.pw);
-    s.count = s.ps + pages_of(s.n) - s.pw;
-    return s;
-}
-
-// The cells of a page that are visible, bit i for cell i0 + i.
-__device__ __forceinline__ unsigned bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
-__device__ __forceinline__ unsigned visible_cells(const Span &s, int i0) {
-    return bits_below(s.n - i0) & (~bits_below(s.lo - i0) | bits_below(s.sink - i0));
-}
-
-// K and V are read once a call, with the non-temporal hint: 128 sequences (1.2 GB) 225 us without it, 205 with it on one of the
-// two, 200 on both; two of 100000 cells 89, 82 and 79.
-__device__ __forceinline__ uint4 read_once(const char *p) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
-    return make_uint4(v.x, v.y, v.z, v.w);
-}
-__device__ __forceinline__ half8v halves(unsigned a, unsigned b, unsigned c, unsigned d) {
-    return __builtin_bit_cast(half8v, make_uint4(a, b, c, d));
-}
-__device__ __forceinline__ float4v mfma(const half8v &a, const half8v &b, const float4v &c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ float across_groups_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, kWave));
-    return fmaxf(v, __shfl_xor(v, 32, kWave));
-}
-__device__ __forceinline__ float across_groups_sum(float v) {
-    v += __shfl_xor(v, 16, kWave);
-    return v + __shfl_xor(v, 32, kWave);
-}
-
-// A value that all lanes have alike, kept in scalar registers.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-    const unsigned lo = __builtin_amdgcn_readfirstlane((int) v), hi = __builtin_amdgcn_readfirstlane((int) (v >> 32));
-    return (int64_t) ((uint64_t) hi << 32 | lo);
-}
-
-// The share of a work-group in the list: `left` pages from page j of task `task` of sequence b on. The sequences' lengths and
-// first table entries stay in LDS where they fit, so that the way to the first page is one wait for them and not three.
-constexpr int kPaKept = kPaWaves * kWave;
-struct Share {
-    int b, task, j;
-    int64_t left, each, total; // each: pages of a full share; total: of the list
-};
-struct Kept {
-    int len[kPaKept], first[kPaKept];
-};
-__device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, Kept &K) {
-    __shared__ int64_t s_sum[kPaWaves], s_before;
-    __shared__ int s_b;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
-    int64_t sum = 0;
-    int mine = 0; // pages of sequence tid, and of the last one of every kPaKept
-    for (int b = tid; b < P.n_seq; b += kPaKept) {
-        const int len = P.len[b];
-        if (P.n_seq <= kPaKept) {
-            K.len[tid] = len;
-            K.first[tid] = P.first[b];
-        }
-        mine = listed(span_of(P, len));
-        sum += mine;
-    }
-    for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d, kWave);
-    if (lane == 0) s_sum[wv] = sum;
-    __syncthreads();
-    Share s;
-    s.total = 0;
-    for (int w = 0; w < kPaWaves; w++) s.total += s_sum[w];
-    s.total = uniform(s.total * tasks);
-    // Small shares are whole rounds of the wavefronts, so that few sequences have fewer parts to join. Us a call so and without, with
-    // room for 131072 cells: one sequence of 5000 cells 14.1 and 15.9, four of 200 to 3000 at 64 heads on 4 13.8 and 15.8; but 24
-    // of 100 to 1500 18.4 and 16.8, 24 of 45 to 500 at 16 on 2 of 256 17.1 and 14.5; larger calls differ by 2% or less.
-    s.each = (s.total + gridDim.x - 1) / gridDim.x;
-    if (s.each <= kPaRound * kPaWaves) s.each = (s.each + kPaWaves - 1) / kPaWaves * kPaWaves;
-    const int64_t lo = s.each * blockIdx.x;
-    s.each = uniform(s.each);
-    s.left = uniform(min(s.each, s.total - lo));
-    if (s.left <= 0) return s;
-    // the sequence that page `lo` of the list is of
-    int64_t before = 0; // of the sequences so far
-    for (int b0 = 0; b0 < P.n_seq; b0 += kPaKept) {
-        const int b = b0 + tid;
-        if (P.n_seq > kPaKept) mine = b < P.n_seq ? listed(span_of(P, P.len[b])) : 0;
-        int64_t upto = mine;
-        for (int d = 1; d < kWave; d *= 2) {
-            const int64_t o = __shfl_up(upto, d, kWave);
-            if (lane >= d) upto += o;
-        }
-        __syncthreads();
-        if (lane == kWave - 1) s_sum[wv] = upto;
-        __syncthreads();
-        upto += before;
-        for (int i = 0; i < wv; i++) upto += s_sum[i];
-        if ((upto - mine) * tasks <= lo && lo < upto * tasks) {
-            s_b = b;
-            s_before = upto - mine;
-        }
-        for (int i = 0; i < kPaWaves; i++) before += s_sum[i];
-        if (lo < before * tasks) break;
-    }
-    __syncthreads();
-    s.b = __builtin_amdgcn_readfirstlane(s_b);
-    const int64_t into = lo - s_before * tasks;
-    const int count = listed(span_of(P, P.n_seq <= kPaKept ? K.len[s.b] : P.len[s.b]));
-    s.task = __builtin_amdgcn_readfirstlane((int) (into / count));
-    s.j = __builtin_amdgcn_readfirstlane((int) (into - (int64_t) s.task * count));
-    return s;
-}
-
-// SPLIT: equal shares of the list; otherwise a task each.
-template <int HD, bool SPLIT>
+// SPLIT: equal shares of the list; otherwise a task each. PRE: the parts of a prefix are joined to what begins a task.
+template <int HD, bool SPLIT, bool PRE>
 __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(PagedAttnParams P) {
     constexpr int NK = HD / 16, NM = HD / 32; // 16-byte K loads of a lane per page; matrix steps over the dims
     __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
@@ -186,7 +44,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
     }
     const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g4 = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int grp = P.n_head / P.n_kv, rows = min(grp, 16);
+    const int grp = P.n_head / P.n_kv;
     for (;;) {
         const int b = share.b, g = share.task % P.n_kv, rb = share.task / P.n_kv, row = rb * 16 + col;
         const bool kept = SPLIT && P.n_seq <= kPaKept;
@@ -235,6 +93,18 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         };
         int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
         if (n_page > 0) load_k(id);
+        if constexpr (PRE) {
+            if (j0 == 0)
+                take_prefix<HD>(P, b, g * grp + min(row, grp - 1), wv, g4 == 0, m_run, l_run, [&](const float *part, float f, float e) {
+#pragma unroll
+                    for (int t = 0; t < NM; t++) {
+                        const float4 x = *reinterpret_cast<const float4 *>(part + 32 * t + 8 * g4),
+                                     y = *reinterpret_cast<const float4 *>(part + 32 * t + 8 * g4 + 4);
+                        o[2 * t] = o[2 * t] * f + float4v{x.x, x.z, y.x, y.z} * e;
+                        o[2 * t + 1] = o[2 * t + 1] * f + float4v{x.y, x.w, y.y, y.w} * e;
+                    }
+                });
+        }
         __syncthreads();
         for (int it = 0; it < n_page; it++) {
             const int64_t cell0 = (int64_t) max(id, 0) * kPageCells;
@@ -331,43 +201,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == count;
-        // a part that continues one of the work-group before goes to the first of the work-group's two places, one that begins a
-        // task to the second
-        const int64_t place = 2 * (int64_t) blockIdx.x + (j0 == 0 ? 1 : 0);
-        for (int i = tid; i < 16 * (HD / 4); i += kPaWaves * kWave) {
-            const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
-            if (rb * 16 + r >= grp) continue;
-            float4 a = *reinterpret_cast<const float4 *>(&s_o[0][r][d]);
-            float l = s_l[0][r];
-#pragma unroll
-            for (int w = 1; w < kPaWaves; w++) {
-                const float4 e = *reinterpret_cast<const float4 *>(&s_o[w][r][d]);
-                a.x += e.x;
-                a.y += e.y;
-                a.z += e.z;
-                a.w += e.w;
-                l += s_l[w][r];
-            }
-            if (whole) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l; // no visible cell: zeros
-                ushort4 h;
-                h.x = __half_as_ushort(__float2half_rn(a.x * inv));
-                h.y = __half_as_ushort(__float2half_rn(a.y * inv));
-                h.z = __half_as_ushort(__float2half_rn(a.z * inv));
-                h.w = __half_as_ushort(__float2half_rn(a.w * inv));
-                *reinterpret_cast<ushort4 *>(P.out + ((int64_t) b * P.n_head + g * grp + rb * 16 + r) * HD + d) = h;
-            } else {
-                float *dst = P.part + (place * rows + r) * (HD + 4);
-                *reinterpret_cast<float4 *>(dst + 4 + d) = a;
-                if (d == 0) {
-                    float m = s_m[0][r];
-#pragma unroll
-                    for (int w = 1; w < kPaWaves; w++) m = fmaxf(m, s_m[w][r]);
-                    dst[0] = m;
-                    dst[1] = l;
-                }
-            }
-        }
+        write_part<HD>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o);
         if constexpr (!SPLIT) return;
         // where this part begins a task: how many other work-groups have the rest (the last is the one whose share holds the
         // task's last page)
@@ -470,9 +304,12 @@ __global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams
 
 template <int HD>
 hipError_t launch_paged_attn_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
-    const dim3 block(kPaWaves * kWave);
-    if (P.n_wg > 0) return launch(paged_attn_kernel<HD, true>, dim3(P.n_wg), block, 0, st, tm, P);
-    return launch(paged_attn_kernel<HD, false>, dim3((unsigned) P.n_seq * P.n_kv * P.n_rowblk), block, 0, st, tm, P);
+    const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
+    if (P.n_pre > 0)
+        return P.n_wg > 0 ? launch(paged_attn_kernel<HD, true, true>, all, block, 0, st, tm, P)
+                          : launch(paged_attn_kernel<HD, false, true>, all, block, 0, st, tm, P);
+    return P.n_wg > 0 ? launch(paged_attn_kernel<HD, true, false>, all, block, 0, st, tm, P)
+                      : launch(paged_attn_kernel<HD, false, false>, all, block, 0, st, tm, P);
 }
 
 template <int HD>

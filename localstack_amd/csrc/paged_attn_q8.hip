@@ -1,0 +1,248 @@
+// paged_attn_q8.hip - attention of one new token per sequence over the quantised cache of cache_q8.h (values d q, blocks of 32 dims).
+//
+//   s_i = scale log2(e) sum_m d_im (q_m . k_im)      k_im: the 32 whole numbers of block m of cell i
+//   o_m = sum_i (p_i d'_im) v_im,  p_i = 2^(s_i - r),  out = o / sum_i p_i
+//
+// List of pages, shares, parts and joins are those of attention over the fp16 cache (paged_parts.h, paged_attn_join_kernel). The
+// products take the whole numbers, which fp16 holds exactly, so the scales come after the first product (one fma a score and block)
+// and before the second one, in its weights; the result is that of the values d q in fp32.
+#include "cache_q8.h"
+#include "paged_parts.h"
+
+namespace lstk {
+namespace {
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+
+// Eight signed bytes as fp16: the byte with its sign bit flipped, under the exponent of 1024, is 1152 more than the number.
+__device__ __forceinline__ half8v wide(unsigned a, unsigned b) {
+    const half2v less = {(_Float16) 1152.0f, (_Float16) 1152.0f};
+    unsigned r[4];
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    r[0] = __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u);
+    r[1] = __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u);
+    r[2] = __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u);
+    r[3] = __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(unsigned, __builtin_bit_cast(half2v, r[i]) - less);
+    return halves(r[0], r[1], r[2], r[3]);
+}
+// Half e of eight.
+__device__ __forceinline__ float half_of(const uint4 &u, int e) {
+    const unsigned w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
+    return (float) __builtin_bit_cast(half2v, w)[e & 1];
+}
+__device__ __forceinline__ unsigned most_of(unsigned a, unsigned b) { // of two pairs of numbers that are not negative
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a), __builtin_bit_cast(ushort2v, b)));
+}
+
+template <int HD, bool SPLIT, bool PRE>
+__global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn_q8_kernel(PagedAttnParams P) {
+    constexpr int NM = HD / kQ8Dims;
+    __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
+    __shared__ __align__(16) float s_o[kPaWaves][16][HD + 4];
+    __shared__ uint4 s_q[NM][kWave];
+    const int tasks = P.n_kv * P.n_rowblk;
+    __shared__ Kept K;
+    Share share;
+    if constexpr (SPLIT) {
+        share = share_of(P, tasks, K);
+        if (share.left <= 0) return;
+    } else {
+        share.b = blockIdx.x / tasks;
+        share.task = blockIdx.x % tasks;
+        share.j = 0;
+    }
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 15, g4 = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int grp = P.n_head / P.n_kv;
+    for (;;) {
+        const int b = share.b, g = share.task % P.n_kv, rb = share.task / P.n_kv, row = rb * 16 + col;
+        const bool kept = SPLIT && P.n_seq <= kPaKept;
+        const Span sp = span_of(P, kept ? __builtin_amdgcn_readfirstlane(K.len[b]) : P.len[b]);
+        const int count = listed(sp), j0 = share.j, j1 = SPLIT ? (int) min((int64_t) count, j0 + share.left) : count;
+
+        // the operand Q^T: head `col`, dims 32 m + 8 g4 .. + 7
+        for (int m = wv; m < NM; m += kPaWaves) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(P.q + ((int64_t) b * P.n_head + g * grp + min(row, grp - 1)) * HD + 32 * m + 8 * g4);
+            s_q[m][lane] = row < grp ? u : make_uint4(0, 0, 0, 0);
+        }
+        float m_run = kLowest, l_run = 0.0f; // of head `col`; the sum of this lane's cells only
+        float4v o[2 * NM];                   // o[2 m + t]: dims 32 m + 16 t + 4 g4 + 0 .. 3
+#pragma unroll
+        for (int t = 0; t < 2 * NM; t++) o[t] = float4v{0, 0, 0, 0};
+
+        const int begin = j0 + wv, end = min(j1, sp.count);
+        const int n_page = end > begin ? (end - begin + kPaWaves - 1) / kPaWaves : 0;
+        const int64_t first = kept ? __builtin_amdgcn_readfirstlane(K.first[b]) : P.first[b];
+        auto page_of = [&](int i) {
+            const int j = begin + i * kPaWaves;
+            return j < sp.ps ? j : sp.pw + (j - sp.ps);
+        };
+        auto look_up = [&](int i) {
+            const int64_t at = first + page_of(i);
+            const int id = i < n_page && at >= 0 && at < P.n_table ? P.blocks[at] : -1;
+            return id >= 0 && id < P.kv_size / kPageCells ? id : -1;
+        };
+        const int seq = P.cell_seq ? P.seq[b] : 0;
+        auto record = [&](int id) { return reinterpret_cast<const char *>(P.q8) + ((int64_t) max(id, 0) * P.n_kv + g) * q8_record(HD); };
+        uint4 k[NM], kd[NM];
+        int owner = 0;
+        auto load_k = [&](int id) {
+            const char *rec = record(id);
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                k[m] = read_once(rec + 1024 * m + 16 * lane);
+                kd[m] = *reinterpret_cast<const uint4 *>(rec + q8_k_scale(HD, m, 0) + 16 * g4);
+            }
+            if (P.cell_seq) owner = P.cell_seq[(int64_t) max(id, 0) * kPageCells + (lane & (kPageCells - 1))];
+        };
+        int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
+        if (n_page > 0) load_k(id);
+        if constexpr (PRE) {
+            if (j0 == 0)
+                take_prefix<HD>(P, b, g * grp + min(row, grp - 1), wv, g4 == 0, m_run, l_run, [&](const float *part, float f, float e) {
+#pragma unroll
+                    for (int t = 0; t < 2 * NM; t++) {
+                        const float4 x = *reinterpret_cast<const float4 *>(part + 16 * t + 4 * g4);
+                        o[t] = o[t] * f + float4v{x.x, x.y, x.z, x.w} * e;
+                    }
+                });
+        }
+        __syncthreads();
+        for (int it = 0; it < n_page; it++) {
+            const char *rec = record(id);
+            uint4 v[NM], vd[NM];
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                v[m] = read_once(rec + q8_v(HD, m, 0, 0) + 16 * lane);
+                vd[m] = *reinterpret_cast<const uint4 *>(rec + q8_v_scale(HD, m, 0) + 16 * g4);
+            }
+            unsigned see = id >= 0 ? visible_cells(sp, page_of(it) * kPageCells) : 0u;
+            if (P.cell_seq) see &= (unsigned) __ballot(owner == seq);
+            float s[8]; // cells 8 g4 + 0 .. 7
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                const half8v q = __builtin_bit_cast(half8v, s_q[m][lane]);
+                const float4v none{0, 0, 0, 0};
+                const float4v s0 = mfma(wide(k[m].x, k[m].y), q, none), s1 = mfma(wide(k[m].z, k[m].w), q, none);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = e < 4 ? s0[e] : s1[e - 4], d = half_of(kd[m], e);
+                    s[e] = m == 0 ? x * d : fmaf(x, d, s[e]);
+                }
+            }
+            // the next page's K is on its way while this one's scores and V are worked on
+            __builtin_amdgcn_sched_barrier(0);
+            if ((it + 1) % kWave == 0) ids = look_up(it + 1 + lane);
+            id = __builtin_amdgcn_readlane(ids, (it + 1) % kWave);
+            if (it + 1 < n_page) load_k(id);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[e] *= P.scale;
+            if (see != ~0u) {
+                // the scores of cells that are not visible leave the sum, and their scales (what is there may be inf or NaN) the product
+                const unsigned mine = see >> (8 * g4);
+#pragma unroll
+                for (int e = 0; e < 8; e++) s[e] = mine >> e & 1u ? s[e] : -INFINITY;
+                unsigned keep[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    keep[e] = (mine >> (2 * e) & 1u ? 0xffffu : 0u) | (mine >> (2 * e + 1) & 1u ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int m = 0; m < NM; m++) vd[m] = make_uint4(vd[m].x & keep[0], vd[m].y & keep[1], vd[m].z & keep[2], vd[m].w & keep[3]);
+            }
+            // The reference r of the weights takes the scales of V in: p d' has to stay below 2^16 as an fp16 operand whatever the
+            // scales are, and as far up as it can, so that small weights keep their bits. 2^above is more than this lane's scales.
+            unsigned most = 0;
+#pragma unroll
+            for (int m = 0; m < NM; m++) most = most_of(most, most_of(most_of(vd[m].x, vd[m].y), most_of(vd[m].z, vd[m].w)));
+            const int above = (int) (max(most & 0xffffu, most >> 16) >> 10) - 14;
+            float top = s[0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
+            top = fmaxf(m_run, maximum_kept(across_groups_max(top + (float) above)));
+            const float f = __builtin_amdgcn_exp2f(m_run - top);
+            m_run = top;
+            l_run *= f;
+#pragma unroll
+            for (int t = 0; t < 2 * NM; t++) o[t] *= f;
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                p[e] = __builtin_amdgcn_exp2f(s[e] - m_run);
+                l_run += p[e];
+            }
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                // p d' = hi + lo in fp16, as in attention over the fp16 cache
+                half8v hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float w = p[e] * half_of(vd[m], e);
+                    hi[e] = (_Float16) w;
+                    lo[e] = (_Float16) (w - (float) hi[e]);
+                }
+                const half8v v0 = wide(v[m].x, v[m].y), v1 = wide(v[m].z, v[m].w);
+                o[2 * m] = mfma(v0, lo, o[2 * m]);
+                o[2 * m + 1] = mfma(v1, lo, o[2 * m + 1]);
+                o[2 * m] = mfma(v0, hi, o[2 * m]);
+                o[2 * m + 1] = mfma(v1, hi, o[2 * m + 1]);
+            }
+        }
+
+        // the wavefronts' shares at one maximum
+        l_run = across_groups_sum(l_run);
+        if (g4 == 0) s_m[wv][col] = m_run;
+        __syncthreads();
+        float top = kLowest;
+#pragma unroll
+        for (int w = 0; w < kPaWaves; w++) top = fmaxf(top, s_m[w][col]);
+        const float f = __builtin_amdgcn_exp2f(m_run - top);
+        if (g4 == 0) s_l[wv][col] = l_run * f;
+#pragma unroll
+        for (int t = 0; t < 2 * NM; t++)
+            *reinterpret_cast<float4 *>(&s_o[wv][col][16 * t + 4 * g4]) = make_float4(o[t][0] * f, o[t][1] * f, o[t][2] * f, o[t][3] * f);
+        __syncthreads();
+        const bool whole = j0 == 0 && j1 == count;
+        write_part<HD>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o);
+        if constexpr (!SPLIT) return;
+        if (tid == 0 && j0 == 0) {
+            const int64_t last = min(share.each * (blockIdx.x + 1), share.total) - share.left + count - 1;
+            P.split[(int64_t) b * tasks + share.task] = {(int) blockIdx.x, whole ? 0 : (int) (last / share.each) - (int) blockIdx.x};
+        }
+        share.left -= j1 - j0;
+        if (share.left == 0) return;
+        share.j = 0;
+        if (++share.task == tasks) {
+            share.task = 0;
+            share.b++;
+        }
+        __syncthreads(); // s_m, s_l and s_o are written again
+    }
+}
+
+template <int HD>
+hipError_t launch_paged_attn_q8_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
+    const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
+    if (P.n_pre > 0)
+        return P.n_wg > 0 ? launch(paged_attn_q8_kernel<HD, true, true>, all, block, 0, st, tm, P)
+                          : launch(paged_attn_q8_kernel<HD, false, true>, all, block, 0, st, tm, P);
+    return P.n_wg > 0 ? launch(paged_attn_q8_kernel<HD, true, false>, all, block, 0, st, tm, P)
+                      : launch(paged_attn_q8_kernel<HD, false, false>, all, block, 0, st, tm, P);
+}
+
+}  // namespace
+
+hipError_t launch_paged_attn_q8(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
+    switch (P.hd) {
+    case 64: return launch_paged_attn_q8_hd<64>(P, st, tm);
+    case 128: return launch_paged_attn_q8_hd<128>(P, st, tm);
+    case 256: return launch_paged_attn_q8_hd<256>(P, st, tm);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace lstk
