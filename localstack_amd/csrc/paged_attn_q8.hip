@@ -34,16 +34,63 @@ __device__ __forceinline__ float half_of(const uint4 &u, int e) {
     const unsigned w = e < 2 ? u.x : e < 4 ? u.y : e < 6 ? u.z : u.w;
     return (float) __builtin_bit_cast(half2v, w)[e & 1];
 }
-__device__ __forceinline__ unsigned most_of(unsigned a, unsigned b) { // of two pairs of numbers that are not negative
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { // of two pairs of halves that are not negative
     return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(ushort2v, a), __builtin_bit_cast(ushort2v, b)));
 }
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ unsigned dpp_bits(unsigned v) {
+    return (unsigned) __builtin_amdgcn_update_dpp(0, (int) v, CTRL, ROWS, 0xF, false);
+}
+// The largest of the wavefront's halves, numbers that are not negative, as bits.
+__device__ __forceinline__ unsigned most_of(unsigned v) {
+    v = larger(v, dpp_bits<0xB1>(v));
+    v = larger(v, dpp_bits<0x4E>(v));
+    v = larger(v, dpp_bits<0x141>(v));
+    v = larger(v, dpp_bits<0x140>(v));
+    v = larger(v, dpp_bits<kDppRowBcast15, 0xA>(v));
+    v = larger(v, dpp_bits<kDppRowBcast31, 0x8>(v));
+    v = (unsigned) __builtin_amdgcn_readlane((int) v, 63);
+    return max(v & 0xffffu, v >> 16);
+}
+// A page's scales, HD numbers of fp16: a lane's share of them on the way to LDS.
+template <int HD>
+struct ScaleShare {
+    static constexpr int kLanes = HD == 64 ? 32 : 64, kWords = HD == 256 ? 2 : 1;
+    unsigned w[kWords];
+    __device__ __forceinline__ void load(const char *p, int lane) {
+        if constexpr (kWords == 2) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p + 8 * lane);
+            w[0] = u.x;
+            w[1] = u.y;
+        } else {
+            w[0] = *reinterpret_cast<const unsigned *>(p + 4 * (lane % kLanes));
+        }
+    }
+    // Of cells that are not visible: 0.
+    __device__ __forceinline__ void hide(unsigned see, int lane) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            const unsigned two = see >> ((2 * kWords * lane + 2 * i) % kPageCells);
+            w[i] &= (two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u);
+        }
+    }
+    __device__ __forceinline__ unsigned most() const { return most_of(larger(w[0], w[kWords - 1])); }
+    __device__ __forceinline__ void store(uint4 *dst, int lane) const {
+        unsigned *p = reinterpret_cast<unsigned *>(dst) + kWords * (lane % kLanes);
+        if constexpr (kWords == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+        else *p = w[0];
+    }
+};
+// Between a wavefront's writes to LDS and its own reads of them.
+__device__ __forceinline__ void lds_settled() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <int HD, bool SPLIT, bool PRE>
-__global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn_q8_kernel(PagedAttnParams P) {
+__global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 3 : 2) void paged_attn_q8_kernel(PagedAttnParams P) {
     constexpr int NM = HD / kQ8Dims;
     __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
     __shared__ __align__(16) float s_o[kPaWaves][16][HD + 4];
     __shared__ uint4 s_q[NM][kWave];
+    __shared__ uint4 s_d[2][kPaWaves][NM * 4]; // a page's scales of K and of V, of each wavefront
     const int tasks = P.n_kv * P.n_rowblk;
     __shared__ Kept K;
     Share share;
@@ -88,15 +135,14 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
         };
         const int seq = P.cell_seq ? P.seq[b] : 0;
         auto record = [&](int id) { return reinterpret_cast<const char *>(P.q8) + ((int64_t) max(id, 0) * P.n_kv + g) * q8_record(HD); };
-        uint4 k[NM], kd[NM];
+        uint4 k[NM];
+        ScaleShare<HD> kd;
         int owner = 0;
         auto load_k = [&](int id) {
             const char *rec = record(id);
 #pragma unroll
-            for (int m = 0; m < NM; m++) {
-                k[m] = read_once(rec + 1024 * m + 16 * lane);
-                kd[m] = *reinterpret_cast<const uint4 *>(rec + q8_k_scale(HD, m, 0) + 16 * g4);
-            }
+            for (int m = 0; m < NM; m++) k[m] = read_once(rec + 1024 * m + 16 * lane);
+            kd.load(rec + q8_k_scale(HD, 0, 0), lane);
             if (P.cell_seq) owner = P.cell_seq[(int64_t) max(id, 0) * kPageCells + (lane & (kPageCells - 1))];
         };
         int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
@@ -114,23 +160,25 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
         __syncthreads();
         for (int it = 0; it < n_page; it++) {
             const char *rec = record(id);
-            uint4 v[NM], vd[NM];
+            uint4 v[NM];
+            ScaleShare<HD> vd;
+            kd.store(s_d[0][wv], lane);
+            vd.load(rec + q8_v_scale(HD, 0, 0), lane);
 #pragma unroll
-            for (int m = 0; m < NM; m++) {
-                v[m] = read_once(rec + q8_v(HD, m, 0, 0) + 16 * lane);
-                vd[m] = *reinterpret_cast<const uint4 *>(rec + q8_v_scale(HD, m, 0) + 16 * g4);
-            }
+            for (int m = 0; m < NM; m++) v[m] = read_once(rec + q8_v(HD, m, 0, 0) + 16 * lane);
             unsigned see = id >= 0 ? visible_cells(sp, page_of(it) * kPageCells) : 0u;
             if (P.cell_seq) see &= (unsigned) __ballot(owner == seq);
+            lds_settled();
             float s[8]; // cells 8 g4 + 0 .. 7
 #pragma unroll
             for (int m = 0; m < NM; m++) {
                 const half8v q = __builtin_bit_cast(half8v, s_q[m][lane]);
+                const uint4 d8 = s_d[0][wv][4 * m + g4];
                 const float4v none{0, 0, 0, 0};
                 const float4v s0 = mfma(wide(k[m].x, k[m].y), q, none), s1 = mfma(wide(k[m].z, k[m].w), q, none);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float x = e < 4 ? s0[e] : s1[e - 4], d = half_of(kd[m], e);
+                    const float x = e < 4 ? s0[e] : s1[e - 4], d = half_of(d8, e);
                     s[e] = m == 0 ? x * d : fmaf(x, d, s[e]);
                 }
             }
@@ -147,28 +195,24 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
                 const unsigned mine = see >> (8 * g4);
 #pragma unroll
                 for (int e = 0; e < 8; e++) s[e] = mine >> e & 1u ? s[e] : -INFINITY;
-                unsigned keep[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    keep[e] = (mine >> (2 * e) & 1u ? 0xffffu : 0u) | (mine >> (2 * e + 1) & 1u ? 0xffff0000u : 0u);
-#pragma unroll
-                for (int m = 0; m < NM; m++) vd[m] = make_uint4(vd[m].x & keep[0], vd[m].y & keep[1], vd[m].z & keep[2], vd[m].w & keep[3]);
+                vd.hide(see, lane);
             }
             // The reference r of the weights takes the scales of V in: p d' has to stay below 2^16 as an fp16 operand whatever the
-            // scales are, and as far up as it can, so that small weights keep their bits. 2^above is more than this lane's scales.
-            unsigned most = 0;
-#pragma unroll
-            for (int m = 0; m < NM; m++) most = most_of(most, most_of(most_of(vd[m].x, vd[m].y), most_of(vd[m].z, vd[m].w)));
-            const int above = (int) (max(most & 0xffffu, most >> 16) >> 10) - 14;
+            // scales are, and as far up as it can, so that small weights keep their bits. 2^above is more than any scale of the page.
+            const int above = (int) (vd.most() >> 10) - 14;
+            vd.store(s_d[1][wv], lane);
             float top = s[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
             top = fmaxf(m_run, maximum_kept(across_groups_max(top + (float) above)));
-            const float f = __builtin_amdgcn_exp2f(m_run - top);
-            m_run = top;
-            l_run *= f;
+            if (__any(top > m_run)) {
+                const float f = __builtin_amdgcn_exp2f(m_run - top);
+                m_run = top;
+                l_run *= f;
 #pragma unroll
-            for (int t = 0; t < 2 * NM; t++) o[t] *= f;
+                for (int t = 0; t < 2 * NM; t++) o[t] *= f;
+            }
+            lds_settled();
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -177,11 +221,12 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
             }
 #pragma unroll
             for (int m = 0; m < NM; m++) {
+                const uint4 d8 = s_d[1][wv][4 * m + g4];
                 // p d' = hi + lo in fp16, as in attention over the fp16 cache
                 half8v hi, lo;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float w = p[e] * half_of(vd[m], e);
+                    const float w = p[e] * half_of(d8, e);
                     hi[e] = (_Float16) w;
                     lo[e] = (_Float16) (w - (float) hi[e]);
                 }
