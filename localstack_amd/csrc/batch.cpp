@@ -3,6 +3,7 @@
 // lstk_moe_select (include/lstk_moe.h). They hold no state: the caller owns every buffer, the workspaces among them.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -29,8 +30,9 @@ constexpr int kMostTokens = 1 << 24;
 constexpr float kLog2e = 1.44269504088896341f;
 
 // Shapes of a paged attention call, checked, and its plan.
-int paged_plan(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink, lstk::PagedAttnParams &P,
+int paged_plan(bool q8, int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink, lstk::PagedAttnParams &P,
                size_t &bytes) {
+    P.in_q8 = q8;
     if (n_seq < 0) return bad("n_seq must be >= 0");
     if (n_head < 1 || n_head_kv < 1 || n_head % n_head_kv) return bad("n_head must be a positive multiple of n_head_kv");
     if (!lstk::attn_supported(head_dim)) return bad("head_dim must be 64, 128 or 256");
@@ -114,7 +116,7 @@ int run_shared(const lstk_prefix *prefix, const Cache *cache, const lstk_paged_s
     lstk::PagedAttnParams P{};
     lstk::PrefixAttnParams X{};
     size_t own = 0, pre = 0;
-    int rc = paged_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, 0, 0, P, own);
+    int rc = paged_plan(q8, seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, 0, 0, P, own);
     if (rc == LSTK_OK) rc = prefix_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, prefix->max_len, X, pre);
     if (rc != LSTK_OK) return rc;
     if (prefix->cache->n_head_kv != cache->n_head_kv || prefix->cache->head_dim != cache->head_dim)
@@ -175,7 +177,7 @@ extern "C" {
 size_t lstk_attn_paged_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink) {
     lstk::PagedAttnParams P{};
     size_t bytes = 0;
-    return paged_plan(n_seq, n_head, n_head_kv, head_dim, max_len, window, n_sink, P, bytes) == LSTK_OK ? bytes : 0;
+    return paged_plan(false, n_seq, n_head, n_head_kv, head_dim, max_len, window, n_sink, P, bytes) == LSTK_OK ? bytes : 0;
 }
 
 int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head, int window,
@@ -183,7 +185,7 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
     if (!cache || !seqs) return bad("null argument");
     lstk::PagedAttnParams P{};
     size_t bytes = 0;
-    int rc = paged_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
+    int rc = paged_plan(false, seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
     if (rc != LSTK_OK) return rc;
     if (seqs->n_table < 0) return bad("n_table must be >= 0");
     if (!std::isfinite(scale)) return bad("scale must be finite");
@@ -197,7 +199,9 @@ int lstk_attn_paged(const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, 
 }
 
 size_t lstk_attn_paged_q8_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int window, int n_sink) {
-    return lstk_attn_paged_work_bytes(n_seq, n_head, n_head_kv, head_dim, max_len, window, n_sink);
+    lstk::PagedAttnParams P{};
+    size_t bytes = 0;
+    return paged_plan(true, n_seq, n_head, n_head_kv, head_dim, max_len, window, n_sink, P, bytes) == LSTK_OK ? bytes : 0;
 }
 
 int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head, int window, int n_sink,
@@ -205,7 +209,7 @@ int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, 
     if (!cache || !seqs) return bad("null argument");
     lstk::PagedAttnParams P{};
     size_t bytes = 0;
-    int rc = paged_plan(seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
+    int rc = paged_plan(true, seqs->n_seq, n_head, cache->n_head_kv, cache->head_dim, seqs->max_len, window, n_sink, P, bytes);
     if (rc != LSTK_OK) return rc;
     if (seqs->n_table < 0) return bad("n_table must be >= 0");
     if (!std::isfinite(scale)) return bad("scale must be finite");
@@ -220,12 +224,16 @@ int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, 
     return e == hipSuccess ? LSTK_OK : hip_fail(e, "paged attention launch");
 }
 
+// What serves both kinds of caches.
 size_t lstk_attn_shared_work_bytes(int n_seq, int n_head, int n_head_kv, int head_dim, int max_len, int max_prefix) {
     lstk::PagedAttnParams P{};
     lstk::PrefixAttnParams X{};
-    size_t own = 0, pre = 0;
-    return paged_plan(n_seq, n_head, n_head_kv, head_dim, max_len, 0, 0, P, own) == LSTK_OK &&
-                   prefix_plan(n_seq, n_head, n_head_kv, head_dim, max_prefix, X, pre) == LSTK_OK ? pre + own : 0;
+    size_t own = 0, own_q8 = 0, pre = 0;
+    return paged_plan(false, n_seq, n_head, n_head_kv, head_dim, max_len, 0, 0, P, own) == LSTK_OK &&
+                   paged_plan(true, n_seq, n_head, n_head_kv, head_dim, max_len, 0, 0, P, own_q8) == LSTK_OK &&
+                   prefix_plan(n_seq, n_head, n_head_kv, head_dim, max_prefix, X, pre) == LSTK_OK
+               ? pre + std::max(own, own_q8)
+               : 0;
 }
 
 int lstk_attn_shared(const lstk_prefix *prefix, const lstk_paged_cache *cache, const lstk_paged_seqs *seqs, const uint16_t *d_q, int n_head,

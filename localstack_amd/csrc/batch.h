@@ -32,7 +32,8 @@ struct PagedAttnParams {
     PagedAttnSplit *split; // [n_seq][n_kv * n_rowblk], a task each
     float *part;           // [n_wg][2][min(16, heads per KV head)][hd + 4]: max, sum, 2 unused, unnormalised output of a part of a task
     uint16_t *out;         // [n_seq][n_head][hd] fp16
-    const uint8_t *q8 = nullptr;  // in place of kc and vc: the records of a quantised cache (cache_q8.h), kv_size / 32 pages
+    bool in_q8 = false;           // the cache is a quantised one (set before paged_attn_plan):
+    const uint8_t *q8 = nullptr;  // its records (cache_q8.h) in place of kc and vc, kv_size / 32 pages
     const float *pre = nullptr;   // [n_pre][n_seq][n_head][hd + 4]: what parts of a prefix left, in the form of `part`
     int n_pre = 0;
 };

@@ -339,8 +339,10 @@ size_t paged_attn_plan(PagedAttnParams &P) {
     // the equal shares cost some 10 us more (their way to the first page and the second launch). Us a call at 32 heads on 4:
     // 64 sequences of 100 to 500 cells 12 and 22, 64 of 100 to 1000 18 and 26, one of 1000 15 and 14.
     if (pages <= 16 || (pages <= 64 && tasks >= kPaCus) || tasks == 0) return 0;
-    // equal shares, of kPaLeast pages or more, for two work-groups a CU: all of them are there at once
-    P.n_wg = (int) std::max<int64_t>(1, std::min<int64_t>(kPaCus * kPaPerCu, tasks * pages / kPaLeast));
+    // equal shares, of kPaLeast pages or more, for two work-groups a CU (three where they take half the bytes and registers allow it):
+    // all of them are there at once
+    const int per_cu = P.in_q8 && P.hd < 256 ? kPaPerCuQ8 : kPaPerCu;
+    P.n_wg = (int) std::max<int64_t>(1, std::min<int64_t>(kPaCus * per_cu, tasks * pages / kPaLeast));
     return split_entries(P) * sizeof(PagedAttnSplit) + (size_t) P.n_wg * 2 * std::min(grp, 16) * (P.hd + 4) * sizeof(float);
 }
 

@@ -85,7 +85,7 @@ struct ScaleShare {
 __device__ __forceinline__ void lds_settled() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <int HD, bool SPLIT, bool PRE>
-__global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 3 : 2) void paged_attn_q8_kernel(PagedAttnParams P) {
+__global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn_q8_kernel(PagedAttnParams P) {
     constexpr int NM = HD / kQ8Dims;
     __shared__ float s_m[kPaWaves][16], s_l[kPaWaves][16];
     __shared__ __align__(16) float s_o[kPaWaves][16][HD + 4];
@@ -116,6 +116,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 3 : 2) void paged_attn_
             const uint4 u = *reinterpret_cast<const uint4 *>(P.q + ((int64_t) b * P.n_head + g * grp + min(row, grp - 1)) * HD + 32 * m + 8 * g4);
             s_q[m][lane] = row < grp ? u : make_uint4(0, 0, 0, 0);
         }
+        float minus = -1.0f; // kept from the compiler: w - hi is one instruction as an fma of fp16 numbers, four as a difference
+        asm("" : "+v"(minus));
         float m_run = kLowest, l_run = 0.0f; // of head `col`; the sum of this lane's cells only
         float4v o[2 * NM];                   // o[2 m + t]: dims 32 m + 16 t + 4 g4 + 0 .. 3
 #pragma unroll
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 3 : 2) void paged_attn_
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float x = e < 4 ? s0[e] : s1[e - 4], d = half_of(d8, e);
-                    s[e] = m == 0 ? x * d : fmaf(x, d, s[e]);
+                    s[e] = fmaf(x, d, m == 0 ? 0.0f : s[e]); // (an fma takes d as fp16, a product does not)
                 }
             }
             // the next page's K is on its way while this one's scores and V are worked on
@@ -226,9 +228,9 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 3 : 2) void paged_attn_
                 half8v hi, lo;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float w = p[e] * half_of(d8, e);
+                    const float w = fmaf(p[e], half_of(d8, e), 0.0f);
                     hi[e] = (_Float16) w;
-                    lo[e] = (_Float16) (w - (float) hi[e]);
+                    lo[e] = (_Float16) fmaf((float) hi[e], minus, w);
                 }
                 const half8v v0 = wide(v[m].x, v[m].y), v1 = wide(v[m].z, v[m].w);
                 o[2 * m] = mfma(v0, lo, o[2 * m]);

@@ -13,7 +13,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 
 constexpr int kPaWaves = 4;
 constexpr int kPaCus = 256; // of MI355X
-constexpr int kPaPerCu = 2; // work-groups of equal shares per CU
+constexpr int kPaPerCu = 2, kPaPerCuQ8 = 3; // work-groups of equal shares per CU
 constexpr int kPaLeast = 4; // pages of a share
 constexpr int kPaRound = 4;  // rounds of the wavefronts up to which a share is made a whole number of them
 constexpr float kLowest = -3.0e38f; // a running maximum that any score replaces

@@ -99,7 +99,7 @@ def test_shared_attention_of_one_kind_only(lstk):
 
 def test_shared_workspace(lstk):
     """More room is never needed for shorter sequences or prefixes; no prefix needs what attention without one needs."""
-    w, own = lstk.shared_attention_work_bytes, lstk.paged_attention_work_bytes
+    w, own = lstk.shared_attention_work_bytes, lstk.paged_attention_q8_work_bytes
     for n, H, kv, hd in ((1, 32, 4, 128), (3, 64, 4, 128), (100, 4, 2, 64), (128, 32, 4, 128), (1000, 16, 2, 256), (7, 40, 2, 128)):
         assert w(n, H, kv, hd, 1, 0) == 0 and w(n, H, kv, hd, 9000, 0) == own(n, H, kv, hd, 9000)
         sizes = [w(n, H, kv, hd, 100, m) for m in list(range(1, 5000, 37)) + [10 ** 4, 10 ** 5, 10 ** 6, BIG]]
