@@ -9,6 +9,8 @@
 // A page (32 cells) is the A operand of 32 x 32 x 16 fp16 matrix instructions, 32 query rows the B operand: HD / 16 of them for S^T,
 // as many for O^T. Their results leave a lane with 16 cells of one row, 8 in a row of each half of the page, which is what it needs
 // of the operand P: nothing is moved between the products.
+#include <type_traits>
+
 #include "device.h"
 #include "paged_parts.h"
 
@@ -37,8 +39,10 @@ template <int HD, bool SHARED>
 __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 256 ? 2 : 1) void prefix_attn_kernel(PrefixAttnParams P) {
     constexpr int W = px_waves<HD, SHARED>(), G = SHARED ? kPxGroups : W, NT = SHARED ? kPxTiles : 1; // page groups, row tiles
     constexpr int NS = HD / 16, ND = HD / 32;                                                        // steps over the dims; dim tiles
-    constexpr int kBytes = HD * 64;                                                                  // of K, and of V, of a page
-    extern __shared__ __align__(16) char s_mem[]; // SHARED: [2 buffers][G][K | V]; then [W / 2][HD / 4][32 rows] float4
+    constexpr int kBytes = HD * 64, kPages = SHARED && HD < 256 ? 2 : 1; // of K, and of V, of a page; pages of a turn
+    // SHARED: [2 buffers][G][kPages][K | V]; then what W / 2 wavefronts have, [W / 2][HD / 4][32 rows] float4
+    constexpr int kRoom = std::max(SHARED ? 2 * G * kPages * 2 * kBytes : 0, W / 2 * HD * kPxRows * 4);
+    __shared__ __align__(16) char s_mem[kRoom];
     __shared__ float s_m[W][kPxRows], s_l[W][kPxRows];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), col = lane & 31, h = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(tid / kWave), tile = wv % NT, group = wv / NT;
@@ -53,7 +57,7 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 25
     // Q^T: row `col`, dims 16 i + 4 h + 0 .. 3 and 16 i + 8 + 4 h + 0 .. 3; with its sign turned where the scale is negative
     half8v q[NS];
     const unsigned turn = P.scale < 0.0f ? 0x80008000u : 0u;
-    const float scale = fabsf(P.scale);
+    const float scale = fmaxf(fabsf(P.scale), 1e-38f); // (a zero would make NaN of the -inf of cells that are not visible)
 #pragma unroll
     for (int i = 0; i < NS; i++) {
         const uint16_t *src = P.q + head * HD + 16 * i + 4 * h;
@@ -69,32 +73,42 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 25
 
     const int len = max(0, min(P.len[0], P.max_len)), pages = pages_of(len), each = (pages + P.n_chunk - 1) / P.n_chunk;
     const int begin = min(pages, chunk * each), end = min(pages, begin + each);
-    const int n_it = (end - begin + G - 1) / G;
-    auto look_up = [&](int i) { // the page of this group's turn i; -1: none
-        const int j = begin + i * G + group;
-        const int id = i < n_it && j < end && j < P.n_table ? P.blocks[j] : -1;
+    const int n_it = (end - begin + G * kPages - 1) / (G * kPages); // turns of kPages pages
+    auto page_at = [&](int i) { return begin + i * G + group; };      // this group's page i
+    auto look_up = [&](int i) {                                       // its number; -1: none
+        const int j = page_at(i);
+        const int id = j < end && j < P.n_table ? P.blocks[j] : -1;
         return id >= 0 && id < P.kv_size / kPageCells ? id : -1;
     };
     const char *const k_head = reinterpret_cast<const char *>(P.kc) + (int64_t) (g * (HD / 4)) * P.kv_size * 8;
     const char *const v_head = reinterpret_cast<const char *>(P.vc) + (int64_t) g * P.kv_size * (HD * 2);
 
-    // One page: k(i), k'(i): the lane's cell, dims as q[i]; v(s, t): the lane's dim of tile t, cells 16 s + 4 h + 0 .. 3 and
-    // 16 s + 8 + 4 h + 0 .. 3.
-    auto work = [&](unsigned see, auto &&k_of, auto &&between, auto &&v_of) {
-        float16v s;
+    // NP pages: k_of(n, i): the lane's cell of page n, dims as q[i]; v_of(n, s, t): the lane's dim of tile t, cells 16 s + 4 h + 0 .. 3
+    // and 16 s + 8 + 4 h + 0 .. 3, zeros where a cell is not visible.
+    auto work = [&](auto np, const unsigned *see, auto &&k_of, auto &&between, auto &&v_of) {
+        constexpr int NP = decltype(np)::value;
+        float16v s[NP];
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+        for (int n = 0; n < NP; n++)
 #pragma unroll
-        for (int i = 0; i < NS; i++) s = mfma32(k_of(i), q[i], s);
+            for (int i = 0; i < 16; i++) s[n][i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+            for (int n = 0; n < NP; n++) s[n] = mfma32(k_of(n, i), q[i], s[n]);
         between();
-        const unsigned mine = see >> (4 * h); // cell of s[i]: bit 8 (i / 4) + i % 4
-        if (see != ~0u) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = mine >> (8 * (i / 4) + i % 4) & 1u ? s[i] : -INFINITY;
-        }
-        float top = s[0];
+        for (int n = 0; n < NP; n++)
+            if (see[n] != ~0u) {
+                const unsigned mine = see[n] >> (4 * h); // cell of s[i]: bit 8 (i / 4) + i % 4
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+                for (int i = 0; i < 16; i++) s[n][i] = mine >> (8 * (i / 4) + i % 4) & 1u ? s[n][i] : -INFINITY;
+            }
+        float top = s[0][0];
+#pragma unroll
+        for (int n = 0; n < NP; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
         top = fmaxf(top, __shfl_xor(top, 32, kWave)) * scale;
         // Scores so large that they are rounded by more than 2^-4 have the largest itself for a reference.
         const bool fine = fabsf(top) < kExactTo, raise = top > m_run && !(fine && top - m_run <= kPxUnder + kPxSlack);
@@ -108,77 +122,106 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 25
         // (the fma's exact product may lie above the rounded one that the reference comes from)
         if (__any(!(fabsf(m_run) < kExactTo))) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = s[i] * scale - m_run;
+            for (int n = 0; n < NP; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = s[n][i] * scale - m_run;
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = fmaf(s[i], scale, -m_run);
-        }
-        float sum = 0.0f;
-        half8v p[2];
+            for (int n = 0; n < NP; n++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float x = __builtin_amdgcn_exp2f(s[i]);
-            if (see != ~0u) x = mine >> (8 * (i / 4) + i % 4) & 1u ? x : 0.0f;
-            p[i / 8][i % 8] = (_Float16) x;
+                for (int i = 0; i < 16; i++) s[n][i] = fmaf(s[n][i], scale, -m_run);
         }
         // The weights enter the product in one fp16 part, and the sum as they enter it, so that they still add up to one.
 #pragma unroll
-        for (int i = 0; i < 16; i += 2)
-            sum = __builtin_amdgcn_fdot2(half2v{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, half2v{(_Float16) 1.0f, (_Float16) 1.0f}, sum, false);
-        l_run += sum;
+        for (int n = 0; n < NP; n++) {
+            float sum = 0.0f;
+            half8v p[2];
 #pragma unroll
-        for (int t = 0; t < ND; t++)
+            for (int i = 0; i < 16; i++) p[i / 8][i % 8] = (_Float16) __builtin_amdgcn_exp2f(s[n][i]);
 #pragma unroll
-            for (int s2 = 0; s2 < 2; s2++) {
-                uint2 a, b;
-                v_of(s2, t, a, b);
-                if (see != ~0u) {
-                    // what the cache holds in cells that are not visible leaves the product too
-                    auto keep = [&](int c) { return (mine >> c & 1u ? 0xffffu : 0u) | (mine >> (c + 1) & 1u ? 0xffff0000u : 0u); };
-                    a = make_uint2(a.x & keep(16 * s2), a.y & keep(16 * s2 + 2));
-                    b = make_uint2(b.x & keep(16 * s2 + 8), b.y & keep(16 * s2 + 10));
-                }
-                o[t] = mfma32(pair(a, b), p[s2], o[t]);
-            }
+            for (int i = 0; i < 16; i += 2)
+                sum = __builtin_amdgcn_fdot2(half2v{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, half2v{(_Float16) 1.0f, (_Float16) 1.0f}, sum, false);
+            l_run += sum;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; s2++)
+#pragma unroll
+                for (int t = 0; t < ND; t++) o[t] = mfma32(v_of(n, s2, t), p[s2], o[t]);
+        }
     };
-    auto seen = [&](int id, int i) { return id < 0 ? 0u : bits_below(len - (begin + i * G + group) * kPageCells); };
+    auto seen = [&](int id, int i) { return id < 0 ? 0u : bits_below(len - page_at(i) * kPageCells); };
+    auto keep = [](unsigned see, int c) { return (see >> c & 1u ? 0xffffu : 0u) | (see >> (c + 1) & 1u ? 0xffff0000u : 0u); }; // cells c, c + 1
 
     if constexpr (SHARED) {
-        // Pages go straight to LDS as they lie in the cache: K [HD / 4][32 cells][4 dims], V [8][HD][4 cells].
-        typedef __attribute__((address_space(3))) void lds_void;
-        typedef const __attribute__((address_space(1))) void global_void;
-        auto ask = [&](int id, int buffer) {
-            if (id < 0) return;
-            char *dst = s_mem + (buffer * G + group) * 2 * kBytes;
-            const char *kp = k_head + (int64_t) id * (kPageCells * 8), *vp = v_head + (int64_t) id * (kPageCells * HD * 2);
+        // Pages go by way of registers to LDS as they lie in the cache: K [HD / 4][32 cells][4 dims], V [8][HD][4 cells]. The next
+        // ones are on their way while these are worked on.
+        constexpr int NP = kPages, NL = kBytes / 1024 / NT; // a wavefront's KiB of K, and of V, of a page
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 kl[NP][NL], vl[NP][NL];
+        int id[NP], next[NP];
+        auto ask = [&](const int *id) {
 #pragma unroll
-            for (int c = 0; c < kBytes / 1024 / NT; c++) {
-                const int part = c * NT + tile; // 1 KiB: 4 quads of dims of K
-                __builtin_amdgcn_global_load_lds((global_void *) (kp + (int64_t) (4 * part + lane / 16) * P.kv_size * 8 + lane % 16 * 16),
-                                                 (lds_void *) (dst + part * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((global_void *) (vp + part * 1024 + lane * 16), (lds_void *) (dst + kBytes + part * 1024), 16, 0, 0);
+            for (int n = 0; n < NP; n++) {
+                const char *kp = k_head + (int64_t) max(id[n], 0) * (kPageCells * 8), *vp = v_head + (int64_t) max(id[n], 0) * (kPageCells * HD * 2);
+#pragma unroll
+                for (int c = 0; c < NL; c++) {
+                    const int part = c * NT + tile; // 1 KiB: 4 quads of dims of K
+                    kl[n][c] = *reinterpret_cast<const u32x4 *>(kp + (int64_t) (4 * part + lane / 16) * P.kv_size * 8 + lane % 16 * 16);
+                    vl[n][c] = *reinterpret_cast<const u32x4 *>(vp + part * 1024 + lane * 16);
+                }
             }
         };
-        int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
-        ask(id, 0);
+        auto put = [&](const int *id, int it, int buffer) {
+            char *dst = s_mem + (buffer * G + group) * NP * 2 * kBytes;
+#pragma unroll
+            for (int n = 0; n < NP; n++) {
+                const unsigned see = seen(id[n], it * NP + n);
+#pragma unroll
+                for (int c = 0; c < NL; c++) {
+                    const int part = c * NT + tile;
+                    u32x4 v = vl[n][c];
+                    if (see != ~0u) {
+                        // what the cache holds in cells that are not visible (it may be inf or NaN) leaves the product
+                        const int cell = (part * 1024 + lane * 16) / (HD * 8) * 4;
+                        const unsigned k0 = keep(see, cell), k1 = keep(see, cell + 2);
+                        v &= u32x4{k0, k1, k0, k1};
+                    }
+                    *reinterpret_cast<u32x4 *>(dst + n * 2 * kBytes + part * 1024 + lane * 16) = kl[n][c];
+                    *reinterpret_cast<u32x4 *>(dst + n * 2 * kBytes + kBytes + part * 1024 + lane * 16) = v;
+                }
+            }
+        };
+        int ids = look_up(lane);
+        auto ids_of = [&](int it, int *id) {
+            if (it * NP % kWave == 0 && it > 0) ids = look_up(it * NP + lane);
+#pragma unroll
+            for (int n = 0; n < NP; n++) id[n] = __builtin_amdgcn_readlane(ids, (it * NP + n) % kWave);
+        };
+        ids_of(0, id);
+        if (n_it > 0) {
+            ask(id);
+            put(id, 0, 0);
+        }
         for (int it = 0; it < n_it; it++) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads(); // this page is there, and nobody reads the one before any more
-            if ((it + 1) % kWave == 0) ids = look_up(it + 1 + lane);
-            const int next = __builtin_amdgcn_readlane(ids, (it + 1) % kWave);
-            ask(next, (it + 1) & 1);
-            const unsigned see = seen(id, it);
-            const char *src = s_mem + ((it & 1) * G + group) * 2 * kBytes;
-            if (see != 0)
-                work(see, [&](int i) {
-                    const char *p = src + (4 * i + h) * 256 + col * 8;
+            __syncthreads(); // these pages are there, and nobody reads the ones before any more
+            if (it + 1 < n_it) {
+                ids_of(it + 1, next);
+                ask(next);
+            }
+            unsigned see[NP], any = 0;
+#pragma unroll
+            for (int n = 0; n < NP; n++) any |= see[n] = seen(id[n], it * NP + n);
+            const char *src = s_mem + ((it & 1) * G + group) * NP * 2 * kBytes;
+            if (any != 0)
+                work(std::integral_constant<int, NP>(), see, [&](int n, int i) {
+                    const char *p = src + n * 2 * kBytes + (4 * i + h) * 256 + col * 8;
                     return pair(*reinterpret_cast<const uint2 *>(p), *reinterpret_cast<const uint2 *>(p + 512));
-                }, [] {}, [&](int s2, int t, uint2 &a, uint2 &b) {
-                    const char *p = src + kBytes + ((4 * s2 + h) * HD + 32 * t + col) * 8;
-                    a = *reinterpret_cast<const uint2 *>(p);
-                    b = *reinterpret_cast<const uint2 *>(p + 2 * HD * 8);
+                }, [] {}, [&](int n, int s2, int t) {
+                    const char *p = src + n * 2 * kBytes + kBytes + ((4 * s2 + h) * HD + 32 * t + col) * 8;
+                    return pair(*reinterpret_cast<const uint2 *>(p), *reinterpret_cast<const uint2 *>(p + 2 * HD * 8));
                 });
-            id = next;
+            if (it + 1 < n_it) put(next, it + 1, (it + 1) & 1);
+#pragma unroll
+            for (int n = 0; n < NP; n++) id[n] = next[n];
         }
         __syncthreads(); // the pages' room is written again
     } else {
@@ -200,15 +243,21 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 25
             const unsigned see = seen(id, it);
             if ((it + 1) % kWave == 0) ids = look_up(it + 1 + lane);
             id = __builtin_amdgcn_readlane(ids, (it + 1) % kWave);
-            work(see, [&](int i) { return pair(k[2 * i], k[2 * i + 1]); }, [&] {
+            work(std::integral_constant<int, 1>(), &see, [&](int, int i) { return pair(k[2 * i], k[2 * i + 1]); }, [&] {
                 // the next page's K is on its way while this one's scores and V are worked on
                 __builtin_amdgcn_sched_barrier(0);
                 if (it + 1 < n_it) load_k(id);
                 __builtin_amdgcn_sched_barrier(0);
-            }, [&](int s2, int t, uint2 &a, uint2 &b) {
-                a = v[2 * t + s2][0];
-                b = v[2 * t + s2][1];
-            });
+                if (see != ~0u) {
+#pragma unroll
+                    for (int i = 0; i < 2 * ND; i++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int c = 16 * (i & 1) + 8 * e + 4 * h;
+                            v[i][e] = make_uint2(v[i][e].x & keep(see, c), v[i][e].y & keep(see, c + 2));
+                        }
+                }
+            }, [&](int, int s2, int t) { return pair(v[2 * t + s2][0], v[2 * t + s2][1]); });
         }
     }
     l_run += __shfl_xor(l_run, 32, kWave);
@@ -261,14 +310,8 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 25
 
 template <int HD, bool SHARED>
 hipError_t launch_prefix(const PrefixAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
-    constexpr int W = px_waves<HD, SHARED>();
-    // pages while they are worked on, what half the wavefronts have of the sums afterwards
-    constexpr size_t lds = std::max<size_t>(SHARED ? 2 * kPxGroups * 2 * HD * 64 : 0, (size_t) W / 2 * HD * kPxRows * sizeof(float));
-    static std::atomic<uint64_t> asked{0};
-    const hipError_t e = allow_dynamic_lds(reinterpret_cast<const void *>(prefix_attn_kernel<HD, SHARED>), lds, asked);
-    if (e != hipSuccess) return e;
     const unsigned pairs = ((unsigned) P.n_chunk * P.n_kv + 7) / 8 * 8;
-    return launch(prefix_attn_kernel<HD, SHARED>, dim3(pairs * P.n_rowblk), dim3(W * kWave), lds, st, tm, P);
+    return launch(prefix_attn_kernel<HD, SHARED>, dim3(pairs * P.n_rowblk), dim3(px_waves<HD, SHARED>() * kWave), 0, st, tm, P);
 }
 
 template <int HD>
