@@ -34,7 +34,7 @@ struct PagedAttnParams {
     uint16_t *out;         // [n_seq][n_head][hd] fp16
     bool in_q8 = false;           // the cache is a quantised one (set before paged_attn_plan):
     const uint8_t *q8 = nullptr;  // its records (cache_q8.h) in place of kc and vc, kv_size / 32 pages
-    const float *pre = nullptr;   // [n_pre][n_seq][n_head][hd + 4]: what parts of a prefix left, in the form of `part`
+    float *pre = nullptr;         // [n_pre + 1][n_seq][n_head][hd + 4]: what parts of a prefix left, in the form of `part`, and room
     int n_pre = 0;
 };
 // Fills n_rowblk and n_wg; returns the bytes of workspace (16-byte aligned) that calls of these shapes with this max_len or a
@@ -58,7 +58,7 @@ struct PrefixAttnParams {
     bool shared;           // the wavefronts of a work-group share pages; otherwise each takes its own
     float *part;
 };
-// Fills n_chunk, n_rowblk and shared; returns the bytes of `part` (0: no prefix).
+// Fills n_chunk, n_rowblk and shared; returns the bytes of `part` with room for one more (0: no prefix).
 size_t prefix_attn_plan(PrefixAttnParams &P);
 hipError_t launch_prefix_attn(const PrefixAttnParams &P, hipStream_t st, const LaunchTiming *tm);
 

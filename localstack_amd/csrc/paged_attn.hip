@@ -24,7 +24,8 @@
 namespace lstk {
 namespace {
 
-// SPLIT: equal shares of the list; otherwise a task each. PRE: the parts of a prefix are joined to what begins a task.
+// SPLIT: equal shares of the list; otherwise a task each. PRE: the parts of a prefix are joined to a task (SPLIT leaves that to the
+// launch that joins a task's own parts).
 template <int HD, bool SPLIT, bool PRE>
 __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(PagedAttnParams P) {
     constexpr int NK = HD / 16, NM = HD / 32; // 16-byte K loads of a lane per page; matrix steps over the dims
@@ -93,18 +94,6 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         };
         int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
         if (n_page > 0) load_k(id);
-        if constexpr (PRE) {
-            if (j0 == 0)
-                take_prefix<HD>(P, b, g * grp + min(row, grp - 1), wv, g4 == 0, m_run, l_run, [&](const float *part, float f, float e) {
-#pragma unroll
-                    for (int t = 0; t < NM; t++) {
-                        const float4 x = *reinterpret_cast<const float4 *>(part + 32 * t + 8 * g4),
-                                     y = *reinterpret_cast<const float4 *>(part + 32 * t + 8 * g4 + 4);
-                        o[2 * t] = o[2 * t] * f + float4v{x.x, x.z, y.x, y.z} * e;
-                        o[2 * t + 1] = o[2 * t + 1] * f + float4v{x.y, x.w, y.y, y.w} * e;
-                    }
-                });
-        }
         __syncthreads();
         for (int it = 0; it < n_page; it++) {
             const int64_t cell0 = (int64_t) max(id, 0) * kPageCells;
@@ -183,6 +172,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
             }
         }
 
+        PrefixParts<HD> ahead;
+        if constexpr (PRE) ask_first(P, b, g, rb, ahead);
         // the wavefronts' shares at one maximum
         l_run = across_groups_sum(l_run);
         if (g4 == 0) s_m[wv][col] = m_run;
@@ -201,7 +192,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
         }
         __syncthreads();
         const bool whole = j0 == 0 && j1 == count;
-        write_part<HD>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o);
+        write_part<HD, SPLIT, PRE>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o, ahead);
         if constexpr (!SPLIT) return;
         // where this part begins a task: how many other work-groups have the rest (the last is the one whose share holds the
         // task's last page)
@@ -220,7 +211,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) 
     }
 }
 
-// The parts of a task that lie in several shares: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A work-group takes NR of
+// The parts of a task that lie in several shares, and those of a prefix: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A work-group takes NR of
 // the task's heads; a thread four dims of a head, of every (kBlock / (NR HD / 4))-th part.
 template <int HD, int NR>
 __global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams P) {
@@ -229,13 +220,17 @@ __global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams
     __shared__ float s_l[NR][NC];
     const int tasks = P.n_kv * P.n_rowblk, b = blockIdx.x / tasks, task = blockIdx.x % tasks;
     const PagedAttnSplit d = P.split[blockIdx.x];
-    if (d.more == 0) return;
+    if (d.more == 0 && P.n_pre == 0) return;
     const int tid = threadIdx.x, dq = tid % NQ, rl = tid / NQ % NR, cl = tid / (NQ * NR);
     const int grp = P.n_head / P.n_kv, g = task % P.n_kv, rb = task / P.n_kv;
-    const int n = d.more + 1, rows = min(grp, 16);
+    const int own = d.more == 0 ? 0 : d.more + 1, n = own + P.n_pre + (d.more == 0), rows = min(grp, 16); // (a whole task: behind the prefix's)
     const float *rest = P.part + 2 * (int64_t) d.wg * rows * (HD + 4), *first = rest + (int64_t) rows * (HD + 4);
     const int r = blockIdx.y * NR + rl;
-    auto part = [&](int c) { return (c == 0 ? first : rest + (int64_t) c * 2 * rows * (HD + 4)) + min(r, rows - 1) * (HD + 4); };
+    const float *pre = P.pre + ((int64_t) b * P.n_head + g * grp + min(rb * 16 + r, grp - 1)) * (HD + 4);
+    auto part = [&](int c) {
+        if (c >= own) return pre + (int64_t) (c - own) * P.n_seq * P.n_head * (HD + 4);
+        return (c == 0 ? first : rest + (int64_t) c * 2 * rows * (HD + 4)) + min(r, rows - 1) * (HD + 4);
+    };
     float m = kLowest, l = 0.0f;
     float4 a = make_float4(0, 0, 0, 0);
     for (int c0 = cl; c0 < n; c0 += kAhead * NC) {
@@ -305,11 +300,9 @@ __global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams
 template <int HD>
 hipError_t launch_paged_attn_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
     const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
-    if (P.n_pre > 0)
-        return P.n_wg > 0 ? launch(paged_attn_kernel<HD, true, true>, all, block, 0, st, tm, P)
-                          : launch(paged_attn_kernel<HD, false, true>, all, block, 0, st, tm, P);
-    return P.n_wg > 0 ? launch(paged_attn_kernel<HD, true, false>, all, block, 0, st, tm, P)
-                      : launch(paged_attn_kernel<HD, false, false>, all, block, 0, st, tm, P);
+    if (P.n_wg > 0) return launch(paged_attn_kernel<HD, true, false>, all, block, 0, st, tm, P);
+    return P.n_pre > 0 ? launch(paged_attn_kernel<HD, false, true>, all, block, 0, st, tm, P)
+                       : launch(paged_attn_kernel<HD, false, false>, all, block, 0, st, tm, P);
 }
 
 template <int HD>
@@ -356,7 +349,7 @@ hipError_t launch_paged_attn(const PagedAttnParams &P, hipStream_t st, const Lau
 }
 
 hipError_t launch_paged_attn_join(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
-    if (P.n_wg <= 1) return hipSuccess;
+    if (P.n_wg == 0 || (P.n_wg == 1 && P.n_pre == 0)) return hipSuccess;
     switch (P.hd) {
     case 64: return launch_paged_attn_join_hd<64>(P, st, tm);
     case 128: return launch_paged_attn_join_hd<128>(P, st, tm);

@@ -149,16 +149,6 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
         };
         int ids = look_up(lane), id = __builtin_amdgcn_readlane(ids, 0);
         if (n_page > 0) load_k(id);
-        if constexpr (PRE) {
-            if (j0 == 0)
-                take_prefix<HD>(P, b, g * grp + min(row, grp - 1), wv, g4 == 0, m_run, l_run, [&](const float *part, float f, float e) {
-#pragma unroll
-                    for (int t = 0; t < 2 * NM; t++) {
-                        const float4 x = *reinterpret_cast<const float4 *>(part + 16 * t + 4 * g4);
-                        o[t] = o[t] * f + float4v{x.x, x.y, x.z, x.w} * e;
-                    }
-                });
-        }
         __syncthreads();
         for (int it = 0; it < n_page; it++) {
             const char *rec = record(id);
@@ -240,6 +230,8 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
             }
         }
 
+        PrefixParts<HD> ahead;
+        if constexpr (PRE) ask_first(P, b, g, rb, ahead);
         // the wavefronts' shares at one maximum
         l_run = across_groups_sum(l_run);
         if (g4 == 0) s_m[wv][col] = m_run;
@@ -254,7 +246,7 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
             *reinterpret_cast<float4 *>(&s_o[wv][col][16 * t + 4 * g4]) = make_float4(o[t][0] * f, o[t][1] * f, o[t][2] * f, o[t][3] * f);
         __syncthreads();
         const bool whole = j0 == 0 && j1 == count;
-        write_part<HD>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o);
+        write_part<HD, SPLIT, PRE>(P, b, g, rb, j0 == 0, whole, s_m, s_l, s_o, ahead);
         if constexpr (!SPLIT) return;
         if (tid == 0 && j0 == 0) {
             const int64_t last = min(share.each * (blockIdx.x + 1), share.total) - share.left + count - 1;
@@ -274,11 +266,9 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
 template <int HD>
 hipError_t launch_paged_attn_q8_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
     const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
-    if (P.n_pre > 0)
-        return P.n_wg > 0 ? launch(paged_attn_q8_kernel<HD, true, true>, all, block, 0, st, tm, P)
-                          : launch(paged_attn_q8_kernel<HD, false, true>, all, block, 0, st, tm, P);
-    return P.n_wg > 0 ? launch(paged_attn_q8_kernel<HD, true, false>, all, block, 0, st, tm, P)
-                      : launch(paged_attn_q8_kernel<HD, false, false>, all, block, 0, st, tm, P);
+    if (P.n_wg > 0) return launch(paged_attn_q8_kernel<HD, true, false>, all, block, 0, st, tm, P);
+    return P.n_pre > 0 ? launch(paged_attn_q8_kernel<HD, false, true>, all, block, 0, st, tm, P)
+                       : launch(paged_attn_q8_kernel<HD, false, false>, all, block, 0, st, tm, P);
 }
 
 }  // namespace

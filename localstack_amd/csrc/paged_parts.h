@@ -149,63 +149,94 @@ __device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, K
     return s;
 }
 
-// What a work-group's wavefronts have of a part of a task, in LDS at one maximum: the whole task goes to `out`, a part of it to
-// `part`. A part that continues one of the work-group before goes to the first of the work-group's two places, one that begins a
-// task to the second.
+// What parts of a prefix left (P.pre) for four dims of a head, kPreAhead parts at a time.
+constexpr int kPreAhead = 4;
 template <int HD>
+struct PrefixParts {
+    float2 ml[kPreAhead];
+    float4v o[kPreAhead];
+    __device__ __forceinline__ void ask(const PagedAttnParams &P, int64_t head, int d, int c0) {
+#pragma unroll
+        for (int i = 0; i < kPreAhead; i++) {
+            const float *p = P.pre + ((int64_t) min(c0 + i, P.n_pre - 1) * P.n_seq * P.n_head + head) * (HD + 4);
+            ml[i] = *reinterpret_cast<const float2 *>(p);
+            o[i] = *reinterpret_cast<const float4v *>(p + 4 + d);
+        }
+    }
+    // Joined to sums l and a at maximum m.
+    __device__ __forceinline__ void join(const PagedAttnParams &P, int c0, float &m, float &l, float4v &a) const {
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kPreAhead; i++) top = fmaxf(top, ml[i].x);
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= f;
+        a *= f;
+#pragma unroll
+        for (int i = 0; i < kPreAhead; i++) {
+            const float e = c0 + i < P.n_pre ? __builtin_amdgcn_exp2f(ml[i].x - m) : 0.0f;
+            if (c0 + i < P.n_pre) { // (a part that is there twice may hold NaN)
+                l = fmaf(ml[i].y, e, l);
+#pragma unroll
+                for (int j = 0; j < 4; j++) a[j] = fmaf(o[i][j], e, a[j]);
+            }
+        }
+    }
+};
+
+// What a work-group's wavefronts have of a part of a task, in LDS at one maximum, goes to `out` if it is the whole task, otherwise to
+// `part`. A part that continues one of the work-group before goes to the first of the work-group's two places, one that begins a
+// task to the second; a whole task that a prefix belongs to goes behind the prefix's parts. With PRE the parts of a prefix are joined
+// to the task before; `ahead` holds the first of them for the thread's first place.
+template <int HD, bool SPLIT, bool PRE>
 __device__ __forceinline__ void write_part(const PagedAttnParams &P, int b, int g, int rb, bool begins, bool whole, const float (*s_m)[16],
-                                           const float (*s_l)[16], const float (*s_o)[16][HD + 4]) {
+                                           const float (*s_l)[16], const float (*s_o)[16][HD + 4], PrefixParts<HD> &ahead) {
     const int grp = P.n_head / P.n_kv, rows = min(grp, 16);
     const int64_t place = 2 * (int64_t) blockIdx.x + (begins ? 1 : 0);
     for (int i = threadIdx.x; i < 16 * (HD / 4); i += kPaWaves * kWave) {
         const int r = i / (HD / 4), d = 4 * (i % (HD / 4));
         if (rb * 16 + r >= grp) continue;
-        float4 a = *reinterpret_cast<const float4 *>(&s_o[0][r][d]);
+        const int64_t head = (int64_t) b * P.n_head + g * grp + rb * 16 + r;
+        float4v a = *reinterpret_cast<const float4v *>(&s_o[0][r][d]);
         float l = s_l[0][r];
 #pragma unroll
         for (int w = 1; w < kPaWaves; w++) {
-            const float4 e = *reinterpret_cast<const float4 *>(&s_o[w][r][d]);
-            a.x += e.x;
-            a.y += e.y;
-            a.z += e.z;
-            a.w += e.w;
+            a += *reinterpret_cast<const float4v *>(&s_o[w][r][d]);
             l += s_l[w][r];
         }
-        if (whole) {
+        float m = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < kPaWaves; w++) m = fmaxf(m, s_m[w][r]);
+        if constexpr (PRE) {
+            for (int c0 = 0; c0 < P.n_pre; c0 += kPreAhead) {
+                if (c0 > 0 || i != (int) threadIdx.x) ahead.ask(P, head, d, c0);
+                ahead.join(P, c0, m, l, a);
+            }
+        }
+        const bool behind = SPLIT && whole && P.n_pre > 0;
+        if (!SPLIT || (whole && !behind)) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l; // no visible cell: zeros
             ushort4 h;
             h.x = __half_as_ushort(__float2half_rn(a.x * inv));
             h.y = __half_as_ushort(__float2half_rn(a.y * inv));
             h.z = __half_as_ushort(__float2half_rn(a.z * inv));
             h.w = __half_as_ushort(__float2half_rn(a.w * inv));
-            *reinterpret_cast<ushort4 *>(P.out + ((int64_t) b * P.n_head + g * grp + rb * 16 + r) * HD + d) = h;
+            *reinterpret_cast<ushort4 *>(P.out + head * HD + d) = h;
         } else {
-            float *dst = P.part + (place * rows + r) * (HD + 4);
-            *reinterpret_cast<float4 *>(dst + 4 + d) = a;
+            float *dst = behind ? P.pre + ((int64_t) P.n_pre * P.n_seq * P.n_head + head) * (HD + 4) : P.part + (place * rows + r) * (HD + 4);
+            *reinterpret_cast<float4v *>(dst + 4 + d) = a;
             if (d == 0) {
-                float m = s_m[0][r];
-#pragma unroll
-                for (int w = 1; w < kPaWaves; w++) m = fmaxf(m, s_m[w][r]);
                 dst[0] = m;
                 dst[1] = l;
             }
         }
     }
 }
-
-// A wavefront's share of the parts that a prefix left for head h of sequence b (P.pre): every kPaWaves-th, as if they were pages
-// that it has been through. merge(o, f, e): the lane's own sums times f plus e times the part's, which are at o. `l_run` is of the lane's cells
-// only, so one of the four lanes of a head has the parts' sums.
-template <int HD, typename F>
-__device__ __forceinline__ void take_prefix(const PagedAttnParams &P, int b, int h, int wv, bool sums, float &m_run, float &l_run, F &&merge) {
-    for (int c = wv; c < P.n_pre; c += kPaWaves) {
-        const float *p = P.pre + ((int64_t) c * P.n_seq * P.n_head + (int64_t) b * P.n_head + h) * (HD + 4);
-        const float2 ml = *reinterpret_cast<const float2 *>(p);
-        const float top = fmaxf(m_run, ml.x), f = __builtin_amdgcn_exp2f(m_run - top), e = __builtin_amdgcn_exp2f(ml.x - top);
-        m_run = top;
-        l_run = l_run * f + (sums ? ml.y * e : 0.0f);
-        merge(p + 4, f, e);
-    }
+// The first parts of a prefix for a thread's first place in write_part, asked for before the wavefronts meet.
+template <int HD>
+__device__ __forceinline__ void ask_first(const PagedAttnParams &P, int b, int g, int rb, PrefixParts<HD> &ahead) {
+    const int grp = P.n_head / P.n_kv, r = threadIdx.x / (HD / 4);
+    if (rb * 16 + r < grp) ahead.ask(P, (int64_t) b * P.n_head + g * grp + rb * 16 + r, 4 * (threadIdx.x % (HD / 4)), 0);
 }
 
 }  // namespace

@@ -331,7 +331,7 @@ size_t prefix_attn_plan(PrefixAttnParams &P) {
     // a work-group a CU, with two turns of its wavefronts' pages at least
     const int64_t most = std::max<int64_t>(1, kPaCus / ((int64_t) P.n_rowblk * P.n_kv));
     P.n_chunk = (int) std::max<int64_t>(1, std::min(most, pages / (2 * waves)));
-    return (size_t) P.n_chunk * P.n_seq * P.n_head * (P.hd + 4) * sizeof(float);
+    return (size_t) (P.n_chunk + 1) * P.n_seq * P.n_head * (P.hd + 4) * sizeof(float);
 }
 
 hipError_t launch_prefix_attn(const PrefixAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
