@@ -161,7 +161,7 @@ int cache_rows(const lstk_q8_cache *cache, const void *d_k, const void *d_v, int
     if (type != LSTK_TYPE_F16 && type != LSTK_TYPE_F32) return bad("rows must be of LSTK_TYPE_F16 or LSTK_TYPE_F32");
     const int64_t least = writes_rows && n_rows > 1 ? (int64_t) cache->n_head_kv * cache->head_dim : 0;
     if (ld_k < least || ld_v < least || ld_k % 8 || ld_v % 8) return bad("ld_k and ld_v must be multiples of 8, and hold a row where rows are written");
-    if ((int64_t) (n_rows / 32 + 1) * cache->n_head_kv > kMostGrid) return bad("too many rows for one launch");
+    if ((int64_t) ((n_rows + 38) / 32) * cache->n_head_kv > kMostGrid) return bad("too many rows for one launch");
     if (n_rows == 0) return LSTK_OK;
     if (!d_k || !d_v || !d_cells) return bad("null argument");
     if (!aligned(d_k, 16) || !aligned(d_v, 16) || !aligned(d_cells, 4)) return bad("k and v must be 16-byte aligned, cells 4-byte");

@@ -6,8 +6,9 @@
 // d / 2. The 32-bit quotient only guesses q; the remainder x - q d is exact in one fma and settles it.
 //
 // Bound by memory, and by the launch for the rows of a decode step. A work-group takes kCrRows rows of a KV head: the whole numbers
-// meet in LDS, because a row of V is single bytes 16 apart in its record: where the work-group's rows fill an octet of cells, as
-// the rows of a prompt do, they leave as 8 bytes at a time.
+// meet in LDS, because a row of V is single bytes 16 apart in its record. Where 8 rows fill an octet of cells, as the rows of a
+// prompt do, a thread turns 4 dims of the 8 rows over in registers and moves 8 bytes a dim; the work-groups' rows are shifted so
+// that the first row's octet (and with it those of the rows behind it in a prompt) begins with a work-group's rows.
 #include "cache_q8.h"
 #include "device.h"
 
@@ -21,117 +22,159 @@ constexpr float kMostMost = 65504.0f * 127.0f; // of a block that a finite d can
 struct Cells {
     int cell[kCrRows], octet[kCrRows]; // cell: -1 outside the cache
 };
-__device__ __forceinline__ void look_up_cells(const CacheRowsParams &P, Cells &C, int row0, int n) {
+__device__ __forceinline__ void look_up_cells(const CacheRowsParams &P, Cells &C, int row0) {
     const int i = threadIdx.x;
     if (i < kCrRows) {
-        const int c = i < n ? P.cells[row0 + i] : -1;
+        const int c = row0 + i >= 0 && row0 + i < P.n ? P.cells[row0 + i] : -1;
         C.cell[i] = c >= 0 && c < P.n_cells ? c : -1;
     }
     __syncthreads();
     if (i < kCrRows) {
         const int c = C.cell[i], first = i - (c & 7);
-        bool full = c >= 0 && first >= 0 && first + 8 <= n;
+        bool full = c >= 0 && first >= 0 && first + 8 <= kCrRows;
         for (int k = 0; k < 8 && full; k++) full = C.cell[first + k] == c - (c & 7) + k;
         C.octet[i] = full ? (first == i ? 1 : 2) : 0;
     }
     __syncthreads();
 }
+// The first of a work-group's rows; may be below 0.
+__device__ __forceinline__ int first_row(const CacheRowsParams &P) { return (int) (blockIdx.x / P.n_kv) * kCrRows - (P.cells[0] & 7); }
+// Four 4-byte words as the rows of a 4 x 4 matrix of bytes, turned over.
+__device__ __forceinline__ void turn_over(unsigned (&w)[4]) {
+    const unsigned a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u),
+                   c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
 __device__ __forceinline__ uint8_t *record_of(const CacheRowsParams &P, int cell, int g) {
     return P.cache + ((int64_t) (cell / kPageCells) * P.n_kv + g) * q8_record(P.hd);
 }
 
-// Four neighbouring dims of a row, as 32-bit values.
+// 16 bytes of a row, as 32-bit values: N = 4 or 8 dims.
 template <typename T>
-__device__ __forceinline__ float4 four(const T *p) {
-    if constexpr (sizeof(T) == 4) {
-        return *reinterpret_cast<const float4 *>(p);
-    } else {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        return make_float4(h2f(u.x), h2f(u.x >> 16), h2f(u.y), h2f(u.y >> 16));
+constexpr int kDims = 16 / (int) sizeof(T);
+template <typename T>
+__device__ __forceinline__ void values_of(const uint4 &u, float (&x)[kDims<T>]) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[2 * i] = h2f(w[i]);
+            x[2 * i + 1] = h2f(w[i] >> 16);
+        }
     }
 }
 template <typename T>
-__device__ __forceinline__ void put_four(T *p, float4 v) {
-    if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = v;
-    } else {
-        ushort4 h;
-        h.x = __half_as_ushort(__float2half_rn(v.x));
-        h.y = __half_as_ushort(__float2half_rn(v.y));
-        h.z = __half_as_ushort(__float2half_rn(v.z));
-        h.w = __half_as_ushort(__float2half_rn(v.w));
-        *reinterpret_cast<ushort4 *>(p) = h;
+__device__ __forceinline__ void put_values(T *p, const float (&x)[kDims<T>]) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
+        else w[i] = (unsigned) __half_as_ushort(__float2half_rn(x[2 * i])) | (unsigned) __half_as_ushort(__float2half_rn(x[2 * i + 1])) << 16;
     }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// x / d to the nearest whole number, halves to the even one; |x| <= 127 d.
-__device__ __forceinline__ int whole_of(float x, float d, float inv) {
-    float q = rintf(x * inv);                              // within one of it
-    const float rest = fmaf(-q, d, x), half = 0.5f * d;    // exact: a whole number of bits of x or of d, below 2 d
-    const bool odd = ((int) q & 1) != 0;
-    if (rest > half || (rest == half && odd)) q += 1.0f;
-    else if (rest < -half || (rest == -half && odd)) q -= 1.0f;
-    return (int) q;
+// x / d to the nearest whole numbers, halves to the even one; |x| <= 127 d.
+template <int N>
+__device__ __forceinline__ void whole_of(const float (&x)[N], float d, float inv, int (&q)[N]) {
+    float r[N], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        r[i] = rintf(x[i] * inv);                       // within one of it, and it unless the remainder is nearly d / 2
+        far = fmaxf(far, fabsf(fmaf(-r[i], d, x[i])));
+    }
+    if (far >= 0.4999f * d) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float rest = fmaf(-r[i], d, x[i]), half = 0.5f * d; // exact: a whole number of bits of x or of d, below 2 d
+            const bool odd = ((int) r[i] & 1) != 0;
+            if (rest > half || (rest == half && odd)) r[i] += 1.0f;
+            else if (rest < -half || (rest == -half && odd)) r[i] -= 1.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) q[i] = (int) r[i];
 }
 
 template <int HD, typename T>
 __global__ __launch_bounds__(kBlock) void cache_store_kernel(CacheRowsParams P) {
-    constexpr int NM = HD / kQ8Dims;
+    constexpr int NM = HD / kQ8Dims, N = kDims<T>, NL = kQ8Dims / N; // lanes of a block of 32 dims
     __shared__ Cells C;
     __shared__ uint32_t s_q[2][kCrRows][HD / 4 + 1]; // (+ 1: columns of V are read)
     __shared__ uint16_t s_d[2][kCrRows][NM];
-    const int g = blockIdx.x % P.n_kv, row0 = blockIdx.x / P.n_kv * kCrRows, n = min(kCrRows, P.n - row0), tid = threadIdx.x;
-    look_up_cells(P, C, row0, n);
-    // 8 lanes a block of 32 dims
-    for (int i = tid; i < n * NM * 2 * 8; i += kBlock) {
-        const int lane = i & 7, m = i / 8 % NM, r = i / (8 * NM) % n, kind = i / (8 * NM * n);
-        const T *src = static_cast<const T *>(kind ? P.v : P.k) + (row0 + r) * (kind ? P.ld_v : P.ld_k) + g * HD + 32 * m + 4 * lane;
-        const float4 x = four(src);
+    const int g = blockIdx.x % P.n_kv, row0 = first_row(P), tid = threadIdx.x;
+    // all of a thread's values are on their way while the cells are looked up
+    constexpr int kTurns = 2 * kCrRows * NM * NL / kBlock;
+    uint4 raw[kTurns];
+#pragma unroll
+    for (int t = 0; t < kTurns; t++) {
+        const int i = tid + t * kBlock, lane = i % NL, m = i / NL % NM, r = i / (NL * NM) % kCrRows, kind = i / (NL * NM * kCrRows);
+        const int row = min(max(row0 + r, 0), P.n - 1);
+        raw[t] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(kind ? P.v : P.k) + row * (kind ? P.ld_v : P.ld_k) + g * HD + 32 * m + N * lane);
+    }
+    look_up_cells(P, C, row0);
+#pragma unroll
+    for (int t = 0; t < kTurns; t++) {
+        const int i = tid + t * kBlock, lane = i % NL, m = i / NL % NM, r = i / (NL * NM) % kCrRows, kind = i / (NL * NM * kCrRows);
+        float x[N];
+        values_of<T>(raw[t], x);
         // the largest magnitude by its bits, so that infinities and NaN are larger than any number
-        unsigned most = max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu),
-                            max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
-        for (int d = 1; d < 8; d *= 2) most = max(most, (unsigned) __shfl_xor((int) most, d, kWave));
+        unsigned most = 0;
+#pragma unroll
+        for (int j = 0; j < N; j++) most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int d = 1; d < NL; d *= 2) most = max(most, (unsigned) __shfl_xor((int) most, d, kWave));
         unsigned bits = 0x7e00u; // NaN, for a block that holds one, an infinity or more than d can
-        uint32_t q = 0;
+        int q[N] = {};
         if (most <= __float_as_uint(kMostMost)) {
             const float a = __uint_as_float(most);
             bits = __half_as_ushort(__float2half_rn(a / 127.0f));
             if (h2f(bits) * 127.0f < a) bits++; // (19 bits: exact)
-            const float d = h2f(bits), inv = d == 0.0f ? 0.0f : 1.0f / d;
-            q = ((unsigned) whole_of(x.x, d, inv) & 0xffu) | ((unsigned) whole_of(x.y, d, inv) & 0xffu) << 8 |
-                ((unsigned) whole_of(x.z, d, inv) & 0xffu) << 16 | (unsigned) whole_of(x.w, d, inv) << 24;
+            const float d = h2f(bits);
+            whole_of(x, d, d == 0.0f ? 0.0f : 1.0f / d, q);
         }
-        s_q[kind][r][8 * m + lane] = q;
+#pragma unroll
+        for (int j = 0; j < N / 4; j++)
+            s_q[kind][r][8 * m + lane * (N / 4) + j] = (q[4 * j] & 0xff) | (q[4 * j + 1] & 0xff) << 8 | (q[4 * j + 2] & 0xff) << 16 | (unsigned) q[4 * j + 3] << 24;
         if (lane == 0) s_d[kind][r][m] = (uint16_t) bits;
     }
     __syncthreads();
     // K: 8 dims of a row
-    for (int i = tid; i < n * (HD / 8); i += kBlock) {
-        const int r = i % n, p = i / n, cell = C.cell[r];
+    for (int i = tid; i < kCrRows * (HD / 8); i += kBlock) {
+        const int r = i % kCrRows, p = i / kCrRows, cell = C.cell[r];
         if (cell < 0) continue;
         *reinterpret_cast<uint2 *>(record_of(P, cell, g) + q8_k(p / 4, cell % kPageCells, p % 4 * 8)) =
             make_uint2(s_q[0][r][2 * p], s_q[0][r][2 * p + 1]);
     }
-    // V: a dim of a row, or of 8 rows; lanes take neighbouring dims
-    for (int i = tid; i < n * HD; i += kBlock) {
-        const int r = i / HD, d = i % HD, cell = C.cell[r];
+    // V: 4 dims of a row, or of 8 rows
+    for (int i = tid; i < kCrRows * (HD / 4); i += kBlock) {
+        const int p = i % (HD / 4), r = i / (HD / 4), cell = C.cell[r];
         if (cell < 0 || C.octet[r] == 2) continue;
-        uint8_t *dst = record_of(P, cell, g) + q8_v(HD, d / 32, cell % kPageCells, d % 32);
-        auto byte = [&](int row) { return s_q[1][row][d / 4] >> (8 * (d & 3)) & 0xffu; };
+        uint8_t *dst = record_of(P, cell, g) + q8_v(HD, p / 8, cell % kPageCells, p % 8 * 4); // the dims behind it 16 apart
         if (C.octet[r] == 0) {
-            *dst = (uint8_t) byte(r);
+            const uint32_t w = s_q[1][r][p];
+#pragma unroll
+            for (int j = 0; j < 4; j++) dst[16 * j] = (uint8_t) (w >> (8 * j));
             continue;
         }
-        unsigned lo = 0, hi = 0;
+        unsigned lo[4], hi[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            lo |= byte(r + k) << (8 * k);
-            hi |= byte(r + 4 + k) << (8 * k);
+            lo[k] = s_q[1][r + k][p];
+            hi[k] = s_q[1][r + 4 + k][p];
         }
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
+        turn_over(lo);
+        turn_over(hi);
+#pragma unroll
+        for (int j = 0; j < 4; j++) *reinterpret_cast<uint2 *>(dst + 16 * j) = make_uint2(lo[j], hi[j]);
     }
-    for (int i = tid; i < n * NM * 2; i += kBlock) {
-        const int r = i % n, m = i / n % NM, kind = i / (n * NM), cell = C.cell[r];
+    for (int i = tid; i < 2 * kCrRows * NM; i += kBlock) {
+        const int r = i % kCrRows, m = i / kCrRows % NM, kind = i / (kCrRows * NM), cell = C.cell[r];
         if (cell < 0) continue;
         const int at = kind ? q8_v_scale(HD, m, cell % kPageCells) : q8_k_scale(HD, m, cell % kPageCells);
         *reinterpret_cast<uint16_t *>(record_of(P, cell, g) + at) = s_d[kind][r][m];
@@ -140,52 +183,67 @@ __global__ __launch_bounds__(kBlock) void cache_store_kernel(CacheRowsParams P) 
 
 template <int HD, typename T>
 __global__ __launch_bounds__(kBlock) void cache_load_kernel(CacheRowsParams P) {
-    constexpr int NM = HD / kQ8Dims;
+    constexpr int NM = HD / kQ8Dims, N = kDims<T>, NL = kQ8Dims / N;
     __shared__ Cells C;
     __shared__ uint32_t s_q[2][kCrRows][HD / 4 + 1];
     __shared__ uint16_t s_d[2][kCrRows][NM];
-    const int g = blockIdx.x % P.n_kv, row0 = blockIdx.x / P.n_kv * kCrRows, n = min(kCrRows, P.n - row0), tid = threadIdx.x;
-    look_up_cells(P, C, row0, n);
-    for (int i = tid; i < n * (HD / 8); i += kBlock) {
-        const int r = i % n, p = i / n, cell = C.cell[r];
-        uint2 u = make_uint2(0, 0);
-        if (cell >= 0) u = *reinterpret_cast<const uint2 *>(record_of(P, cell, g) + q8_k(p / 4, cell % kPageCells, p % 4 * 8));
-        s_q[0][r][2 * p] = u.x;
-        s_q[0][r][2 * p + 1] = u.y;
+    const int g = blockIdx.x % P.n_kv, row0 = first_row(P), tid = threadIdx.x;
+    look_up_cells(P, C, row0);
+    constexpr int kTurns = kCrRows * (HD / 8) / kBlock;
+    uint2 raw[kTurns];
+#pragma unroll
+    for (int t = 0; t < kTurns; t++) {
+        const int i = tid + t * kBlock, r = i % kCrRows, p = i / kCrRows, cell = C.cell[r];
+        raw[t] = make_uint2(0, 0);
+        if (cell >= 0) raw[t] = *reinterpret_cast<const uint2 *>(record_of(P, cell, g) + q8_k(p / 4, cell % kPageCells, p % 4 * 8));
     }
-    for (int i = tid; i < n * HD; i += kBlock) {
-        const int r = i / HD, d = i % HD, cell = C.cell[r];
+    for (int i = tid; i < kCrRows * (HD / 4); i += kBlock) {
+        const int p = i % (HD / 4), r = i / (HD / 4), cell = C.cell[r];
         if (C.octet[r] == 2) continue;
-        auto put = [&](int row, unsigned b) { reinterpret_cast<uint8_t *>(&s_q[1][row][0])[d] = (uint8_t) b; };
         if (cell < 0) {
-            put(r, 0);
+            s_q[1][r][p] = 0;
             continue;
         }
-        const uint8_t *src = record_of(P, cell, g) + q8_v(HD, d / 32, cell % kPageCells, d % 32);
+        const uint8_t *src = record_of(P, cell, g) + q8_v(HD, p / 8, cell % kPageCells, p % 8 * 4);
         if (C.octet[r] == 0) {
-            put(r, *src);
+            s_q[1][r][p] = (unsigned) src[0] | (unsigned) src[16] << 8 | (unsigned) src[32] << 16 | (unsigned) src[48] << 24;
             continue;
         }
-        const uint2 u = *reinterpret_cast<const uint2 *>(src);
+        unsigned lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(src + 16 * j);
+            lo[j] = u.x;
+            hi[j] = u.y;
+        }
+        turn_over(lo);
+        turn_over(hi);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            put(r + k, u.x >> (8 * k));
-            put(r + 4 + k, u.y >> (8 * k));
+            s_q[1][r + k][p] = lo[k];
+            s_q[1][r + 4 + k][p] = hi[k];
         }
     }
-    for (int i = tid; i < n * NM * 2; i += kBlock) {
-        const int r = i % n, m = i / n % NM, kind = i / (n * NM), cell = C.cell[r];
+    for (int i = tid; i < 2 * kCrRows * NM; i += kBlock) {
+        const int r = i % kCrRows, m = i / kCrRows % NM, kind = i / (kCrRows * NM), cell = C.cell[r];
         const int at = kind ? q8_v_scale(HD, m, cell % kPageCells) : q8_k_scale(HD, m, cell % kPageCells);
         s_d[kind][r][m] = cell < 0 ? 0 : *reinterpret_cast<const uint16_t *>(record_of(P, cell, g) + at);
     }
+#pragma unroll
+    for (int t = 0; t < kTurns; t++) {
+        const int i = tid + t * kBlock, r = i % kCrRows, p = i / kCrRows;
+        s_q[0][r][2 * p] = raw[t].x;
+        s_q[0][r][2 * p + 1] = raw[t].y;
+    }
     __syncthreads();
-    for (int i = tid; i < n * NM * 2 * 8; i += kBlock) {
-        const int lane = i & 7, m = i / 8 % NM, r = i / (8 * NM) % n, kind = i / (8 * NM * n);
-        const uint32_t q = s_q[kind][r][8 * m + lane];
+    for (int i = tid; i < 2 * kCrRows * NM * NL; i += kBlock) {
+        const int lane = i % NL, m = i / NL % NM, r = i / (NL * NM) % kCrRows, kind = i / (NL * NM * kCrRows), row = row0 + r;
+        if (row < 0 || row >= P.n) continue;
         const float d = h2f(s_d[kind][r][m]);
-        auto value = [&](int k) { return (float) (int8_t) (q >> (8 * k)) * d; };
-        T *dst = static_cast<T *>(const_cast<void *>(kind ? P.v : P.k)) + (row0 + r) * (kind ? P.ld_v : P.ld_k) + g * HD + 32 * m + 4 * lane;
-        put_four(dst, make_float4(value(0), value(1), value(2), value(3)));
+        float x[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = (float) (int8_t) (s_q[kind][r][8 * m + lane * (N / 4) + j / 4] >> (8 * (j % 4))) * d;
+        put_values(static_cast<T *>(const_cast<void *>(kind ? P.v : P.k)) + row * (kind ? P.ld_v : P.ld_k) + g * HD + 32 * m + N * lane, x);
     }
 }
 
@@ -199,7 +257,7 @@ hipError_t launch_load_hd(const CacheRowsParams &P, dim3 grid, hipStream_t st) {
     return P.f32 ? launch(cache_load_kernel<HD, float>, grid, dim3(kBlock), 0, st, nullptr, P)
                  : launch(cache_load_kernel<HD, uint16_t>, grid, dim3(kBlock), 0, st, nullptr, P);
 }
-dim3 rows_grid(const CacheRowsParams &P) { return dim3((unsigned) ((int64_t) ((P.n + kCrRows - 1) / kCrRows) * P.n_kv)); }
+dim3 rows_grid(const CacheRowsParams &P) { return dim3((unsigned) ((int64_t) ((P.n + 7 + kCrRows - 1) / kCrRows) * P.n_kv)); }
 
 }  // namespace
 
