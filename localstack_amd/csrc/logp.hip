@@ -6,7 +6,7 @@
 // A row is read once: a work-group holds a slice of it in registers (kLpThreads * HELD quads), so the maximum is known before the
 // sums are taken, and the largest values can be looked for afterwards. The n-th largest of the threads' own maxima is a bound
 // that the n largest values of the slice reach and few others do; those are gathered in LDS and put in order by counting. A row of
-// several slices is joined by a second launch, a wavefront a row.
+// several slices is joined by a second launch, a work-group a row.
 #include <cfloat>
 #include <type_traits>
 
@@ -22,7 +22,7 @@ constexpr int kLpThreads = 256, kLpWaves = kLpThreads / kWave;
 constexpr int kLpHeld = 16, kLpFew = 4; // quads of a thread
 constexpr int kLpSlices = 64;           // of a row: a lane each in the join
 constexpr int kLpList = 1024;
-constexpr int kLpTarget = 512;          // work-groups of a launch
+constexpr int kLpTarget = 4096;         // work-groups of a launch
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kFar = -1000.0f;        // e^kFar is 0: x - m of -inf, so that 0 times it stays 0
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ void answer(const LogpParams &P, int row, float m, do
     P.logp[row] = v > -INFINITY ? (float) ((double) v - (double) m - lse) : -INFINITY;
     if (P.entropy) P.entropy[row] = m > -INFINITY ? (float) (lse - t / l) : 0.0f;
 }
-__device__ __forceinline__ void alternative(const LogpParams &P, int row, int r, u64 place, float m, double lse) {
+__device__ __forceinline__ void alternative(const LogpParams &P, int row, int r, u64 place, float m, double lse) { // place 0: none
     const int64_t at = (int64_t) row * P.n_top + r;
     P.top_ids[at] = place == 0 ? -1 : (int32_t) ~(unsigned) place;
     P.top_logp[at] = place == 0 ? -INFINITY : (float) ((double) of_key((unsigned) (place >> 32)) - (double) m - lse);
@@ -131,11 +131,11 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
         s_t[wv] = t;
     }
     if (P.n_top > 0 && wv == 0) {
-        // the n-th largest of the threads' maxima, bit by bit
+        // the n-th largest of the threads' maxima, bit by bit; its upper 18 bits (2^-9 of it) let few more values through
         unsigned key[kLpWaves], bound = 0;
 #pragma unroll
         for (int w = 0; w < kLpWaves; w++) key[w] = key_of(s_max[w * kWave + lane]);
-        for (int bit = 31; bit >= 0; bit--) {
+        for (int bit = 31; bit >= 14; bit--) {
             const unsigned c = bound | 1u << bit;
             int n = 0;
 #pragma unroll
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
         else answer(P, row, m, L, T, lse);
     }
     if (P.n_top == 0) return;
-    const float bound = of_key(s_bound);
+    const float bound = s_bound > key_of(-INFINITY) ? of_key(s_bound) : -INFINITY; // (keys below are those of NaN)
 #pragma unroll
     for (int h = 0; h < HELD; h++)
 #pragma unroll
@@ -205,33 +205,66 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
     else alternative(P, row, tid, s_best[tid], m, m > -INFINITY ? log(L) : 0.0);
 }
 
-__global__ __launch_bounds__(kWave) void logp_join_kernel(LogpParams P) {
-    const int row = blockIdx.x, lane = threadIdx.x;
-    const int64_t part = (int64_t) row * P.slices + lane;
-    float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-    if (lane < P.slices) s = *reinterpret_cast<const float4 *>(P.sums + 4 * part);
-    const float m = wave_top(s.x);
-    double l = 0.0, t = 0.0;
-    if (s.x > -INFINITY) {
-        const double d = (double) s.x - (double) m, w = exp(d);
-        l = w * s.y;
-        t = w * s.z + d * l;
-    }
-    l = wave_sum_d(l);
-    t = wave_sum_d(t);
-    double lse = m > -INFINITY ? log(l) : 0.0;
-    if (lane == 0) answer(P, row, m, l, t, lse);
-    // the largest of the slices' next ones, one after the other
-    int at = 0;
-    u64 head = lane < P.slices && P.n_top > 0 ? P.best[part * P.n_top] : 0;
-    for (int r = 0; r < P.n_top; r++) {
-        const u64 top = wave_place_max(head);
-        if (lane == 0) alternative(P, row, r, top, m, lse);
-        if (head == top && top != 0) {
-            at++;
-            head = at < P.n_top ? P.best[part * P.n_top + at] : 0;
+__global__ __launch_bounds__(kLpThreads) void logp_join_kernel(LogpParams P) {
+    __shared__ u64 s_best[kLpSlices * kLogpMaxTop], s_left[kLpSlices * kLogpMaxTop], s_at[kLpSlices], s_bound;
+    __shared__ double s_lse;
+    __shared__ float s_m;
+    __shared__ int s_n;
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), n = P.n_top;
+    // the slices' lists are on their way while the sums are joined
+    constexpr int kEach = kLpSlices * kLogpMaxTop / kLpThreads;
+    u64 list[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; i++)
+        if (tid + i * kLpThreads < P.slices * n) list[i] = P.best[(int64_t) row * P.slices * n + tid + i * kLpThreads];
+    if (tid < kWave) {
+        float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (lane < P.slices) s = *reinterpret_cast<const float4 *>(P.sums + 4 * ((int64_t) row * P.slices + lane));
+        const float m = wave_top(s.x);
+        double l = 0.0, t = 0.0, lse;
+        if (s.x > -INFINITY) {
+            const double d = (double) s.x - (double) m, w = exp(d);
+            l = w * s.y;
+            t = w * s.z + d * l;
+        }
+        l = wave_sum_d(l);
+        t = wave_sum_d(t);
+        if (lane == 0) {
+            answer(P, row, m, l, t, lse);
+            s_lse = lse;
+            s_m = m;
+            s_n = 0;
         }
     }
+    if (n == 0) return;
+#pragma unroll
+    for (int i = 0; i < kEach; i++)
+        if (tid + i * kLpThreads < P.slices * n) s_best[tid + i * kLpThreads] = list[i];
+    __syncthreads();
+    // Element j of every slice's list, in order: the one that has q before it is no more than (q + 1) (j + 1) >= n_top values, so none
+    // below it is among the n_top largest. The few that are left are put in order by counting.
+    const int j = (n - 1) / P.slices, q = (n + j) / (j + 1) - 1;
+    const u64 at = tid < P.slices ? s_best[tid * n + j] : 0;
+    if (tid < kLpSlices) s_at[tid] = at;
+    __syncthreads();
+    if (tid < P.slices) {
+        int before = 0;
+        for (int i = 0; i < P.slices; i++) before += s_at[i] > at || (s_at[i] == at && i < tid);
+        if (before == q) s_bound = at;
+    }
+    __syncthreads();
+    const u64 bound = max(s_bound, (u64) 1);
+    for (int i = tid; i < P.slices * n; i += kLpThreads)
+        if (s_best[i] >= bound) s_left[atomicAdd(&s_n, 1)] = s_best[i]; // (in any order: they are counted)
+    __syncthreads();
+    const int left = s_n;
+    for (int i = tid; i < left; i += kLpThreads) {
+        const u64 place = s_left[i];
+        int r = 0;
+        for (int k = 0; k < left; k++) r += s_left[k] > place;
+        if (r < n) alternative(P, row, r, place, s_m, s_lse);
+    }
+    for (int r = left + tid; r < n; r += kLpThreads) alternative(P, row, r, 0, s_m, s_lse);
 }
 
 }  // namespace
@@ -239,7 +272,7 @@ __global__ __launch_bounds__(kWave) void logp_join_kernel(LogpParams P) {
 size_t logp_plan(LogpParams &P, void *work) {
     const int quads = (P.n_vocab + 6) / 4; // a row out of line has one more
     const int least = (quads + kLpHeld * kLpThreads - 1) / (kLpHeld * kLpThreads);
-    const int want = std::min(kLpTarget / std::max(1, P.n_rows), quads / (kLpFew * kLpThreads));
+    const int want = std::min(kLpTarget / std::max(1, P.n_rows), (quads + kLpFew * kLpThreads - 1) / (kLpFew * kLpThreads));
     P.slices = std::min(kLpSlices, std::max({1, least, want}));
     P.slice = (quads + P.slices - 1) / P.slices;
     if (P.slices == 1) return 0;
@@ -255,7 +288,7 @@ hipError_t launch_logp(const LogpParams &P, hipStream_t st) {
     const hipError_t e = P.slice <= kLpFew * kLpThreads ? launch(logp_slice_kernel<kLpFew>, all, block, 0, st, nullptr, P)
                                                         : launch(logp_slice_kernel<kLpHeld>, all, block, 0, st, nullptr, P);
     if (e != hipSuccess || P.slices == 1) return e;
-    return launch(logp_join_kernel, dim3((unsigned) P.n_rows), dim3(kWave), 0, st, nullptr, P);
+    return launch(logp_join_kernel, dim3((unsigned) P.n_rows), block, 0, st, nullptr, P);
 }
 
 }  // namespace lstk
