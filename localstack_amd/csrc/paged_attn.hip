@@ -24,8 +24,8 @@
 namespace lstk {
 namespace {
 
-// SPLIT: equal shares of the list; otherwise a task each. PRE: the parts of a prefix are joined to a task (SPLIT leaves that to the
-// launch that joins a task's own parts).
+// SPLIT: equal shares of the list; otherwise a task each. PRE: the parts of a prefix are joined to a task (otherwise a
+// later launch does it).
 template <int HD, bool SPLIT, bool PRE>
 __global__ __launch_bounds__(kPaWaves *kWave, HD == 64 ? 4 : HD == 128 ? 3 : 2) void paged_attn_kernel(PagedAttnParams P) {
     constexpr int NK = HD / 16, NM = HD / 32; // 16-byte K loads of a lane per page; matrix steps over the dims
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kBlock) void paged_attn_join_kernel(PagedAttnParams
     __shared__ __align__(16) float4 s_o[NR][NC][NQ];
     __shared__ float s_l[NR][NC];
     const int tasks = P.n_kv * P.n_rowblk, b = blockIdx.x / tasks, task = blockIdx.x % tasks;
-    const PagedAttnSplit d = P.split[blockIdx.x];
+    const PagedAttnSplit d = P.n_wg > 0 ? P.split[blockIdx.x] : PagedAttnSplit{0, 0};
     if (d.more == 0 && P.n_pre == 0) return;
     const int tid = threadIdx.x, dq = tid % NQ, rl = tid / NQ % NR, cl = tid / (NQ * NR);
     const int grp = P.n_head / P.n_kv, g = task % P.n_kv, rb = task / P.n_kv;
@@ -301,8 +301,8 @@ template <int HD>
 hipError_t launch_paged_attn_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
     const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
     if (P.n_wg > 0) return launch(paged_attn_kernel<HD, true, false>, all, block, 0, st, tm, P);
-    return P.n_pre > 0 ? launch(paged_attn_kernel<HD, false, true>, all, block, 0, st, tm, P)
-                       : launch(paged_attn_kernel<HD, false, false>, all, block, 0, st, tm, P);
+    return joins_at_once(P) ? launch(paged_attn_kernel<HD, false, true>, all, block, 0, st, tm, P)
+                            : launch(paged_attn_kernel<HD, false, false>, all, block, 0, st, tm, P);
 }
 
 template <int HD>
@@ -310,7 +310,7 @@ hipError_t launch_paged_attn_join_hd(const PagedAttnParams &P, hipStream_t st, c
     // a task of many parts takes a work-group per head, so that more threads share its parts (two sequences of 100000 tokens at
     // 64 heads in 96 parts a task: 9 us, 20 with four heads to a work-group; in 64 parts, as now, 6)
     const unsigned tasks = (unsigned) P.n_seq * P.n_kv * P.n_rowblk, rows = std::min(16, P.n_head / P.n_kv);
-    if ((int64_t) tasks * 4 <= P.n_wg) return launch(paged_attn_join_kernel<HD, 1>, dim3(tasks, rows), dim3(kBlock), 0, st, tm, P);
+    if ((int64_t) tasks * 4 <= P.n_wg + P.n_pre * (int64_t) tasks / 8) return launch(paged_attn_join_kernel<HD, 1>, dim3(tasks, rows), dim3(kBlock), 0, st, tm, P);
     return launch(paged_attn_join_kernel<HD, 4>, dim3(tasks, (rows + 3) / 4), dim3(kBlock), 0, st, tm, P);
 }
 
@@ -349,7 +349,7 @@ hipError_t launch_paged_attn(const PagedAttnParams &P, hipStream_t st, const Lau
 }
 
 hipError_t launch_paged_attn_join(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
-    if (P.n_wg == 0 || (P.n_wg == 1 && P.n_pre == 0)) return hipSuccess;
+    if (P.n_pre > 0 ? joins_at_once(P) : P.n_wg <= 1) return hipSuccess;
     switch (P.hd) {
     case 64: return launch_paged_attn_join_hd<64>(P, st, tm);
     case 128: return launch_paged_attn_join_hd<128>(P, st, tm);

@@ -267,8 +267,8 @@ template <int HD>
 hipError_t launch_paged_attn_q8_hd(const PagedAttnParams &P, hipStream_t st, const LaunchTiming *tm) {
     const dim3 block(kPaWaves * kWave), all(P.n_wg > 0 ? P.n_wg : (unsigned) P.n_seq * P.n_kv * P.n_rowblk);
     if (P.n_wg > 0) return launch(paged_attn_q8_kernel<HD, true, false>, all, block, 0, st, tm, P);
-    return P.n_pre > 0 ? launch(paged_attn_q8_kernel<HD, false, true>, all, block, 0, st, tm, P)
-                       : launch(paged_attn_q8_kernel<HD, false, false>, all, block, 0, st, tm, P);
+    return joins_at_once(P) ? launch(paged_attn_q8_kernel<HD, false, true>, all, block, 0, st, tm, P)
+                            : launch(paged_attn_q8_kernel<HD, false, false>, all, block, 0, st, tm, P);
 }
 
 }  // namespace

@@ -149,8 +149,10 @@ __device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, K
     return s;
 }
 
-// What parts of a prefix left (P.pre) for four dims of a head, kPreAhead parts at a time.
-constexpr int kPreAhead = 4;
+// What parts of a prefix left (P.pre) for four dims of a head, kPreAhead parts at a time. Up to kPreMost parts are joined where a task
+// is done, more of them (or where a task is done in parts) by the launch that joins parts: it has more threads for a head.
+constexpr int kPreAhead = 4, kPreMost = 8;
+__host__ __device__ inline bool joins_at_once(const PagedAttnParams &P) { return P.n_wg == 0 && P.n_pre > 0 && P.n_pre <= kPreMost; }
 template <int HD>
 struct PrefixParts {
     float2 ml[kPreAhead];
@@ -186,8 +188,8 @@ struct PrefixParts {
 
 // What a work-group's wavefronts have of a part of a task, in LDS at one maximum, goes to `out` if it is the whole task, otherwise to
 // `part`. A part that continues one of the work-group before goes to the first of the work-group's two places, one that begins a
-// task to the second; a whole task that a prefix belongs to goes behind the prefix's parts. With PRE the parts of a prefix are joined
-// to the task before; `ahead` holds the first of them for the thread's first place.
+// task to the second; a whole task whose prefix is joined later goes behind the prefix's parts. With PRE the parts of a prefix are
+// joined to the task before; `ahead` holds the first of them for the thread's first place.
 template <int HD, bool SPLIT, bool PRE>
 __device__ __forceinline__ void write_part(const PagedAttnParams &P, int b, int g, int rb, bool begins, bool whole, const float (*s_m)[16],
                                            const float (*s_l)[16], const float (*s_o)[16][HD + 4], PrefixParts<HD> &ahead) {
@@ -213,8 +215,8 @@ __device__ __forceinline__ void write_part(const PagedAttnParams &P, int b, int 
                 ahead.join(P, c0, m, l, a);
             }
         }
-        const bool behind = SPLIT && whole && P.n_pre > 0;
-        if (!SPLIT || (whole && !behind)) {
+        const bool behind = !PRE && whole && P.n_pre > 0;
+        if ((!SPLIT || whole) && !behind) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l; // no visible cell: zeros
             ushort4 h;
             h.x = __half_as_ushort(__float2half_rn(a.x * inv));

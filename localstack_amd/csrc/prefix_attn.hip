@@ -22,7 +22,9 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kPxRows = 32;   // query rows of a wavefront
 constexpr int kPxTiles = 4;   // wavefronts that share a page
-constexpr int kPxGroups = 2;  // pages at a time where they share
+// Groups of such wavefronts, a page at a time each. Head size 256 has one, with all registers of a SIMD to each wavefront.
+template <int HD>
+constexpr int px_groups() { return HD == 256 ? 1 : 2; }
 // The reference m lies kPxUnder below the row's largest score when it is set, and is set anew when a score lies more than kPxUnder +
 // kPxSlack above it: weights stay below 2^16, and fp16 holds those down to 2^-26 of the largest as normal numbers, to 2^-36 at all.
 constexpr float kPxUnder = 12.0f, kPxSlack = 3.9f;
@@ -33,11 +35,11 @@ __device__ __forceinline__ float16v mfma32(const half8v &a, const half8v &b, con
 __device__ __forceinline__ half8v pair(const uint2 &a, const uint2 &b) { return halves(a.x, a.y, b.x, b.y); }
 
 template <int HD, bool SHARED>
-constexpr int px_waves() { return SHARED ? kPxTiles * kPxGroups : HD == 256 ? 4 : 8; }
+constexpr int px_waves() { return SHARED ? kPxTiles * px_groups<HD>() : HD == 256 ? 4 : 8; }
 
 template <int HD, bool SHARED>
-__global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, SHARED || HD < 256 ? 2 : 1) void prefix_attn_kernel(PrefixAttnParams P) {
-    constexpr int W = px_waves<HD, SHARED>(), G = SHARED ? kPxGroups : W, NT = SHARED ? kPxTiles : 1; // page groups, row tiles
+__global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, HD < 256 ? 2 : 1) void prefix_attn_kernel(PrefixAttnParams P) {
+    constexpr int W = px_waves<HD, SHARED>(), G = SHARED ? px_groups<HD>() : W, NT = SHARED ? kPxTiles : 1; // page groups, row tiles
     constexpr int NS = HD / 16, ND = HD / 32;                                                        // steps over the dims; dim tiles
     constexpr int kBytes = HD * 64, kPages = SHARED && HD < 256 ? 2 : 1; // of K, and of V, of a page; pages of a turn
     // SHARED: [2 buffers][G][kPages][K | V]; then what W / 2 wavefronts have, [W / 2][HD / 4][32 rows] float4
@@ -326,11 +328,11 @@ size_t prefix_attn_plan(PrefixAttnParams &P) {
     P.n_chunk = P.n_rowblk = 0;
     if (pages == 0 || rows == 0) return 0;
     P.shared = rows > 2 * kPxRows;
-    const int tile = P.shared ? kPxRows * kPxTiles : kPxRows, waves = P.shared ? kPxGroups : P.hd == 256 ? 4 : 8;
+    const int tile = P.shared ? kPxRows * kPxTiles : kPxRows, groups = !P.shared ? (P.hd == 256 ? 4 : 8) : P.hd == 256 ? 1 : 2;
     P.n_rowblk = (int) ((rows + tile - 1) / tile);
-    // a work-group a CU, with two turns of its wavefronts' pages at least
+    // a work-group a CU, with two turns of its groups at least where they share pages, and a page for each wavefront where not
     const int64_t most = std::max<int64_t>(1, kPaCus / ((int64_t) P.n_rowblk * P.n_kv));
-    P.n_chunk = (int) std::max<int64_t>(1, std::min(most, pages / (2 * waves)));
+    P.n_chunk = (int) std::max<int64_t>(1, std::min(most, pages / (P.shared ? 4 * groups : groups)));
     return (size_t) (P.n_chunk + 1) * P.n_seq * P.n_head * (P.hd + 4) * sizeof(float);
 }
 
