@@ -1053,17 +1053,26 @@ class Qwen3Model:
         return self._batch_call(n_seq, logits, trace, stream, lambda out, tr, st: lib().lstk_model_forward_batch(
             self._h, n_seq, max_len, window, n_sink, out, tr, st))
 
-    def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0):
+    def generate(self, prompts, n_new, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None, window=0, n_sink=0,
+                 logprobs=None):
         """Continues several sequences together: prompts is {seq: token ids}, each is decoded (appended to what seq holds), then
         n_new tokens are sampled for all of them, a batch step each. Returns {seq: the n_new tokens}; the last is not appended.
         The settings are numbers, or sequences with one per prompt; generator: a torch generator on the model's device. Arguments
         are checked before anything is appended; where a later step fails (no room in the cache, a sequence without a finite
-        logit) every sequence is cut back to what it held before."""
+        logit) every sequence is cut back to what it held before.
+        logprobs: None, or how many alternatives (0 to 32) to report; then the result is ({seq: tokens}, {seq: a dict for each token}) with
+        the token's "logprob" under softmax of the logits (no temperature, no cut), their "entropy", and "top", the largest logits'
+        (id, log probability) (token_logprobs)."""
         import torch
         seqs = _ids32(list(prompts), "sequences").tolist()
         n, V = len(seqs), self.hp["n_vocab"]
+        if logprobs is not None:
+            logprobs = _i32(logprobs, "logprobs")
+            if not 0 <= logprobs <= 32 or V > 2 ** 20 - 16:
+                raise LstkError(E_INVALID, "logprobs must be in [0, 32], for a vocabulary of at most 2^20 - 16")
         if n == 0 or n_new <= 0:
-            return {s: [] for s in seqs}
+            none = {s: [] for s in seqs}
+            return none if logprobs is None else (none, {s: [] for s in seqs})
         if n > self.n_batch:
             raise LstkError(E_INVALID, f"{n} sequences in a model of {self.n_batch} tokens a step")
         if min(seqs) < 0:
@@ -1095,10 +1104,13 @@ class Qwen3Model:
                 logits = torch.empty(n, V, dtype=torch.float32, device=self.device)
                 for i, s in enumerate(seqs):
                     self.decode(s, tokens[s], logits=logits[i])
-                got = []
+                got, said = [], []
                 for i in range(n_new):
                     u = torch.rand(n, device=self.device, generator=generator)
-                    t = sample(logits, u, **how)[0].cpu().numpy()
+                    drawn = sample(logits, u, **how)[0]
+                    if logprobs is not None:
+                        said.append([x.tolist() for x in token_logprobs(logits, drawn, n_top=logprobs)])
+                    t = drawn.cpu().numpy()
                     if t.min() < 0:
                         raise LstkError(E_INVALID, f"sequence {seqs[int(t.argmin())]} has no finite logit at new token {i}")
                     got.append(t)
@@ -1112,7 +1124,11 @@ class Qwen3Model:
                 except LstkError:
                     pass  # the first error is the one to report
             raise
-        return {s: [int(t[i]) for t in got] for i, s in enumerate(seqs)}
+        tokens = {s: [int(t[i]) for t in got] for i, s in enumerate(seqs)}
+        if logprobs is None:
+            return tokens
+        return tokens, {s: [dict(logprob=of[i], entropy=ent[i], top=[(a, p) for a, p in zip(ids[i], at[i]) if a >= 0])
+                            for of, ent, ids, at in said] for i, s in enumerate(seqs)}
 
     def fill_context(self, seq, n_cells, seed=0, stream=None):
         """Appends n_cells synthetic positions (seeded random K/V, no tokens run) to sequence seq."""
