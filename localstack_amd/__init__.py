@@ -543,6 +543,14 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     return tokens, probs
 
 
+def _out(given, name, dtype, shape, dev, stream):
+    """(tensor, pointer) of the caller's output, or of a new one."""
+    if given is None:
+        given = _empty(shape, dtype, dev, stream)
+        return given, given.data_ptr()
+    return given, _tensor(given, name, dtype, shape, dev)
+
+
 def q8_cache_shape(n_cells, n_head_kv, head_dim):
     """Shape of the uint8 tensor that holds n_cells cells (rounded up to whole pages of 32) of K and V in 8 bits (lstk_q8_cache,
     include/lstk_qwen3.h)."""
@@ -615,12 +623,17 @@ def load_q8(cache, cells, dtype=None, k=None, v=None, stream=None):
         dtype = torch.float16 if k is None else getattr(k, "dtype", None)
     kind = _rows_type(dtype)
     shape = (n, c.n_head_kv, c.head_dim)
+    row = c.n_head_kv * c.head_dim
     if k is None:
         k = _empty(shape, dtype, dev, stream)
+        kp, ldk = k.data_ptr(), row
+    else:
+        kp, ldk = _cache_rows(k, "k", *shape, dtype, dev)
     if v is None:
         v = _empty(shape, dtype, dev, stream)
-    kp, ldk = _cache_rows(k, "k", *shape, dtype, dev)
-    vp, ldv = _cache_rows(v, "v", *shape, dtype, dev)
+        vp, ldv = v.data_ptr(), row
+    else:
+        vp, ldv = _cache_rows(v, "v", *shape, dtype, dev)
     _check(_on_device(dev, stream, lambda st: lib().lstk_cache_q8_load(ctypes.byref(c), kp, vp, kind, ldk, ldv, at, n, st)))
     return k, v
 
@@ -656,9 +669,7 @@ def paged_attention_q8(q, cache, lens, first, blocks, max_len, window=0, n_sink=
     if not (0 <= window <= _MOST and 0 <= n_sink <= _MOST):
         _check_i32(window=window, n_sink=n_sink)
     s = _own_seqs(n, lens, first, blocks, max_len, seqs, dev)
-    if out is None:
-        out = _empty(shape, torch.float16, dev, stream)
-    op = _tensor(out, "out", torch.float16, shape, dev)
+    out, op = _out(out, "out", torch.float16, shape, dev, stream)
     need = 0 if work is not None else lib().lstk_attn_paged_q8_work_bytes(n, H, c.n_head_kv, hd, s.max_len, window, n_sink)
     wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
     f = float(hd ** -0.5 if scale is None else scale)
@@ -698,9 +709,7 @@ def _shared(call, q, qp, prefix, cache, s, scale, out, work, stream):
     dev = q.get_device()
     if prefix.device != dev:
         raise LstkError(E_INVALID, f"the prefix is on GPU {prefix.device}, q on GPU {dev}")
-    if out is None:
-        out = _empty(shape, torch.float16, dev, stream)
-    op = _tensor(out, "out", torch.float16, shape, dev)
+    out, op = _out(out, "out", torch.float16, shape, dev, stream)
     need = 0 if work is not None else lib().lstk_attn_shared_work_bytes(n, H, cache.n_head_kv, hd, s.max_len, prefix.c.max_len)
     wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
     f = float(hd ** -0.5 if scale is None else scale)
@@ -754,16 +763,10 @@ def token_logprobs(logits, tokens, n_top=0, logprobs=None, entropy=None, top_ids
         _check_i32(n_rows=n, n_vocab=V, n_top=n_top)
     tp = _tensor(tokens, "tokens", i32, (n,), dev)
     shape, tops = (n,), (n, max(n_top, 0))
-    if logprobs is None:
-        logprobs = _empty(n, f32, dev, stream)
-    if entropy is None:
-        entropy = _empty(n, f32, dev, stream)
-    if top_ids is None:
-        top_ids = _empty(tops, i32, dev, stream)
-    if top_logprobs is None:
-        top_logprobs = _empty(tops, f32, dev, stream)
-    lp, ep = _tensor(logprobs, "logprobs", f32, shape, dev), _tensor(entropy, "entropy", f32, shape, dev)
-    ip, ap = _tensor(top_ids, "top_ids", i32, tops, dev), _tensor(top_logprobs, "top_logprobs", f32, tops, dev)
+    logprobs, lp = _out(logprobs, "logprobs", f32, shape, dev, stream)
+    entropy, ep = _out(entropy, "entropy", f32, shape, dev, stream)
+    top_ids, ip = _out(top_ids, "top_ids", i32, tops, dev, stream)
+    top_logprobs, ap = _out(top_logprobs, "top_logprobs", f32, tops, dev, stream)
     need = 0 if work is not None else lib().lstk_token_logprobs_work_bytes(n, V, n_top)
     wt, wp, wn = (None, None, 0) if work is None and need == 0 else _work(work, need, dev, stream)
     _check(_on_device(dev, stream, lambda st: lib().lstk_token_logprobs(p, ld, n, V, tp, n_top, lp, ep, ip, ap, wp, wn, st)))
