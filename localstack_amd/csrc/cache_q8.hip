@@ -9,6 +9,9 @@
 // meet in LDS, because a row of V is single bytes 16 apart in its record. Where 8 rows fill an octet of cells, as the rows of a
 // prompt do, a thread turns 4 dims of the 8 rows over in registers and moves 8 bytes a dim; the work-groups' rows are shifted so
 // that the first row's octet (and with it those of the rows behind it in a prompt) begins with a work-group's rows.
+// Measured on MI355X, 20000 rows of 4 heads of 128 in fp16 (63 MB in and out): store 21 us (36 with single bytes and rows where they
+// lie), load 18 us; 10 us would be HBM's. A work-group is a chain of waits (the first cell, the rows, LDS), and there are 1.2 rounds
+// of them.
 #include "cache_q8.h"
 #include "device.h"
 

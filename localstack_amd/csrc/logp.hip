@@ -3,6 +3,9 @@
 //   m = max x,  l = sum e^(x - m),  t = sum (x - m) e^(x - m)
 //   log p(i) = x_i - m - ln l,  entropy = ln l - t / l
 //
+// Bound by HBM where there are many rows: 1000 rows of 151936 values (608 MB) 97 us on MI355X, 6.3 TB/s, and 5 us for the join; 64 rows
+// with 20 values each 14 and 6 us, one row with 5 values 5.5 and 4.6 us, bound by waits.
+//
 // A row is read once: a work-group holds a slice of it in registers (kLpThreads * HELD quads), so the maximum is known before the
 // sums are taken, and the largest values can be looked for afterwards. The n-th largest of the threads' own maxima is a bound
 // that the n largest values of the slice reach and few others do; those are gathered in LDS and put in order by counting. A row of
