@@ -216,9 +216,9 @@ int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, 
  * (whole ones), but the prefix is read once for all rows. The prefix is the first *d_len cells (held in [0, max_len]) of the pages
  * d_blocks [n_table] of an fp16 cache; pages out of range are not visible. seqs describes the sequences' own cells, in an fp16 cache
  * (the same or another one) or a quantised one, by the rules of lstk_attn_paged without a window; prefix->cache->d_cell_seq must be NULL.
- * A row without a visible cell gets zeros. Over the prefix a weight is rounded to one fp16 part, good to 2^-11 (to 2^-37 of the
- * largest where it is below 2^-26 of it); sums are fp32. The workspace is as lstk_attn_paged's; one size serves both kinds of caches, and
- * smaller lengths and prefixes.
+ * A row without a visible cell gets zeros. A weight enters the sums (fp32) as two fp16 parts, over the prefix as over own cells: good to
+ * 2^-22 (over the prefix to 2^-37 of the largest where it is below 2^-15 of it). The workspace is as lstk_attn_paged's; one size serves
+ * both kinds of caches, and smaller lengths and prefixes.
  * Worth it from some 8 sequences and 1000 cells on: it takes a launch more than attention over lists that begin alike. */
 typedef struct lstk_prefix {
     const lstk_paged_cache *cache;

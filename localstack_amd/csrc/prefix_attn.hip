@@ -25,7 +25,6 @@ namespace lstk {
 namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kPxRows = 32;   // query rows of a wavefront
 constexpr int kPxTiles = 4;   // wavefronts that share a page
@@ -33,7 +32,8 @@ constexpr int kPxTiles = 4;   // wavefronts that share a page
 template <int HD>
 constexpr int px_groups() { return HD == 256 ? 1 : 2; }
 // The reference m lies kPxUnder below the row's largest score when it is set, and is set anew when a score lies more than kPxUnder +
-// kPxSlack above it: weights stay below 2^16, and fp16 holds those down to 2^-26 of the largest as normal numbers, to 2^-36 at all.
+// kPxSlack above it: weights stay below 2^16, the largest at 2^12 or more, so that half a step of fp16's subnormal numbers (2^-25) is
+// 2^-37 of it or less.
 constexpr float kPxUnder = 12.0f, kPxSlack = 3.9f;
 
 __device__ __forceinline__ float16v mfma32(const half8v &a, const half8v &b, const float16v &c) {
@@ -140,21 +140,26 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, HD < 256 ? 2 : 1)
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[n][i] = fmaf(s[n][i], scale, -m_run);
         }
-        // The weights enter the product in one fp16 part, and the sum as they enter it, so that they still add up to one.
+        // p = hi + lo in fp16 for the products, as over a sequence's own cells: to 2^-22 of each weight, or to 2^-37 of the largest where
+        // lo leaves fp16's normal numbers; the sum takes p itself.
 #pragma unroll
         for (int n = 0; n < NP; n++) {
-            float sum = 0.0f;
-            half8v p[2];
+            half8v hi[2], lo[2];
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[i / 8][i % 8] = (_Float16) __builtin_amdgcn_exp2f(s[n][i]);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2)
-                sum = __builtin_amdgcn_fdot2(half2v{p[i / 8][i % 8], p[i / 8][i % 8 + 1]}, half2v{(_Float16) 1.0f, (_Float16) 1.0f}, sum, false);
-            l_run += sum;
+            for (int i = 0; i < 16; i++) {
+                const float p = __builtin_amdgcn_exp2f(s[n][i]);
+                hi[i / 8][i % 8] = (_Float16) p;
+                lo[i / 8][i % 8] = (_Float16) (p - (float) hi[i / 8][i % 8]);
+                l_run += p;
+            }
 #pragma unroll
             for (int s2 = 0; s2 < 2; s2++)
 #pragma unroll
-                for (int t = 0; t < ND; t++) o[t] = mfma32(v_of(n, s2, t), p[s2], o[t]);
+                for (int t = 0; t < ND; t++) {
+                    const half8v v = v_of(n, s2, t);
+                    o[t] = mfma32(v, lo[s2], o[t]);
+                    o[t] = mfma32(v, hi[s2], o[t]);
+                }
         }
     };
     auto seen = [&](int id, int i) { return id < 0 ? 0u : bits_below(len - page_at(i) * kPageCells); };
