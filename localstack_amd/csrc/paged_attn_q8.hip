@@ -198,12 +198,15 @@ __global__ __launch_bounds__(kPaWaves *kWave, HD == 256 ? 2 : 3) void paged_attn
             }
             // The reference r of the weights takes the scales of V in: p d' has to stay below 2^16 as an fp16 operand whatever the
             // scales are, and as far up as it can, so that small weights keep their bits. 2^above is more than any scale of the page.
+            // Among scores whose neighbours lie far apart a sum with `above` may be rounded up by a whole step, and the weights be
+            // lost; there they are 1 at most, which a scale may multiply as it is.
             const int above = (int) (vd.most() >> 10) - 14;
             vd.store(s_d[1][wv], lane);
             float top = s[0];
 #pragma unroll
             for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
-            top = fmaxf(m_run, maximum_kept(across_groups_max(top + (float) above)));
+            top = across_groups_max(top);
+            top = fmaxf(m_run, fabsf(top) < kExactTo ? top + ((float) above - kBelow) : top + (float) min(above, 0));
             if (__any(top > m_run)) {
                 const float f = __builtin_amdgcn_exp2f(m_run - top);
                 m_run = top;
