@@ -237,7 +237,8 @@ int lstk_attn_shared_q8(const lstk_prefix *prefix, const lstk_q8_cache *cache, c
  * the probability that softmax gives d_tokens[r]; d_entropy [n_rows] (or NULL), -sum p ln p; and the n_top (at most 32) largest values'
  * ids and log probabilities, d_top_ids and d_top_logprobs [n_rows][n_top], in descending order, equal ones by id. A token outside the
  * vocabulary, or one at -inf, has -inf; a row with fewer than n_top values above -inf has id -1 and -inf in the other places, one with
- * none of them entropy 0. n_vocab is at most 2^20 - 16; the workspace is as lstk_attn_paged's. */
+ * none of them entropy 0. Log probabilities near 0 and small entropies (a token that has nearly all of the probability) keep their relative
+ * precision; a share below 2^-126 of the largest value's counts as 0. n_vocab is at most 2^20 - 16; the workspace is as lstk_attn_paged's. */
 size_t lstk_token_logprobs_work_bytes(int n_rows, int n_vocab, int n_top);
 int lstk_token_logprobs(const float *d_logits, int64_t ld_logits, int n_rows, int n_vocab, const int32_t *d_tokens, int n_top,
                         float *d_logprobs, float *d_entropy, int32_t *d_top_ids, float *d_top_logprobs, void *d_work, size_t work_bytes,

@@ -87,8 +87,8 @@ struct LogpParams {
     float *logp, *entropy; // entropy may be null
     int32_t *top_ids;      // [n_rows][n_top]
     float *top_logp;
-    int slices, slice;     // work-groups per row and values per slice (logp_plan)
-    float *sums;           // [n_rows][slices][4]: max, sum of e^(x - max), sum of (x - max) e^(x - max), unused
+    int slices, slice;     // work-groups per row and 16-byte quads per slice (logp_plan)
+    float *sums;           // [n_rows][slices][4]: max, values alike it, sum of e^(x - max) of the others, sum of (x - max) e^(x - max)
     unsigned long long *best; // [n_rows][slices][n_top] (value, lowest index), largest first
 };
 size_t logp_plan(LogpParams &P, void *work);

@@ -3,6 +3,9 @@
 //   m = max x,  l = sum e^(x - m),  t = sum (x - m) e^(x - m)
 //   log p(i) = x_i - m - ln l,  entropy = ln l - t / l
 //
+// l is held as k + r, k values at the maximum and the sum r of the others, and ln l as log1p(k - 1 + r): beside a nearly certain token the
+// others' share may be far below the last bit of 1, and is what the token's log probability and the entropy consist of.
+//
 // Bound by HBM where there are many rows: 1000 rows of 151936 values (608 MB) 97 us on MI355X, 6.3 TB/s, and 5 us for the join; 64 rows
 // with 20 values each 14 and 6 us, one row with 5 values 5.5 and 4.6 us, bound by waits.
 //
@@ -57,15 +60,16 @@ __device__ __forceinline__ u64 wave_place_max(u64 p) {
 // wave_max gives rows that a DPP step leaves out a 0; here the maxima may be below it
 __device__ __forceinline__ float wave_top(float v) { return of_key(wave_umax(key_of(v))); }
 
-// A row's answers from its sums (m: its largest value).
-__device__ __forceinline__ void answer(const LogpParams &P, int row, float m, double l, double t, double &lse) {
-    lse = m > -INFINITY ? log(l) : 0.0;
+__device__ __forceinline__ double log_sum(double k, double r) { return log1p(k - 1.0 + r); } // ln(k + r), k >= 1
+// A row's answers from its sums (m: its largest value, of which there are k).
+__device__ __forceinline__ void answer(const LogpParams &P, int row, float m, double k, double r, double t, double &lse) {
+    lse = m > -INFINITY ? log_sum(k, r) : 0.0;
     const float *x = P.logits + (int64_t) row * P.ld;
     const int token = P.tokens[row];
     float v = -INFINITY;
     if (token >= 0 && token < P.n_vocab) v = counted(x[token]);
     P.logp[row] = v > -INFINITY ? (float) ((double) v - (double) m - lse) : -INFINITY;
-    if (P.entropy) P.entropy[row] = m > -INFINITY ? (float) (lse - t / l) : 0.0f;
+    if (P.entropy) P.entropy[row] = m > -INFINITY ? (float) (lse - t / (k + r)) : 0.0f;
 }
 __device__ __forceinline__ void alternative(const LogpParams &P, int row, int r, u64 place, float m, double lse) { // place 0: none
     const int64_t at = (int64_t) row * P.n_top + r;
@@ -75,7 +79,7 @@ __device__ __forceinline__ void alternative(const LogpParams &P, int row, int r,
 
 template <int HELD>
 __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
-    __shared__ float s_max[kLpThreads], s_l[kLpWaves], s_t[kLpWaves];
+    __shared__ float s_max[kLpThreads], s_k[kLpWaves], s_r[kLpWaves], s_t[kLpWaves];
     __shared__ unsigned s_bound, s_n;
     __shared__ u64 s_list[kLpList], s_best[kLogpMaxTop], s_place[kLpWaves];
     const int row = blockIdx.x / P.slices, slice = blockIdx.x % P.slices, tid = threadIdx.x, lane = tid & (kWave - 1), wv = tid / kWave;
@@ -110,27 +114,35 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
     s_max[tid] = most;
     if (tid == 0) s_n = 0;
     const float wave_most = wave_top(most);
-    if (lane == 0) s_l[wv] = wave_most;
+    if (lane == 0) s_r[wv] = wave_most;
     __syncthreads();
-    float m = s_l[0];
+    float m = s_r[0];
 #pragma unroll
-    for (int w = 1; w < kLpWaves; w++) m = fmaxf(m, s_l[w]);
+    for (int w = 1; w < kLpWaves; w++) m = fmaxf(m, s_r[w]);
     __syncthreads();
-    float l = 0.0f, t = 0.0f;
+    float k = 0.0f, r = 0.0f, t = 0.0f;
     if (m > -INFINITY) {
 #pragma unroll
         for (int h = 0; h < HELD; h++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float d = fmaxf(v[h][e] - m, kFar), w = __builtin_amdgcn_exp2f(d * kLog2e);
-                l += w;
+                const float d = fmaxf(v[h][e] - m, kFar), w = d < 0.0f ? __builtin_amdgcn_exp2f(d * kLog2e) : 0.0f;
+                r += w;
                 t = fmaf(d, w, t);
             }
+        if (most == m) { // few threads have any
+#pragma unroll
+            for (int h = 0; h < HELD; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) k += v[h][e] == m ? 1.0f : 0.0f;
+        }
     }
-    l = wave_sum_tree(l);
+    k = wave_sum_tree(k);
+    r = wave_sum_tree(r);
     t = wave_sum_tree(t);
     if (lane == 0) {
-        s_l[wv] = l;
+        s_k[wv] = k;
+        s_r[wv] = r;
         s_t[wv] = t;
     }
     if (P.n_top > 0 && wv == 0) {
@@ -148,17 +160,18 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
         if (lane == 0) s_bound = bound;
     }
     __syncthreads();
-    double L = 0.0, T = 0.0;
+    double K = 0.0, R = 0.0, T = 0.0;
 #pragma unroll
     for (int w = 0; w < kLpWaves; w++) {
-        L += s_l[w];
+        K += s_k[w];
+        R += s_r[w];
         T += s_t[w];
     }
     const int64_t part = (int64_t) row * P.slices + slice;
     double lse = 0.0;
     if (tid == 0) {
-        if (P.slices > 1) *reinterpret_cast<float4 *>(P.sums + 4 * part) = make_float4(m, (float) L, (float) T, 0.0f);
-        else answer(P, row, m, L, T, lse);
+        if (P.slices > 1) *reinterpret_cast<float4 *>(P.sums + 4 * part) = make_float4(m, (float) K, (float) R, (float) T);
+        else answer(P, row, m, K, R, T, lse);
     }
     if (P.n_top == 0) return;
     const float bound = s_bound > key_of(-INFINITY) ? of_key(s_bound) : -INFINITY; // (keys below are those of NaN)
@@ -205,7 +218,7 @@ __global__ __launch_bounds__(kLpThreads) void logp_slice_kernel(LogpParams P) {
     __syncthreads();
     if (tid >= P.n_top) return;
     if (P.slices > 1) P.best[part * P.n_top + tid] = s_best[tid];
-    else alternative(P, row, tid, s_best[tid], m, m > -INFINITY ? log(L) : 0.0);
+    else alternative(P, row, tid, s_best[tid], m, m > -INFINITY ? log_sum(K, R) : 0.0);
 }
 
 __global__ __launch_bounds__(kLpThreads) void logp_join_kernel(LogpParams P) {
@@ -224,16 +237,21 @@ __global__ __launch_bounds__(kLpThreads) void logp_join_kernel(LogpParams P) {
         float4 s = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         if (lane < P.slices) s = *reinterpret_cast<const float4 *>(P.sums + 4 * ((int64_t) row * P.slices + lane));
         const float m = wave_top(s.x);
-        double l = 0.0, t = 0.0, lse;
-        if (s.x > -INFINITY) {
+        double k = 0.0, r = 0.0, t = 0.0, lse;
+        if (s.x == m) {
+            k = s.y;
+            r = s.z;
+            t = s.w;
+        } else if (s.x > -INFINITY) {
             const double d = (double) s.x - (double) m, w = exp(d);
-            l = w * s.y;
-            t = w * s.z + d * l;
+            r = w * ((double) s.y + (double) s.z);
+            t = w * s.w + d * r;
         }
-        l = wave_sum_d(l);
+        k = wave_sum_d(k);
+        r = wave_sum_d(r);
         t = wave_sum_d(t);
         if (lane == 0) {
-            answer(P, row, m, l, t, lse);
+            answer(P, row, m, k, r, t, lse);
             s_lse = lse;
             s_m = m;
             s_n = 0;
