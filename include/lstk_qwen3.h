@@ -198,8 +198,10 @@ typedef struct lstk_q8_cache {
 } lstk_q8_cache;
 /* store: quantises n_rows (at most 2^24) rows of K and V, [n_rows][n_head_kv][head_dim] of type LSTK_TYPE_F16 or LSTK_TYPE_F32, as they
  * are written to the cells d_cells [n_rows]. load: reads the rows of these cells back, rounded to fp16, or exact in f32. Row r is at
- * d_k + r * ld_k and d_v + r * ld_v (in values; multiples of 8; pointers 16-byte aligned). A cell outside the cache is left alone by
- * store, its row zeros in load. The cells of one store must differ: a cell that several rows name holds bytes of more than one of
+ * d_k + r * ld_k and d_v + r * ld_v (in values; multiples of 8; pointers 16-byte aligned). d is rounded up, so d q can lie past the
+ * value that it stands for, and past fp16's range, where load to fp16 gives an infinity: of fp16 rows, values of 65280 and more in a block
+ * whose largest is 65472 or 65504 (d = 516, 127 d = 65532); load to f32 gives 65532. A cell outside the cache is left alone by store, its
+ * row zeros in load. Rows times heads are bounded by one launch: (n_rows + 38) / 32 (whole) times n_head_kv below 2^22. The cells of one store must differ: a cell that several rows name holds bytes of more than one of
  * them afterwards. Other cells keep every bit. */
 int lstk_cache_q8_store(const lstk_q8_cache *cache, const void *d_k, const void *d_v, int type, int64_t ld_k, int64_t ld_v,
                         const int32_t *d_cells, int n_rows, lstk_stream_t stream);

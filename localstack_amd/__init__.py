@@ -612,7 +612,8 @@ def store_q8(cache, k, v, cells, stream=None):
 
 def load_q8(cache, cells, dtype=None, k=None, v=None, stream=None):
     """The rows of these cells (int32 [n]; zeros for one outside the cache) as (k, v), each [n][n_head_kv][head_dim] of `dtype`
-    (float16, or float32, which is exact): lstk_cache_q8_load. k, v: where they go, rows may be strided."""
+    (float16, infinities where the cache holds more than fp16 can, as it may for a value of 65280 or more; or float32, which is exact):
+    lstk_cache_q8_load. k, v: where they go, rows may be strided."""
     import torch
     c, dev = _q8(cache)
     at = _tensor(cells, "cells", torch.int32, (None,), dev)
