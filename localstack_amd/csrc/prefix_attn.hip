@@ -25,6 +25,8 @@ namespace lstk {
 namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kPxRows = 32;   // query rows of a wavefront
 constexpr int kPxTiles = 4;   // wavefronts that share a page
@@ -73,6 +75,8 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, HD < 256 ? 2 : 1)
         uint2 a = *reinterpret_cast<const uint2 *>(src), b = *reinterpret_cast<const uint2 *>(src + 8);
         q[i] = halves(a.x ^ turn, a.y ^ turn, b.x ^ turn, b.y ^ turn);
     }
+    float minus = -1.0f; // kept from the compiler: p - hi is one instruction as an fma of fp16 numbers, three as a difference
+    asm("" : "+v"(minus));
     float m_run = kLowest, l_run = 0.0f; // of row `col`; the sum of this lane's cells
     float16v o[ND];                      // o[t][i]: dim 32 t + 8 (i / 4) + 4 h + i % 4
 #pragma unroll
@@ -146,11 +150,16 @@ __global__ __launch_bounds__((px_waves<HD, SHARED>()) * kWave, HD < 256 ? 2 : 1)
         for (int n = 0; n < NP; n++) {
             half8v hi[2], lo[2];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = __builtin_amdgcn_exp2f(s[n][i]);
-                hi[i / 8][i % 8] = (_Float16) p;
-                lo[i / 8][i % 8] = (_Float16) (p - (float) hi[i / 8][i % 8]);
-                l_run += p;
+            for (int i = 0; i < 16; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(s[n][i]), p1 = __builtin_amdgcn_exp2f(s[n][i + 1]);
+                const half2v h = __builtin_convertvector(float2v{p0, p1}, half2v);
+                const half2v r = __builtin_convertvector(float2v{fmaf((float) h[0], minus, p0), fmaf((float) h[1], minus, p1)}, half2v);
+                hi[i / 8][i % 8] = h[0];
+                hi[i / 8][i % 8 + 1] = h[1];
+                lo[i / 8][i % 8] = r[0];
+                lo[i / 8][i % 8 + 1] = r[1];
+                l_run += p0;
+                l_run += p1;
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; s2++)
