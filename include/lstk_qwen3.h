@@ -221,7 +221,8 @@ int lstk_attn_paged_q8(const lstk_q8_cache *cache, const lstk_paged_seqs *seqs, 
  * A row without a visible cell gets zeros. A weight enters the sums (fp32) as two fp16 parts, over the prefix as over own cells: good to
  * 2^-22 (over the prefix to 2^-37 of the largest where it is below 2^-15 of it). The workspace is as lstk_attn_paged's; one size serves
  * both kinds of caches, and smaller lengths and prefixes.
- * Worth it from some 8 sequences and 1000 cells on: it takes a launch more than attention over lists that begin alike. */
+ * It takes a launch more than lstk_attn_paged over lists that begin alike, which caches serve well while the prefix is short: at 32 heads
+ * on 4 of 128 it is faster from 4 sequences on 16000 cells, 8 on 8000 and 32 on 2000 on, and not on 1000 cells for up to 128 sequences. */
 typedef struct lstk_prefix {
     const lstk_paged_cache *cache;
     int32_t max_len;         /* bound of the length: sizes the launch and the workspace */

@@ -1,5 +1,6 @@
-// batch.h - launchers of the operators of a decode step of many sequences: attention of one new token per
-// sequence over the paged cache (paged_attn.hip), sampling (sample.hip) and routing by a rule (select.hip).
+// batch.h - launchers of the operators of a decode step of many sequences: attention of one new token per sequence over the paged
+// cache in fp16 (paged_attn.hip) or 8 bits (paged_attn_q8.hip) and over a prefix that they share (prefix_attn.hip), rows into and out of
+// the 8-bit cache (cache_q8.hip), log probabilities (logp.hip), sampling (sample.hip) and routing by a rule (select.hip).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -7,7 +7,7 @@
 // others' share may be far below the last bit of 1, and is what the token's log probability and the entropy consist of.
 //
 // Bound by HBM where there are many rows: 1000 rows of 151936 values (608 MB) 97 us on MI355X, 6.3 TB/s, and 5 us for the join; 64 rows
-// with 20 values each 14 and 6 us, one row with 5 values 5.5 and 4.6 us, bound by waits.
+// with 20 values each 15 and 6 us, one row with 5 values 5.8 and 4.7 us, bound by waits.
 //
 // A row is read once: a work-group holds a slice of it in registers (kLpThreads * HELD quads), so the maximum is known before the
 // sums are taken, and the largest values can be looked for afterwards. The n-th largest of the threads' own maxima is a bound

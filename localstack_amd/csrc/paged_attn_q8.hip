@@ -22,7 +22,8 @@ namespace {
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
 
-// Eight signed bytes as fp16: the byte with its sign bit flipped, under the exponent of 1024, is 1152 more than the number.
+// Eight signed bytes as fp16, by the well-known way of writing a small whole number into the mantissa: the byte with its sign bit
+// flipped, under the exponent of 1024, is 1152 more than the number.
 __device__ __forceinline__ half8v wide(unsigned a, unsigned b) {
     const half2v less = {(_Float16) 1152.0f, (_Float16) 1152.0f};
     unsigned r[4];

@@ -111,7 +111,9 @@ __device__ __forceinline__ Share share_of(const PagedAttnParams &P, int tasks, K
     s.total = uniform(s.total * tasks);
     // Small shares are whole rounds of the wavefronts, so that few sequences have fewer parts to join. Us a call so and without, with
     // room for 131072 cells: one sequence of 5000 cells 14.1 and 15.9, four of 200 to 3000 at 64 heads on 4 13.8 and 15.8; but 24
-    // of 100 to 1500 18.4 and 16.8, 24 of 45 to 500 at 16 on 2 of 256 17.1 and 14.5; larger calls differ by 2% or less.
+    // of 100 to 1500 18.4 and 16.8, 24 of 45 to 500 at 16 on 2 of 256 17.1 and 14.5; larger calls differ by 2% or less. Over the 8-bit
+    // cache, whose work-groups are three a CU: 14.1 and 16.9, 14.0 and 16.1, 17.2 and 17.2, 18.6 and 16.4; 24 of 100 to 4100 with no
+    // spare room 23.5 and 22.2 (9 pages a share become 12, and a third of the work-groups have none); larger calls differ by 1%.
     s.each = (s.total + gridDim.x - 1) / gridDim.x;
     if (s.each <= kPaRound * kPaWaves) s.each = (s.each + kPaWaves - 1) / kPaWaves * kPaWaves;
     const int64_t lo = s.each * blockIdx.x;

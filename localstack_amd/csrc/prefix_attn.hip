@@ -4,18 +4,20 @@
 // row block and not once a sequence:
 //   S^T = K Q^T,  p = 2^(s - m),  O^T += V^T P^T,  l += sum p       (m: a row's running reference, s in units of log 2)
 // over a share of the prefix's pages; what a share leaves (m, l, O) goes to `part` and is joined where a sequence's own cells are
-// done (take_prefix, paged_parts.h).
+// done (write_part, paged_parts.h) or by the launch that joins parts.
 //
 // A page (32 cells) is the A operand of 32 x 32 x 16 fp16 matrix instructions, 32 query rows the B operand: HD / 16 of them for S^T,
-// as many for O^T. Their results leave a lane with 16 cells of one row, 8 in a row of each half of the page, which is what it needs
-// of the operand P: nothing is moved between the products.
+// twice as many for O^T, whose P enters as two fp16 parts. Their results leave a lane with 16 cells of one row, 8 in a row of each half
+// of the page, which is what it needs of the operand P: nothing is moved between the products. One part a
+// weight took 101 us where two take 121 (the long prefix below), but is off by 2^-12 of the weight and not 2^-22, which values that nearly
+// cancel bring out.
 //
 // Many rows: four wavefronts (128 rows) share a page in LDS, two such groups a work-group, two pages a turn; few rows (up to 64): each
-// wavefront takes a page of its own from memory to registers. Measured on MI355X at 1024 rows a KV head, 4 KV heads of 128: 8000 cells 37
-// us, 30001 100 us (629 TFLOP/s; 85 us of it at 740, the rest the way to the first page and 17 MB of parts). In variants with pieces left
-// out the products alone took 56 us, all else alone 68, each with some 14 that are there without any page: the vector units, LDS (16 KB a wavefront and page, at 280 bytes a ns and CU) and the
-// matrix units hardly overlap, with two wavefronts a SIMD or three, in step or not. The work-groups of the same pages run on one XCD,
-// whose L2 then has 86% of the reads.
+// wavefront takes a page of its own from memory to registers. Measured on MI355X at 1024 rows a KV head, 4 KV heads of 128: 8000 cells 43
+// us, 30001 121 us (520 TFLOP/s of the sums' flops; some 15 us of it are the way to the first page and 17 MB of parts). Of 217 k busy cycles
+// there the vector units take 93 k, the matrix units 91 k and LDS (16 KB a wavefront and page, at 280 bytes a ns and CU) 78 k: the three
+// hardly overlap, with two wavefronts a SIMD or three, in step or not. The work-groups of the same pages run on one XCD, whose L2 then has
+// 86% of the reads.
 #include <type_traits>
 
 #include "device.h"
